@@ -104,7 +104,8 @@ class _Operand:
     """A torch tensor handed to the operators: they take anything with a device pointer and a length."""
 
     def __init__(self, t: torch.Tensor):
-        self.t, self.ptr, self.n = t, t.data_ptr(), t.numel()
+        self.t, self.ptr = t, t.data_ptr()
+        self.n = 1 + sum((size - 1) * step for size, step in zip(t.shape, t.stride()))  # from its first element to its last
 
     def __len__(self):
         return self.n
