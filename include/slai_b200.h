@@ -31,6 +31,7 @@ typedef struct slai_ctx slai_ctx;         /* LlmOps<B> + backend + one stream (c
 typedef struct slai_qmatrix slai_qmatrix; /* GpuQuantMatrix<B> (quantized_matrix.rs:11-22)            */
 typedef struct slai_llama slai_llama;     /* Llama2State + Llama2Weights (models/llama2/transformer.rs) */
 typedef struct slai_gpt2 slai_gpt2;       /* Gpt2Model (models/gpt2/cpu.rs:66-112)                    */
+typedef struct slai_paged slai_paged;     /* keys and values in pages (the reference has one dense cache, transformer.rs:87-106) */
 typedef struct slai_tp slai_tp;           /* tensor-parallel group (no counterpart in the reference)  */
 
 enum slai_status {
@@ -263,6 +264,57 @@ int slai_attention_static(slai_ctx* ctx, const slai_attn_params* p, const float*
  * GEMVs write into `key_cache.column(pos)` directly, transformer.rs:329-334). */
 int slai_kv_append(slai_ctx* ctx, void* d_key_cache, void* d_value_cache, int kv_dtype, const float* d_k,
                    const float* d_v, int kv_dim, int pos);
+
+/* ---- keys and values in pages -------------------------------------------------------------------------
+ * The reference keeps one sequence in one dense cache (models/llama2/transformer.rs:16-44,87-106).  A host that serves many sequences of
+ * lengths it does not know beforehand keeps them in pages: `n_pages` pages of `page_size` positions, which it hands to sequences as they grow.  The
+ * buffers are the caller's (one pair per layer, all of the same shape); a handle holds what is common to a model's layers and the current step.
+ *
+ * slai_paged_step describes a step: sequence b has h_pos0[b] positions cached and h_n_new[b] new tokens behind them (one while it answers, a chunk of its
+ * prompt before that; 0: it takes no part), and row b of h_tables ([n_seq][table_ld], table_ld >= the pages in use) names the pages of positions
+ * 0 .. h_pos0 + h_n_new - 1 in order.  The step's rows (of q, k, v and of the results) are the new tokens, sequence after sequence.  Lengths and tables are
+ * checked on the host (SLAI_ERR_SHAPE; the step before stays in force): capacity, page numbers, and that a page which gets new tokens is used once (pages that
+ * are only read may be shared).  The call copies the tables and returns; it serves every layer until the next step.  It cannot be recorded: a recorded
+ * append or attention (slai_pass_*) reads the step that is current when it runs, up to the handle's capacity.
+ * One handle is used on one context's stream.  Destroy handles before their context. */
+typedef struct slai_paged_config {
+    int32_t n_q_heads, n_kv_heads, head_size; /* n_kv_heads divides n_q_heads; head_size 1 .. 256 */
+    int32_t page_size, n_pages, kv_dtype;     /* slai_kv_dtype */
+    int32_t max_seqs, max_tokens, max_table;  /* capacity of a step: sequences, new tokens, table entries in use */
+} slai_paged_config;
+/* A layer's pages.  Element e of cache head h at place s of page p is d_keys[p * page_stride + h * head_stride + s * pos_stride + e]; strides in
+ * elements, each at least head_size: position-major pages as in the reference's cache, head-major ones, or anything between. */
+typedef struct slai_paged_layer {
+    void* d_keys;
+    void* d_values;
+    int64_t page_stride, head_stride, pos_stride;
+} slai_paged_layer;
+int slai_paged_create(slai_ctx* ctx, const slai_paged_config* cfg, slai_paged** out);
+int slai_paged_destroy(slai_paged* p);
+int slai_paged_step(slai_paged* p, int n_seq, const int32_t* h_pos0, const int32_t* h_n_new, const int32_t* h_tables, int64_t table_ld);
+
+/* What happens to q and k between their product and the attention.  Per head: RmsNorm (ops/rms_norm.rs:35-77) by `head_size` weights where they are given,
+ * then the rotation of its pairs by the token's position (ops/rope.rs:45-85; -1 none, 0 Original, 1 Neox).  Angles keep their digits at any position (the
+ * product is formed in 64 bits; slai_rope's in f32, as in the reference).  Leading dimensions: floats between the rows of two tokens, 0 = packed; q, k and v may
+ * be parts of one product's rows.  An output may be its own input. */
+typedef struct slai_qk_params {
+    int32_t head_size, n_q_heads, n_kv_heads; /* head_size 1 .. 256, even with a rotation */
+    int32_t rope_variant;
+    float rope_base_freq, norm_eps;
+    const float* d_q_norm; /* head_size weights; NULL: queries are not normalised */
+    const float* d_k_norm;
+    int64_t q_ld, k_ld, v_ld, q_out_ld, k_out_ld;
+} slai_qk_params;
+/* Rows of n_tokens tokens, token t at position d_pos[t] (negative: its rows are left as they are).  Either head count may be 0. */
+int slai_qk_norm_rope(slai_ctx* ctx, const slai_qk_params* params, int n_tokens, const int32_t* d_pos, const float* d_q, const float* d_k, float* d_q_out,
+                      float* d_k_out);
+/* The same for the rows of the current step, keys and values going into their pages (slai_kv_append's rounding); q goes to d_q_out (n_q_heads 0: no queries). */
+int slai_paged_append(slai_paged* p, const slai_paged_layer* layer, const slai_qk_params* params, const float* d_q, const float* d_k, const float* d_v,
+                      float* d_q_out);
+/* Causal attention (ops/batched_multiquery_attention.rs:32-156) of the step's tokens: token at position t attends to positions 0 .. t of its sequence, which
+ * are in the pages by then.  Rows of q and out: n_q_heads * head_size floats, q_ld / out_ld apart (0 = packed).  scale 0: 1 / sqrt(head_size).  Sums,
+ * weights and results are f32; f16 keys and values take part as they are cached.  Results do not depend on timing; their last bits may depend on what else is in the step. */
+int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, const float* d_q, int64_t q_ld, float scale, float* d_out, int64_t out_ld);
 
 /* ---- Llama-2 family: Llama2Config (models/llama2/cpu.rs:46-67), Llama2::launch (transformer.rs:316-381) */
 typedef struct slai_llama_config {

@@ -4,7 +4,7 @@
 use std::os::raw::{c_char, c_void};
 
 macro_rules! opaque { ($($n:ident),*) => { $(#[repr(C)] pub struct $n { _private: [u8; 0] })* } }
-opaque!(slai_ctx, slai_qmatrix, slai_llama, slai_gpt2, slai_pass);
+opaque!(slai_ctx, slai_qmatrix, slai_llama, slai_gpt2, slai_pass, slai_paged);
 
 pub const SLAI_OK: i32 = 0;
 pub const SLAI_ERR_INVALID_ARG: i32 = 1;
@@ -35,6 +35,19 @@ pub struct slai_llama_stats_t { pub us_total: f32, pub us: [f32; 7], pub launche
 #[repr(C)]
 #[derive(Copy, Clone, Debug)]
 pub struct slai_gpt2_config { pub n_vocab: i32, pub n_seq: i32, pub n_embd: i32, pub n_head: i32, pub n_layer: i32, pub ff_len: i32, pub layernorm_eps: f32, pub kv_dtype: i32 }
+
+/// Keys and values in pages: geometry and capacity of a handle, a layer's pages, and what happens to q and k (see the C header).
+#[repr(C)]
+#[derive(Copy, Clone, Debug)]
+pub struct slai_paged_config { pub n_q_heads: i32, pub n_kv_heads: i32, pub head_size: i32, pub page_size: i32, pub n_pages: i32, pub kv_dtype: i32,
+    pub max_seqs: i32, pub max_tokens: i32, pub max_table: i32 }
+#[repr(C)]
+#[derive(Copy, Clone, Debug)]
+pub struct slai_paged_layer { pub d_keys: *mut c_void, pub d_values: *mut c_void, pub page_stride: i64, pub head_stride: i64, pub pos_stride: i64 }
+#[repr(C)]
+#[derive(Copy, Clone, Debug)]
+pub struct slai_qk_params { pub head_size: i32, pub n_q_heads: i32, pub n_kv_heads: i32, pub rope_variant: i32, pub rope_base_freq: f32, pub norm_eps: f32,
+    pub d_q_norm: *const f32, pub d_k_norm: *const f32, pub q_ld: i64, pub k_ld: i64, pub v_ld: i64, pub q_out_ld: i64, pub k_out_ld: i64 }
 
 extern "C" {
     pub fn slai_ctx_create(device: i32, out: *mut *mut slai_ctx) -> i32;
@@ -93,6 +106,12 @@ extern "C" {
     pub fn slai_attention(ctx: *mut slai_ctx, p: *const slai_attn_params, d_q: *const f32, d_key_cache: *const c_void, d_value_cache: *const c_void, kv_dtype: i32, d_xb: *mut f32) -> i32;
     pub fn slai_attention_static(ctx: *mut slai_ctx, p: *const slai_attn_params, d_q: *const f32, d_key_cache: *const c_void, d_value_cache: *const c_void, kv_dtype: i32, d_xb: *mut f32) -> i32;
     pub fn slai_kv_append(ctx: *mut slai_ctx, d_key_cache: *mut c_void, d_value_cache: *mut c_void, kv_dtype: i32, d_k: *const f32, d_v: *const f32, kv_dim: i32, pos: i32) -> i32;
+    pub fn slai_paged_create(ctx: *mut slai_ctx, cfg: *const slai_paged_config, out: *mut *mut slai_paged) -> i32;
+    pub fn slai_paged_destroy(p: *mut slai_paged) -> i32;
+    pub fn slai_paged_step(p: *mut slai_paged, n_seq: i32, h_pos0: *const i32, h_n_new: *const i32, h_tables: *const i32, table_ld: i64) -> i32;
+    pub fn slai_qk_norm_rope(ctx: *mut slai_ctx, params: *const slai_qk_params, n_tokens: i32, d_pos: *const i32, d_q: *const f32, d_k: *const f32, d_q_out: *mut f32, d_k_out: *mut f32) -> i32;
+    pub fn slai_paged_append(p: *mut slai_paged, layer: *const slai_paged_layer, params: *const slai_qk_params, d_q: *const f32, d_k: *const f32, d_v: *const f32, d_q_out: *mut f32) -> i32;
+    pub fn slai_paged_attention(p: *mut slai_paged, layer: *const slai_paged_layer, d_q: *const f32, q_ld: i64, scale: f32, d_out: *mut f32, out_ld: i64) -> i32;
     pub fn slai_llama_create(ctx: *mut slai_ctx, cfg: *const slai_llama_config, out: *mut *mut slai_llama) -> i32;
     pub fn slai_llama_destroy(m: *mut slai_llama) -> i32;
     pub fn slai_llama_set_matrix(m: *mut slai_llama, weight_id: i32, layer: i32, w: *const slai_qmatrix) -> i32;

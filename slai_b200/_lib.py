@@ -51,6 +51,20 @@ class Gpt2Config(C.Structure):
                 ("n_layer", C.c_int32), ("ff_len", C.c_int32), ("layernorm_eps", C.c_float), ("kv_dtype", C.c_int32)]
 
 
+class PagedConfig(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_q_heads", "n_kv_heads", "head_size", "page_size", "n_pages", "kv_dtype", "max_seqs", "max_tokens", "max_table")]
+
+
+class PagedLayer(C.Structure):
+    _fields_ = [("d_keys", C.c_void_p), ("d_values", C.c_void_p), ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("pos_stride", C.c_int64)]
+
+
+class QkParams(C.Structure):
+    _fields_ = [("head_size", C.c_int32), ("n_q_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("rope_variant", C.c_int32), ("rope_base_freq", C.c_float),
+                ("norm_eps", C.c_float), ("d_q_norm", C.c_void_p), ("d_k_norm", C.c_void_p), ("q_ld", C.c_int64), ("k_ld", C.c_int64), ("v_ld", C.c_int64),
+                ("q_out_ld", C.c_int64), ("k_out_ld", C.c_int64)]
+
+
 _vp, _i64, _i32, _sz, _f = C.c_void_p, C.c_int64, C.c_int32, C.c_size_t, C.c_float
 _pp = C.POINTER(C.c_void_p)
 
@@ -112,6 +126,12 @@ SIGNATURES = {
     "slai_attention": (C.c_int, [_vp, C.POINTER(AttnParams), _vp, _vp, _vp, C.c_int, _vp]),
     "slai_attention_static": (C.c_int, [_vp, C.POINTER(AttnParams), _vp, _vp, _vp, C.c_int, _vp]),
     "slai_kv_append": (C.c_int, [_vp, _vp, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int]),
+    "slai_paged_create": (C.c_int, [_vp, C.POINTER(PagedConfig), _pp]),
+    "slai_paged_destroy": (C.c_int, [_vp]),
+    "slai_paged_step": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _i64]),
+    "slai_qk_norm_rope": (C.c_int, [_vp, C.POINTER(QkParams), C.c_int, _vp, _vp, _vp, _vp, _vp]),
+    "slai_paged_append": (C.c_int, [_vp, C.POINTER(PagedLayer), C.POINTER(QkParams), _vp, _vp, _vp, _vp]),
+    "slai_paged_attention": (C.c_int, [_vp, C.POINTER(PagedLayer), _vp, _i64, C.c_float, _vp, _i64]),
     "slai_llama_create": (C.c_int, [_vp, C.POINTER(LlamaConfig), _pp]),
     "slai_llama_destroy": (C.c_int, [_vp]),
     "slai_llama_set_matrix": (C.c_int, [_vp, C.c_int, C.c_int, _vp]),

@@ -20,6 +20,12 @@ struct RopeTable {
     float* d_theta;  // head_size/2 inverse frequencies, computed on the host with libm powf
 };
 
+struct TurnTable {
+    int head_size;
+    float base;
+    double* d_turns;  // head_size/2: turns per position of each pair (paged.cu)
+};
+
 // Tensor-parallel exchange over peer memory (tp.cu): every rank owns a region [2 parities][ranks][XCHG_MAX_DIM] of
 // (value, sequence tag) pairs; peers store their partial vectors straight into it over NVLink, one 8-byte store per
 // element, and the reader knows an element has arrived when its tag equals the exchange's sequence number.
@@ -43,6 +49,7 @@ struct slai_ctx {
     size_t scratch_bytes = 0;
     std::vector<void*> retired_scratch;  // outgrown scratch buffers: recorded passes may still point at them, freed with the context
     std::vector<RopeTable> rope_tables;
+    std::vector<TurnTable> turn_tables;
     unsigned long long* trace_buf = nullptr;  // trace build only: per-block stamps of the last 64 GEMV launches
     unsigned long long trace_launches = 0;
     unsigned long long* tl = nullptr;         // trace build only: the launch timeline

@@ -82,6 +82,7 @@ SLAI_API int slai_ctx_destroy(slai_ctx* ctx) {
     SLAI_ENTER(ctx);
     cudaStreamSynchronize(ctx->stream);
     for (auto& t : ctx->rope_tables) cudaFree(t.d_theta);
+    for (auto& t : ctx->turn_tables) cudaFree(t.d_turns);
     if (ctx->d_scratch) cudaFree(ctx->d_scratch);
     for (void* p : ctx->retired_scratch) cudaFree(p);
     if (ctx->d_counters) cudaFree(ctx->d_counters);

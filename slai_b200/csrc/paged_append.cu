@@ -1,0 +1,124 @@
+// What happens to a step's q, k and v between their product and the attention, in one pass: RmsNorm of every head of q and k
+// (y = x * rsqrt(mean x^2 + eps) * w), rotation of its pairs by the token's position, keys and values into the pages of their sequences.  (The reference does
+// the parts as operators of their own: crates/slai/src/ops/rms_norm.rs:35-77, ops/rope.rs:45-85, key_cache.column(pos) at
+// models/llama2/transformer.rs:329-334.)
+//
+// The angle of pair i at position p is p * base^(-2i / hs): far into a long context its f32 value has lost the digits that matter (at position 120000 it is off
+// by up to 0.008), so the turns p * base^(-2i / hs) / 2 pi are formed in 64 bits, the whole ones dropped, and the rest goes to sincospi in f32.
+#include "paged.cuh"
+
+namespace {
+
+constexpr int QT = 256;
+
+// cos and sin of pair i at position p
+__device__ __forceinline__ float2 turn(const double* turns, int i, int p) {
+    const double t = (double)p * turns[i];
+    float s, c;
+    sincospif((float)(2.0 * (t - rint(t))), &s, &c);
+    return make_float2(c, s);
+}
+
+// A head of one token: where it comes from and goes to.
+struct Head {
+    const float* in;
+    float* out;         // f32 result, or
+    char* cache;        // place in the cache (bytes)
+    const float* norm;
+    bool turn;
+};
+__device__ __forceinline__ Head head_of(const QkArgs& A, int row, int slot, int h) {
+    Head H = {nullptr, nullptr, nullptr, nullptr, A.turns != nullptr};
+    if (h < A.n_q) {
+        H.in = A.q + row * A.q_ld + (long long)h * A.hs;
+        H.out = A.q_out + row * A.q_out_ld + (long long)h * A.hs;
+        H.norm = A.q_norm;
+        return H;
+    }
+    const int kv = (h - A.n_q) % A.n_kv;
+    const bool value = h >= A.n_q + A.n_kv;
+    H.in = value ? A.v + row * A.v_ld + (long long)kv * A.hs : A.k + row * A.k_ld + (long long)kv * A.hs;
+    H.norm = value ? nullptr : A.k_norm;
+    if (value) H.turn = false;
+    if (A.v) {
+        const paged::Cache& c = A.cache;
+        const int page = slot / c.page_size;
+        H.cache = (value ? c.values : c.keys) + (A.kv_f16 ? 2 : 4) * (page * c.page_stride + kv * c.head_stride + (slot - page * c.page_size) * c.pos_stride);
+    } else {
+        H.out = A.k_out + row * A.k_out_ld + (long long)kv * A.hs;
+    }
+    return H;
+}
+
+// Any head size and alignment: a warp takes one head of one token.
+__global__ void __launch_bounds__(QT) qk_any_kernel(const QkArgs A) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int heads = A.n_q + (A.v ? 2 : 1) * A.n_kv, lane = threadIdx.x & 31;
+    const long long w = (long long)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
+    if (w >= (long long)A.rows * heads) return;
+    const int row = (int)(w / heads), h = (int)(w - (long long)row * heads);
+    if (A.counted && row >= __ldcg(A.cache.plan + A.cache.count_at)) return;
+    const int2 ps = A.v ? __ldcg(reinterpret_cast<const int2*>(A.cache.plan + A.cache.rows_at) + row) : make_int2(__ldcg(A.pos + row), 0);
+    if (ps.x < 0) return;
+    const Head H = head_of(A, row, ps.y, h);
+    // pairs (lane + 32 j) of the head (variant 0: elements 2i, 2i + 1; else i, i + hs / 2), then the last element of an odd head
+    const int half = A.hs / 2;
+    float x[4][2], last = 0.f, ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int i = lane + 32 * j;
+        x[j][0] = x[j][1] = 0.f;
+        if (i < half) {
+            x[j][0] = __ldcg(H.in + (A.variant == 0 ? 2 * i : i));
+            x[j][1] = __ldcg(H.in + (A.variant == 0 ? 2 * i + 1 : i + half));
+        }
+        ss = fmaf(x[j][0], x[j][0], fmaf(x[j][1], x[j][1], ss));
+    }
+    const bool odd = (A.hs & 1) && lane == 0;
+    if (odd) {
+        last = __ldcg(H.in + A.hs - 1);
+        ss = fmaf(last, last, ss);
+    }
+    if (H.norm) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = rsqrtf(ss / (float)A.hs + A.eps);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int i = lane + 32 * j;
+            if (i < half) {
+                x[j][0] = x[j][0] * r * H.norm[A.variant == 0 ? 2 * i : i];
+                x[j][1] = x[j][1] * r * H.norm[A.variant == 0 ? 2 * i + 1 : i + half];
+            }
+        }
+        if (odd) last = last * r * H.norm[A.hs - 1];
+    }
+    __syncwarp();
+    auto put = [&](int e, float y) {
+        if (H.out) H.out[e] = y;
+        else if (A.kv_f16) reinterpret_cast<__half*>(H.cache)[e] = __float2half_rn(y);
+        else reinterpret_cast<float*>(H.cache)[e] = y;
+    };
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int i = lane + 32 * j;
+        if (i >= half) continue;
+        float2 cs = make_float2(1.f, 0.f);
+        if (H.turn) cs = turn(A.turns, i, ps.x);
+        const float a = H.turn ? x[j][0] * cs.x - x[j][1] * cs.y : x[j][0], b = H.turn ? x[j][0] * cs.y + x[j][1] * cs.x : x[j][1];
+        put(A.variant == 0 ? 2 * i : i, a);
+        put(A.variant == 0 ? 2 * i + 1 : i + half, b);
+    }
+    if (odd) put(A.hs - 1, last);
+}
+
+}  // namespace
+
+int qk_launch(slai_ctx* ctx, QkArgs& A, bool pdl) {
+    const long long heads = A.n_q + (A.v ? 2 : 1) * A.n_kv, warps = (long long)A.rows * heads;
+    if (warps == 0) return SLAI_OK;
+    const long long blocks = (warps + QT / 32 - 1) / (QT / 32);
+    SLAI_REQUIRE(ctx, blocks <= 0x7fffffffll, SLAI_ERR_SHAPE, "rows: too many (%d tokens of %lld heads)", A.rows, heads);
+    return launch_dependent(ctx, qk_any_kernel, dim3((unsigned)blocks), QT, 0, pdl, A);
+}

@@ -1,0 +1,232 @@
+// The host's side of a step over a paged cache: checks of lengths and page tables, and who computes what.  Plain C++ (the tests compile it by itself).
+//
+// A sequence's rows of the step's attention are (token, query head of the group) pairs, one cache head at a time: rows [R i, R i + R) of them are a
+// tile.  A tile's work is its positions, 0 .. the last one its last row sees, in units of `unit` positions; the units of all (tile, cache head) pairs stand
+// in one line, tile by tile and head by head, and a block takes an equal share of that line, from somewhere in one pair to somewhere in another.  So
+// one long sequence and many short ones keep all SMs equally long; a pair that lies on several blocks leaves partial results (two a block at most),
+// which the block that comes last joins in the order of their positions.
+#pragma once
+#include <stdint.h>
+
+#include <algorithm>
+#include <string>
+#include <vector>
+
+namespace paged {
+
+struct Config {
+    int n_q_heads, n_kv_heads, head_size, page_size, n_pages, kv_dtype;
+    int max_seqs, max_tokens, max_table;
+};
+
+// What a kernel reads.  All offsets are in ints from the start of the device copy.
+struct Tile {
+    int row0;     // first row (token) of the sequence in q / out
+    int pos0;     // position of that token
+    int first;    // first packed row of the tile (token first / group, head first % group)
+    int rows;     // packed rows of the tile
+    int table;    // page table of the sequence
+    int units;    // of one cache head
+    int line;     // place in the line of the tile's first unit
+    int pad;
+};
+struct Start {  // where a block begins
+    int tile, head, unit, count;   // count: units of the block
+    Tile t;                        // tiles[tile]
+    int tiles;                     // offset of the tiles
+    int units, blocks, me;         // of the whole line; blocks that share it
+};
+struct Row {  // a token of the step
+    int pos, slot;  // slot: page * page_size + place in the page
+};
+static_assert(sizeof(Tile) == 32 && sizeof(Start) == 64 && sizeof(Row) == 8, "read as words by the kernels");
+
+struct Lane {  // one of the two kinds of kernel
+    int rows = 0, unit = 0;    // tile height, positions of a unit
+    int blocks = 0;            // most blocks
+    int least = 1;             // units a block has at least, if the line allows it
+};
+
+struct Layout {  // of the device copy, in ints
+    int starts[2], count, rows, dynamic, total;  // count: rows of the step
+};
+inline int tiles_cap(const Config& c, const Lane& l) {
+    return l.blocks ? (int)std::min<long long>(((long long)c.max_tokens * (c.n_q_heads / c.n_kv_heads)) / l.rows + c.max_seqs, 1ll << 30) : 0;
+}
+inline Layout layout(const Config& c, const Lane (&lanes)[2]) {
+    Layout L;
+    L.starts[0] = 0;
+    L.starts[1] = L.starts[0] + lanes[0].blocks * (int)(sizeof(Start) / 4);
+    L.count = L.starts[1] + lanes[1].blocks * (int)(sizeof(Start) / 4);
+    L.rows = L.count + 8;
+    L.dynamic = (L.rows + 2 * c.max_tokens + 7) & ~7;
+    L.total = L.dynamic + ((c.max_table + 7) & ~7) + (tiles_cap(c, lanes[0]) + tiles_cap(c, lanes[1])) * (int)(sizeof(Tile) / 4);
+    return L;
+}
+
+struct Step {
+    int n_rows = -1;          // -1: there has been no step
+    int blocks[2] = {0, 0};   // blocks with work
+    int used = 0;             // ints of the dynamic part
+};
+
+// Why `c` cannot be served, or "".
+inline std::string check_config(const Config& c) {
+    auto bad = [](const char* what, long long v) { return std::string(what) + " (" + std::to_string(v) + ")"; };
+    if (c.n_kv_heads < 1 || c.n_q_heads < 1 || c.n_q_heads > 65536 || c.n_q_heads % std::max(1, c.n_kv_heads)) return "n_kv_heads must divide n_q_heads (" + std::to_string(c.n_q_heads) + " on " + std::to_string(c.n_kv_heads) + ")";
+    if (c.head_size < 1 || c.head_size > 256) return bad("head_size must be 1 .. 256", c.head_size);
+    if (c.page_size < 1 || c.page_size > (1 << 20)) return bad("page_size must be 1 .. 2^20", c.page_size);
+    if (c.n_pages < 1 || (long long)c.n_pages * c.page_size > 0x7fffffffll) return bad("n_pages must be at least 1 and n_pages * page_size below 2^31", c.n_pages);
+    if (c.kv_dtype != 0 && c.kv_dtype != 1) return bad("unknown cache type", c.kv_dtype);
+    if (c.max_seqs < 1 || c.max_seqs > (1 << 20)) return bad("max_seqs must be 1 .. 2^20", c.max_seqs);
+    if (c.max_tokens < 1 || c.max_tokens > (1 << 24)) return bad("max_tokens must be 1 .. 2^24", c.max_tokens);
+    if (c.max_table < 1 || c.max_table > (1 << 28)) return bad("max_table must be 1 .. 2^28", c.max_table);
+    if ((long long)c.max_tokens * (c.n_q_heads / c.n_kv_heads) > 0x7fffffffll / 2) return bad("max_tokens * group is too large", c.max_tokens);
+    return "";
+}
+
+class Planner {
+  public:
+    // `few`: rows a sequence may have (tokens * group) and still go to lane 0; lane 1 may be absent (blocks 0).
+    void init(const Config& c, const Lane& a, const Lane& b, int few) {
+        cfg_ = c;
+        lanes_[0] = a;
+        lanes_[1] = b;
+        few_ = b.blocks ? few : 0x7fffffff;
+        lay_ = layout(cfg_, lanes_);
+        seen_.assign((size_t)c.n_pages, 0);
+    }
+    const Layout& lay() const { return lay_; }
+    const Lane& lane(int i) const { return lanes_[i]; }
+
+    // Sequence b: pos0[b] positions are cached, n_new[b] tokens follow (0: it takes no part); row b of `tables` ([n_seq][ld]) names the pages of positions
+    // 0 .. pos0 + n_new - 1 in order.  Writes the device copy to `out` (lay().total ints) and `step`; returns why not, or "" (nothing is written then).
+    std::string plan(int n_seq, const int32_t* pos0, const int32_t* n_new, const int32_t* tables, int64_t ld, int32_t* out, Step* step) {
+        auto say = [](const char* what, long long b, long long v) { return std::string(what) + " (sequence " + std::to_string(b) + ": " + std::to_string(v) + ")"; };
+        if (n_seq < 0 || n_seq > cfg_.max_seqs) return "n_seq must be 0 .. " + std::to_string(cfg_.max_seqs) + " (" + std::to_string(n_seq) + ")";
+        if (n_seq > 0 && (!pos0 || !n_new || !tables)) return "lengths and tables are missing";
+        const int group = cfg_.n_q_heads / cfg_.n_kv_heads, ps = cfg_.page_size;
+        long long rows = 0, entries = 0, line[2] = {0, 0};
+        for (int b = 0; b < n_seq; b++) {
+            if (pos0[b] < 0) return say("a negative number of cached positions", b, pos0[b]);
+            if (n_new[b] < 0) return say("a negative number of new tokens", b, n_new[b]);
+            if (n_new[b] == 0) continue;
+            const long long held = (long long)pos0[b] + n_new[b], pages = (held + ps - 1) / ps;
+            if (held > 0x7fffffffll - 1024) return say("too many positions", b, held);
+            if (pages > ld) return say("the page table is too narrow", b, ld);
+            rows += n_new[b];
+            entries += pages;
+            if (rows > cfg_.max_tokens) return "more new tokens than max_tokens (" + std::to_string(cfg_.max_tokens) + ")";
+            if (entries > cfg_.max_table) return "more pages than max_table (" + std::to_string(cfg_.max_table) + ")";
+            const int k = lane_of(n_new[b]);
+            for_tiles(b, pos0[b], n_new[b], group, [&](const Tile& t) { line[k] += (long long)t.units * cfg_.n_kv_heads; });
+        }
+        if (line[0] > 0x7fffffffll || line[1] > 0x7fffffffll) return "the step's attention is too large";
+        // Every page exists; one that gets new tokens belongs to its sequence alone, and to one place of it (pages that are only read may be shared).
+        if (++mark_ > 0x3fffffff) {
+            std::fill(seen_.begin(), seen_.end(), 0);
+            mark_ = 1;
+        }
+        const int written = 2 * mark_, read = 2 * mark_ + 1;
+        for (int pass = 0; pass < 2; pass++)
+            for (int b = 0; b < n_seq; b++) {
+                if (n_new[b] == 0) continue;
+                const int32_t* tab = tables + (int64_t)b * ld;
+                const int pages = (int)(((long long)pos0[b] + n_new[b] + ps - 1) / ps), first_new = pos0[b] / ps;
+                for (int i = pass ? first_new : 0; i < (pass ? pages : first_new); i++) {
+                    const int id = tab[i];
+                    if (id < 0 || id >= cfg_.n_pages) return say("no such page", b, id);
+                    if (pass && (seen_[id] == read || seen_[id] == written)) return say("a page that gets new tokens is used twice", b, id);
+                    seen_[id] = pass ? written : read;
+                }
+            }
+        // -- nothing fails from here on --
+        step->n_rows = (int)rows;
+        out[lay_.count] = (int)rows;
+        int* row = out + lay_.rows;
+        int at = lay_.dynamic, r0 = 0;
+        std::vector<int>& tab_at = tmp_;
+        tab_at.assign((size_t)std::max(1, n_seq), 0);
+        for (int b = 0; b < n_seq; b++) {
+            if (n_new[b] == 0) continue;
+            const int32_t* tab = tables + (int64_t)b * ld;
+            const int held = pos0[b] + n_new[b], pages = (held + ps - 1) / ps;
+            tab_at[b] = at;
+            std::copy(tab, tab + pages, out + at);
+            at += pages;
+            for (int i = 0; i < n_new[b]; i++) {
+                const int p = pos0[b] + i;
+                *row++ = p;
+                *row++ = tab[p / ps] * ps + p % ps;
+            }
+        }
+        at = (at + 7) & ~7;
+        for (int k = 0; k < 2; k++) {
+            Tile* tiles = reinterpret_cast<Tile*>(out + at);
+            const int tiles_at = at;
+            int n = 0, so_far = 0;
+            r0 = 0;
+            for (int b = 0; b < n_seq; b++) {
+                if (n_new[b] > 0 && lane_of(n_new[b]) == k)
+                    for_tiles(b, pos0[b], n_new[b], group, [&](Tile t) {
+                        t.row0 = r0;
+                        t.table = tab_at[b];
+                        t.line = so_far;
+                        so_far += t.units * cfg_.n_kv_heads;
+                        tiles[n++] = t;
+                    });
+                r0 += n_new[b];
+            }
+            at += n * (int)(sizeof(Tile) / 4);
+            const long long U = so_far;
+            const int C = (int)std::min<long long>(lanes_[k].blocks, (U + lanes_[k].least - 1) / std::max(1, lanes_[k].least));
+            step->blocks[k] = C;
+            Start* st = reinterpret_cast<Start*>(out + lay_.starts[k]);
+            int tile = 0;
+            for (int c = 0; c < lanes_[k].blocks; c++) {
+                Start s = {};
+                if (c < C) {
+                    const long long lo = U * c / C, hi = U * (c + 1) / C;
+                    while (lo >= tiles[tile].line + (long long)tiles[tile].units * cfg_.n_kv_heads) tile++;
+                    const int in = (int)(lo - tiles[tile].line);
+                    s.tile = tile;
+                    s.head = in / tiles[tile].units;
+                    s.unit = in % tiles[tile].units;
+                    s.count = (int)(hi - lo);
+                    s.t = tiles[tile];
+                    s.tiles = tiles_at;
+                    s.units = (int)U;
+                    s.blocks = C;
+                    s.me = c;
+                }
+                st[c] = s;
+            }
+        }
+        step->used = at - lay_.dynamic;
+        return "";
+    }
+
+  private:
+    int lane_of(int n_new) const { return (long long)n_new * (cfg_.n_q_heads / cfg_.n_kv_heads) <= few_ ? 0 : 1; }
+    template <class F>
+    void for_tiles(int, int pos0, int n_new, int group, F f) const {
+        const Lane& l = lanes_[lane_of(n_new)];
+        const int all = n_new * group;
+        for (int first = 0; first < all; first += l.rows) {
+            Tile t = {};
+            t.pos0 = pos0;
+            t.first = first;
+            t.rows = std::min(l.rows, all - first);
+            const int last = pos0 + (first + t.rows - 1) / group;  // the last position any of its rows sees
+            t.units = last / l.unit + 1;
+            f(t);
+        }
+    }
+    Config cfg_ = {};
+    Lane lanes_[2];
+    Layout lay_ = {};
+    int few_ = 0, mark_ = 0;
+    std::vector<int> seen_, tmp_;
+};
+
+}  // namespace paged

@@ -294,6 +294,81 @@ class BatchedMultiqueryAttentionParams:
         return AttnParams(self.seq_len, self.kv_dim, self.kv_mul, self.n_heads, self.head_size, self.pos)
 
 
+class PagedLayer:
+    """A layer's pages (`slai_paged_layer`): key and value buffers and the strides, in elements, between pages, cache heads and positions."""
+
+    def __init__(self, keys, values, page_stride: int, head_stride: int, pos_stride: int):
+        self.keys, self.values = keys, values  # held: the pages outlive the layer
+        self.c = _lib.PagedLayer(keys.ptr, values.ptr, page_stride, head_stride, pos_stride)
+
+    def span(self, n_pages: int, page_size: int, n_kv_heads: int, head_size: int) -> int:
+        """Elements from the first to the last of all pages."""
+        c = self.c
+        return (n_pages - 1) * c.page_stride + (n_kv_heads - 1) * c.head_stride + (page_size - 1) * c.pos_stride + head_size
+
+
+class PagedKv:
+    """Keys and values of many sequences in pages (`slai_paged`): what a model's layers have in common, and the current step.  The reference's cache is
+    one dense tensor of one sequence (crates/slai/src/models/llama2/transformer.rs:87-106)."""
+
+    def __init__(self, backend: Backend, n_q_heads: int, n_kv_heads: int, head_size: int, page_size: int, n_pages: int, kv_dtype: int = KV_F16,
+                 max_seqs: int = 8, max_tokens: int = 512, max_table: int | None = None):
+        self.backend = backend
+        self.n_q_heads, self.n_kv_heads, self.head_size, self.page_size, self.n_pages = n_q_heads, n_kv_heads, head_size, page_size, n_pages
+        self.kv_dtype, self.max_tokens = kv_dtype, max_tokens
+        self.rows = None  # of the current step
+        cfg = _lib.PagedConfig(n_q_heads, n_kv_heads, head_size, page_size, n_pages, kv_dtype, max_seqs, max_tokens, max_table or max(1, n_pages))
+        h = C.c_void_p()
+        backend.check(backend.lib.slai_paged_create(backend.h, C.byref(cfg), C.byref(h)))
+        self.h = h
+
+    def step(self, pos0, n_new, tables):
+        """Sequence b: `pos0[b]` cached positions, `n_new[b]` new tokens behind them, pages `tables[b]` in order of their positions."""
+        pos0, n_new = np.ascontiguousarray(pos0, dtype=np.int32), np.ascontiguousarray(n_new, dtype=np.int32)
+        tables = np.ascontiguousarray(tables, dtype=np.int32)
+        n = pos0.size
+        if pos0.ndim != 1 or n_new.shape != pos0.shape or tables.ndim != 2 or tables.shape[0] != n:
+            raise SlaiError(_lib.ERR_SHAPE, f"paged step: lengths of {pos0.shape}, {n_new.shape} and tables of {tables.shape}")
+        at = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
+        self.backend.check(self.backend.lib.slai_paged_step(self.h, n, at(pos0), at(n_new), at(tables), tables.shape[1]))
+        self.rows = int(n_new.sum())
+
+    def check_layer(self, layer: PagedLayer):
+        need = layer.span(self.n_pages, self.page_size, self.n_kv_heads, self.head_size)
+        if len(layer.keys) < need or len(layer.values) < need:
+            raise SlaiError(_lib.ERR_SHAPE, f"paged: pages of {len(layer.keys)} and {len(layer.values)} elements, {need} needed")
+
+    def __del__(self):
+        try:
+            if self.backend.h and self.h and not getattr(self.backend, "_recording", False):
+                self.backend.lib.slai_paged_destroy(self.h)
+                self.h = None
+        except Exception:
+            pass
+
+
+class QkNormRope:
+    """`slai_qk_params`: RmsNorm of every head of q and k (where weights are given) and their rotation by position (`variant` None: none).  Leading
+    dimensions: floats between two tokens' rows, 0 = packed."""
+
+    def __init__(self, head_size: int, n_q_heads: int, n_kv_heads: int, variant: RoPEVariant | None = RoPEVariant.Original, base_freq: float = 10000.0,
+                 eps: float = 1e-5, q_norm=None, k_norm=None, q_ld: int = 0, k_ld: int = 0, v_ld: int = 0, q_out_ld: int = 0, k_out_ld: int = 0):
+        for w in (q_norm, k_norm):
+            if w is not None and len(w) != head_size:
+                raise SlaiError(_lib.ERR_SHAPE, f"qk: {len(w)} norm weights for heads of {head_size}")
+        self.norms = (q_norm, k_norm)  # held
+        self.n_q_heads, self.n_kv_heads, self.head_size = n_q_heads, n_kv_heads, head_size
+        self.c = _lib.QkParams(head_size, n_q_heads, n_kv_heads, -1 if variant is None else int(variant), base_freq, eps, _ptr(q_norm).value,
+                               _ptr(k_norm).value, q_ld, k_ld, v_ld, q_out_ld, k_out_ld)
+
+
+def _check_rows(what: str, x, rows: int, width: int, ld: int):
+    """`x` holds `rows` rows of `width` floats, `ld` (0: packed) apart."""
+    need = (rows - 1) * (ld or width) + width if rows > 0 and width > 0 else 0
+    if (0 if x is None else len(x)) < need:
+        raise SlaiError(_lib.ERR_SHAPE, f"{what}: {0 if x is None else len(x)} floats for {rows} rows of {width}, {ld or width} apart")
+
+
 class LlmContext:
     """`LlmContext<'a, B>` (crates/slai/src/context.rs:68-96): one method per operator; work is enqueued on the
     backend's stream (`begin_submission` ... `submit`), nothing blocks until `submit().synchronize()`."""
@@ -389,6 +464,32 @@ class LlmContext:
 
     def kv_append(self, key_cache, value_cache, k, v, kv_dim: int, pos: int, kv_dtype: int = KV_F32):
         self.backend.check(self.lib.slai_kv_append(self.h, _ptr(key_cache), _ptr(value_cache), kv_dtype, _ptr(k), _ptr(v), kv_dim, pos))
+
+    # Paged caches (the operators they stand beside: RmsNorm, RoPE, key_cache.column(pos), BatchedMultiqueryAttention)
+    def qk_norm_rope(self, how: QkNormRope, positions, q, k, q_out, k_out):
+        """Norm and rotation of the rows of q and k, token t at position positions[t] (int32 on the device; negative: left as it is)."""
+        n, hs = len(positions), how.head_size
+        for what, x, heads, ld in (("q", q, how.n_q_heads, how.c.q_ld), ("q_out", q_out, how.n_q_heads, how.c.q_out_ld),
+                                   ("k", k, how.n_kv_heads, how.c.k_ld), ("k_out", k_out, how.n_kv_heads, how.c.k_out_ld)):
+            _check_rows(f"qk_norm_rope: {what}", x, n, heads * hs, ld)
+        self.backend.check(self.lib.slai_qk_norm_rope(self.h, C.byref(how.c), n, _ptr(positions), _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out)))
+
+    def paged_append(self, paged: PagedKv, layer: PagedLayer, how: QkNormRope, q, k, v, q_out):
+        """The same for the rows of the current step; keys and values go into their pages, q to q_out."""
+        paged.check_layer(layer)
+        n, hs = paged.rows or 0, how.head_size
+        for what, x, heads, ld in (("q", q, how.n_q_heads, how.c.q_ld), ("q_out", q_out, how.n_q_heads, how.c.q_out_ld),
+                                   ("k", k, how.n_kv_heads, how.c.k_ld), ("v", v, how.n_kv_heads, how.c.v_ld)):
+            _check_rows(f"paged_append: {what}", x, n, heads * hs, ld)
+        self.backend.check(self.lib.slai_paged_append(paged.h, C.byref(layer.c), C.byref(how.c), _ptr(q), _ptr(k), _ptr(v), _ptr(q_out)))
+
+    def paged_attention(self, paged: PagedKv, layer: PagedLayer, q, out, scale: float = 0.0, q_ld: int = 0, out_ld: int = 0):
+        """Causal attention of the step's tokens to what their sequences hold (scale 0: 1 / sqrt(head_size))."""
+        paged.check_layer(layer)
+        width = paged.n_q_heads * paged.head_size
+        _check_rows("paged_attention: q", q, paged.rows or 0, width, q_ld)
+        _check_rows("paged_attention: out", out, paged.rows or 0, width, out_ld)
+        self.backend.check(self.lib.slai_paged_attention(paged.h, C.byref(layer.c), _ptr(q), q_ld, scale, _ptr(out), out_ld))
 
     def sample(self, logits: GpuVector, temperature: float, topp: float, coin: float) -> int:
         """`Sampler::sample` (models/sampler.rs:33-54) on the device, the uniform number `coin` given; `logits` is

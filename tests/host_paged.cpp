@@ -1,0 +1,49 @@
+// The planner of a step over a paged cache (csrc/paged_plan.h), for tests/test_paged_plan.py.
+#include <string.h>
+
+#include "../slai_b200/csrc/paged_plan.h"
+
+using namespace paged;
+
+struct Host {
+    Planner p;
+    Config c;
+    std::string why;
+};
+
+extern "C" {
+// cfg: the nine fields of Config; lanes: {rows, unit, blocks, least} twice; returns null and the reason where the configuration is refused
+Host* host_paged_create(const int* cfg, const int* lanes, int few, char* why, int len) {
+    Config c = {cfg[0], cfg[1], cfg[2], cfg[3], cfg[4], cfg[5], cfg[6], cfg[7], cfg[8]};
+    const std::string w = check_config(c);
+    strncpy(why, w.c_str(), len - 1);
+    why[len - 1] = 0;
+    if (!w.empty()) return nullptr;
+    Lane l[2];
+    for (int i = 0; i < 2; i++) {
+        l[i].rows = lanes[4 * i];
+        l[i].unit = lanes[4 * i + 1];
+        l[i].blocks = lanes[4 * i + 2];
+        l[i].least = lanes[4 * i + 3];
+    }
+    Host* h = new Host();
+    h->c = c;
+    h->p.init(c, l[0], l[1], few);
+    return h;
+}
+void host_paged_destroy(Host* h) { delete h; }
+// total ints; offsets of starts[0], starts[1], count, rows, dynamic
+void host_paged_layout(Host* h, int* out) {
+    const Layout& L = h->p.lay();
+    const int v[6] = {L.total, L.starts[0], L.starts[1], L.count, L.rows, L.dynamic};
+    memcpy(out, v, sizeof(v));
+}
+// out: total ints; step: n_rows, blocks[0], blocks[1], used.  Returns the reason ("" = fine).
+const char* host_paged_plan(Host* h, int n, const int* pos0, const int* n_new, const int* tables, long long ld, int* out, int* step) {
+    Step s;
+    h->why = h->p.plan(n, pos0, n_new, tables, ld, out, &s);
+    const int v[4] = {s.n_rows, s.blocks[0], s.blocks[1], s.used};
+    memcpy(step, v, sizeof(v));
+    return h->why.c_str();
+}
+}
