@@ -113,11 +113,112 @@ __global__ void __launch_bounds__(QT) qk_any_kernel(const QkArgs A) {
     if (odd) put(A.hs - 1, last);
 }
 
+// Heads of a multiple of 8 elements on 16-byte boundaries: LPH lanes take a head, 8 elements a lane (two 16-byte pieces that hold four whole pairs in either
+// variant), a warp 32 / LPH * U heads of one token, whose angles it needs once.
+template <int LPH, int U, bool NEOX>
+__global__ void __launch_bounds__(QT) qk_vec_kernel(const QkArgs A) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int HPW = 32 / LPH;
+    const int heads = A.n_q + (A.v ? 2 : 1) * A.n_kv, chunks = (heads + HPW * U - 1) / (HPW * U), lane = threadIdx.x & 31, l = lane % LPH;
+    const long long w = (long long)blockIdx.x * (QT / 32) + (threadIdx.x >> 5);
+    const int row = (int)(w / chunks), h0 = (int)(w - (long long)row * chunks) * HPW * U;
+    if (row >= A.rows || (A.counted && row >= __ldcg(A.cache.plan + A.cache.count_at))) return;
+    const int2 ps = A.v ? __ldcg(reinterpret_cast<const int2*>(A.cache.plan + A.cache.rows_at) + row) : make_int2(__ldcg(A.pos + row), 0);
+    if (ps.x < 0) return;
+    const bool mine = 8 * l < A.hs;
+    const int e0 = NEOX ? 4 * l : 8 * l, e1 = NEOX ? A.hs / 2 + 4 * l : 8 * l + 4;
+    Head H[U];
+    float4 x[U][2];
+#pragma unroll
+    for (int u = 0; u < U; u++) {  // all loads on their way first
+        const int h = h0 + u * HPW + lane / LPH;
+        x[u][0] = x[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (h < heads) {
+            H[u] = head_of(A, row, ps.y, h);
+            if (mine) {
+                x[u][0] = __ldcg(reinterpret_cast<const float4*>(H[u].in + e0));
+                x[u][1] = __ldcg(reinterpret_cast<const float4*>(H[u].in + e1));
+            }
+        }
+    }
+    float2 cs[4];
+    if (A.turns && h0 < A.n_q + A.n_kv) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) cs[i] = mine ? turn(A.turns, 4 * l + i, ps.x) : make_float2(1.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int h = h0 + u * HPW + lane / LPH;
+        float v[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
+        if (A.q_norm || A.k_norm) {  // (the same for all lanes; the sum of a head that is not normalised goes unused)
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss = fmaf(v[i], v[i], ss);
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (h < heads && mine && H[u].norm) {
+                const float r = rsqrtf(ss / (float)A.hs + A.eps);
+                const float4 w0 = __ldg(reinterpret_cast<const float4*>(H[u].norm + e0)), w1 = __ldg(reinterpret_cast<const float4*>(H[u].norm + e1));
+                const float wn[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = v[i] * r * wn[i];
+            }
+        }
+        if (h >= heads || !mine) continue;
+        if (H[u].turn) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float& a = v[NEOX ? i : 2 * i];
+                float& b = v[NEOX ? i + 4 : 2 * i + 1];
+                const float y = a * cs[i].x - b * cs[i].y;
+                b = a * cs[i].y + b * cs[i].x;
+                a = y;
+            }
+        }
+        if (H[u].cache && A.kv_f16) {
+            __half2 p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            __half* d = reinterpret_cast<__half*>(H[u].cache);
+            *reinterpret_cast<uint2*>(d + e0) = *reinterpret_cast<uint2*>(p);
+            *reinterpret_cast<uint2*>(d + e1) = *reinterpret_cast<uint2*>(p + 2);
+        } else {
+            float* d = H[u].out ? H[u].out : reinterpret_cast<float*>(H[u].cache);
+            *reinterpret_cast<float4*>(d + e0) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(d + e1) = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    }
+}
+
+template <int LPH, bool NEOX>
+int launch_vec(slai_ctx* ctx, QkArgs& A, long long heads, bool pdl) {
+    constexpr int HPW = 32 / LPH;
+    auto blocks = [&](int u) { return ((long long)A.rows * ((heads + HPW * u - 1) / (HPW * u)) + QT / 32 - 1) / (QT / 32); };
+    // Several heads a warp where that leaves enough warps to keep the memory busy.
+    const bool many = blocks(4) >= 8 * (ctx->sm_count > 0 ? ctx->sm_count : 148);
+    SLAI_REQUIRE(ctx, blocks(1) <= 0x7fffffffll, SLAI_ERR_SHAPE, "rows: too many (%d tokens of %lld heads)", A.rows, heads);
+    return many ? launch_dependent(ctx, qk_vec_kernel<LPH, 4, NEOX>, dim3((unsigned)blocks(4)), QT, 0, pdl, A)
+                : launch_dependent(ctx, qk_vec_kernel<LPH, 1, NEOX>, dim3((unsigned)blocks(1)), QT, 0, pdl, A);
+}
+
+bool in_vectors(const QkArgs& A) {
+    const int esz = A.kv_f16 ? 2 : 4;
+    uintptr_t b = (uintptr_t)A.q | (uintptr_t)A.k | (uintptr_t)A.v | (uintptr_t)A.q_out | (uintptr_t)A.k_out | (uintptr_t)A.q_norm | (uintptr_t)A.k_norm;
+    b |= (uintptr_t)(4 * (A.q_ld | A.k_ld | A.v_ld | A.q_out_ld | A.k_out_ld));
+    if (A.v) b |= (uintptr_t)A.cache.keys | (uintptr_t)A.cache.values | (uintptr_t)(esz * (A.cache.page_stride | A.cache.head_stride | A.cache.pos_stride));
+    return A.hs % 8 == 0 && (b & 15) == 0;
+}
+
 }  // namespace
 
 int qk_launch(slai_ctx* ctx, QkArgs& A, bool pdl) {
     const long long heads = A.n_q + (A.v ? 2 : 1) * A.n_kv, warps = (long long)A.rows * heads;
     if (warps == 0) return SLAI_OK;
+    if (in_vectors(A)) {
+        if (A.variant == 0) return A.hs <= 64 ? launch_vec<8, false>(ctx, A, heads, pdl) : A.hs <= 128 ? launch_vec<16, false>(ctx, A, heads, pdl) : launch_vec<32, false>(ctx, A, heads, pdl);
+        return A.hs <= 64 ? launch_vec<8, true>(ctx, A, heads, pdl) : A.hs <= 128 ? launch_vec<16, true>(ctx, A, heads, pdl) : launch_vec<32, true>(ctx, A, heads, pdl);
+    }
     const long long blocks = (warps + QT / 32 - 1) / (QT / 32);
     SLAI_REQUIRE(ctx, blocks <= 0x7fffffffll, SLAI_ERR_SHAPE, "rows: too many (%d tokens of %lld heads)", A.rows, heads);
     return launch_dependent(ctx, qk_any_kernel, dim3((unsigned)blocks), QT, 0, pdl, A);
