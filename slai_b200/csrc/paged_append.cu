@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(QT) qk_vec_kernel(const QkArgs A) {
             for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             if (h < heads && mine && H[u].norm) {
                 const float r = rsqrtf(ss / (float)A.hs + A.eps);
-                const float4 w0 = __ldg(reinterpret_cast<const float4*>(H[u].norm + e0)), w1 = __ldg(reinterpret_cast<const float4*>(H[u].norm + e1));
+                const float4 w0 = *reinterpret_cast<const float4*>(H[u].norm + e0), w1 = *reinterpret_cast<const float4*>(H[u].norm + e1);
                 const float wn[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[i] = v[i] * r * wn[i];
