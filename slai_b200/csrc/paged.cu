@@ -72,7 +72,7 @@ int make_handle(slai_ctx* ctx, slai_paged* p) {
     Lane few, many;
     few.rows = 16;
     few.unit = 64;
-    few.blocks = 4 * sms;
+    few.blocks = (paged_attention_few(c.kv_dtype, c.head_size) ? 2 : 4) * sms;
     few.least = 2;
     p->planner.init(c, few, many, 0);
     const size_t bytes = (size_t)p->planner.lay().total * 4;

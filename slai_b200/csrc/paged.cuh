@@ -25,13 +25,14 @@ struct AttnArgs {
     int vec;                 // rows of the cache can be read in 16-byte pieces
     int qvec;                // ... and rows of q and out
     float* part;             // [block][2][tile_rows][hs]: sums of (tile, head) pairs that lie on several blocks
-    float* part_ml;          // [block][2][tile_rows][2]: their maxima and sums of weights
+    float* part_ml;          // [block][2][tile_rows][2]: their largest scores (times log2 e) and sums of weights
     unsigned int* tickets;   // [block], zero between launches
     unsigned int* err_flag;
     unsigned int wait_limit;
 };
 
 #ifdef __CUDACC__
+constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ Start load_start(const int* plan, int starts_at, int block) {
     Start s;
     const int4* g = reinterpret_cast<const int4*>(plan + starts_at) + 4 * (size_t)block;
@@ -72,7 +73,7 @@ __device__ __forceinline__ bool last_to_come(unsigned int* ticket, int n, int* f
     return *flag != 0;
 }
 
-// Rows of a tile: out = sum_i e^(m_i - M) o_i / sum_i e^(m_i - M) l_i over the blocks' results in order of their positions.  A block that saw nothing of a
+// Rows of a tile: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the blocks' results in order of their positions.  A block that saw nothing of a
 // row has m = -inf, l = 0, o = 0.
 template <int THREADS>
 __device__ __forceinline__ void join(const AttnArgs& A, const Tile& t, int head, int first, int last) {
@@ -86,7 +87,7 @@ __device__ __forceinline__ void join(const AttnArgs& A, const Tile& t, int head,
         for (int b = first; b <= last; b++) {
             const size_t slot = ((size_t)b * 2 + (b == first)) * rows + r;
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(A.part_ml) + slot);
-            const float f = ml.x == -INFINITY ? 0.f : expf(ml.x - M);
+            const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
             den = fmaf(f, ml.y, den);
             if (w == 4) {
                 const float4 o = __ldcg(reinterpret_cast<const float4*>(A.part + slot * hs + d));
@@ -104,6 +105,7 @@ __device__ __forceinline__ void join(const AttnArgs& A, const Tile& t, int head,
 
 }  // namespace paged
 
+bool paged_attention_few(int kv_dtype, int hs);
 int paged_attention_launch(slai_ctx* ctx, paged::AttnArgs& A, int kv_dtype, int lane, int blocks, bool pdl);
 
 // paged_append.cu

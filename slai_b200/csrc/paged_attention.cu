@@ -46,7 +46,7 @@ __device__ __forceinline__ void load_rows(const T* base, const long long* place,
 }
 
 template <typename T>
-__global__ void __launch_bounds__(GT) paged_attn_any_kernel(const AttnArgs A) {
+__global__ void __launch_bounds__(GT) paged_attn_any_kernel(const __grid_constant__ AttnArgs A) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Cache& c = A.c;
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(GT) paged_attn_any_kernel(const AttnArgs A) {
                         const int d = 128 * k + 4 * lane + e;
                         if (d < hs) o[d] = acc[i][k][e] * f;
                     }
-                if (!whole && lane == 0) *reinterpret_cast<float2*>(A.part_ml + (slot + g0 + r) * 2) = make_float2(m[i], l[i]);
+                if (!whole && lane == 0) *reinterpret_cast<float2*>(A.part_ml + (slot + g0 + r) * 2) = make_float2(m[i] * LOG2E, l[i]);
             }
         }
         if (!whole) {
@@ -192,10 +192,332 @@ int launch_any(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
     return launch_dependent(ctx, kern, dim3((unsigned)blocks), GT, smem, pdl, A);
 }
 
+// ---- what the matrix units cannot carry ----------------------------------------------------------------------------------
+// The kernels below multiply whole tiles: a weight of zero times an infinite value that its row does not see would be NaN.  A row whose sums are not finite (this,
+// or the formula's own infinities and NaN) is computed again by one warp, position by position: [lo, hi) of the positions, as the formula says.
+template <typename T>
+__device__ __noinline__ void row_again(const AttnArgs& A, const Tile& t, int head, int r, int lo, int hi, float* out, float* ml) {
+    const Cache& c = A.c;
+    const int lane = threadIdx.x & 31, pr = t.first + r, tok = pr / c.group;
+    const float* q = A.q + (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * c.hs;
+    hi = min(hi, t.pos0 + tok + 1);
+    float m = -INFINITY, l = 0.f, acc[8] = {};
+    for (int p0 = lo; p0 < hi; p0 += 32) {
+        const bool seen = p0 + lane < hi;
+        const long long at = seen ? place_of(c, t.table, p0 + lane, head) : 0;
+        float s = 0.f;
+        if (seen)
+            for (int d = 0; d < c.hs; d++) s = fmaf(__ldcg(q + d) * A.scale, to_float<T>(reinterpret_cast<const T*>(c.keys)[at + d]), s);
+        float mt = seen ? s : -INFINITY;
+        for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+        const float m_new = fmaxf(m, mt), resc = m == -INFINITY ? 1.f : expf(m - m_new);
+        const float w = !seen || s == -INFINITY ? 0.f : expf(s - m_new);
+        float ws = w;
+        for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+        l = l * resc + ws;
+        m = m_new;
+        for (int j = 0; j < 8; j++) acc[j] *= resc;
+        for (int i = 0; i < min(32, hi - p0); i++) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const long long ai = __shfl_sync(0xffffffffu, at, i);
+            for (int j = 0; j < 8; j++)
+                if (lane + 32 * j < c.hs) acc[j] = fmaf(wi, to_float<T>(reinterpret_cast<const T*>(c.values)[ai + lane + 32 * j]), acc[j]);
+        }
+    }
+    for (int j = 0; j < 8; j++)
+        if (lane + 32 * j < c.hs) out[lane + 32 * j] = ml ? acc[j] : acc[j] / l;
+    if (ml && lane == 0) *reinterpret_cast<float2*>(ml) = make_float2(m * LOG2E, l);
+}
+
+// ---- PTX wrappers --------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// v = hi + lo, 22 bits
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const __half2 l = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// 2^x, of the sizes weights have
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The power of two that puts a row's largest query below 2^15, and its inverse: whatever their size they fit a pair of halves.
+__device__ __forceinline__ float power_up(float largest, float& unit) {
+    const int e = max((int)(__float_as_uint(largest) >> 23), 15);  // biased by 127
+    unit = __uint_as_float((uint32_t)(e - 14) << 23);
+    return __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
+}
+
+// ---- f16 caches, few rows: tokens of sequences that answer ---------------------------------------------------------------------
+// Up to 16 rows (a token's or a few tokens' query heads of one cache head) are one operand of the matrix instruction.  What such a call costs is reading the
+// cache: each of the block's four warps has a ring of its own of three stages of 16 positions, brought in by asynchronous copies that go around the registers
+// (two stages ahead; the page numbers one stage further), and takes every fourth 16 positions of the block's share with a running maximum and sum of its own;
+// they are joined in shared memory at the end.  Queries and weights are pairs of halves (22 bits), two products each; sums end every 16 positions (the matrix
+// unit truncates when it adds) and go on in registers.
+constexpr int FT = 128, FW = FT / 32, FP = 16, FS = 3;
+template <int HS>
+constexpr int few_smem() { return FW * FS * 2 * FP * HS * 2; }
+
+template <int HS>
+__global__ void __launch_bounds__(FT, 2) paged_attn_few_kernel(const __grid_constant__ AttnArgs A) {
+    constexpr int ROW = HS * 2, CH = HS / 8, TILE = FP * ROW, STAGE = 2 * TILE, KS = HS / 16, NT8 = HS / 8;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    extern __shared__ __align__(128) unsigned char few_sm[];
+    __shared__ float2 ml_s[FW][16];
+    __shared__ unsigned int bad;
+    __shared__ int flag;
+    const Cache& c = A.c;
+    const Start s = load_start(c.plan, A.starts_at, blockIdx.x);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, hs = c.hs, chunks = hs / 8;
+    const uint32_t sm = (uint32_t)__cvta_generic_to_shared(few_sm), ring = sm + warp * FS * STAGE;
+    const char *keys = c.keys, *values = c.values;
+
+    Tile t = s.t;
+    int head = s.head, unit = s.unit, tile = s.tile;
+    for (int left = s.count; left > 0;) {
+        const int n = min(left, t.units - unit);
+        const bool whole = n == t.units;
+        const int lo = unit * A.unit, hi = min((unit + n) * A.unit, t.pos0 + (t.first + t.rows - 1) / c.group + 1);  // positions [lo, hi)
+        const int subs = (hi - lo + FP - 1) / FP, mine = subs > warp ? (subs - warp + FW - 1) / FW : 0;
+        // place of position (lane & 15) of this warp's i-th 16, in bytes; -1 behind the end
+        auto place = [&](int i) -> long long {
+            const int p = lo + (warp + i * FW) * FP + (lane & 15);
+            return i < mine && p < hi ? 2 * place_of(c, t.table, p, head) : -1;
+        };
+        auto request = [&](int i, long long at) {
+            if (i < mine) {
+                const uint32_t dst = ring + (i % FS) * STAGE;
+#pragma unroll
+                for (int k = 0; k < FP * CH / 32; k++) {
+                    const int r = (lane + 32 * k) / CH, ch = lane % CH;
+                    const long long a = __shfl_sync(0xffffffffu, at, r);
+                    const uint32_t off = r * ROW + ((ch ^ (r & 7)) << 4), bytes = a >= 0 && ch < chunks ? 16u : 0u;
+                    const long long src = bytes ? a + 16 * ch : 0;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + off), "l"(__cvta_generic_to_global(keys + src)), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + TILE + off), "l"(__cvta_generic_to_global(values + src)), "r"(bytes) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        {
+            const long long a0 = place(0), a1 = place(1);
+            request(0, a0);
+            request(1, a1);
+        }
+        long long next = place(2);
+
+        // queries: rows g and g + 8
+        uint32_t qh[KS][4], ql[KS][4];
+        float cexp[2];  // the row's scores to powers of two
+        int vis[2];     // last position the row sees
+        {
+            float2 v[KS][4];
+            float mx[2] = {0.f, 0.f};
+            const float* qr[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int r = g + 8 * h, pr = t.first + r, tok = pr / c.group;
+                vis[h] = r < t.rows ? t.pos0 + tok : -1;
+                qr[h] = A.q + (r < t.rows ? (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs : 0);
+            }
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int d = 16 * k + 2 * t4 + 8 * (i >> 1);
+                    v[k][i] = make_float2(0.f, 0.f);
+                    if (vis[i & 1] >= 0 && d < hs) {
+                        if (A.qvec) v[k][i] = __ldcg(reinterpret_cast<const float2*>(qr[i & 1] + d));
+                        else v[k][i] = make_float2(__ldcg(qr[i & 1] + d), __ldcg(qr[i & 1] + d + 1));
+                    }
+                    v[k][i].x *= A.scale;
+                    v[k][i].y *= A.scale;
+                    mx[i & 1] = fmaxf(mx[i & 1], fmaxf(fabsf(v[k][i].x), fabsf(v[k][i].y)));
+                }
+            float up[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                up[h] = power_up(mx[h], cexp[h]);
+                cexp[h] *= LOG2E;
+            }
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) split2(v[k][i].x * up[i & 1], v[k][i].y * up[i & 1], qh[k][i], ql[k][i]);
+        }
+        float acc[NT8][4];
+#pragma unroll
+        for (int i = 0; i < NT8; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m: largest score so far, as a power of two's exponent
+
+        for (int i = 0; i < mine; i++) {
+            request(i + 2, next);
+            next = place(i + 3);
+            asm volatile("cp.async.wait_group 2;" ::: "memory");
+            __syncwarp();
+            const uint32_t ks = ring + (i % FS) * STAGE, vs = ks + TILE;
+            const int p0 = lo + (warp + i * FW) * FP;
+            float sc[2][4];
+#pragma unroll
+            for (int nn = 0; nn < 2; nn++) {
+                float c0[4] = {}, c1[4] = {};
+                uint32_t b[KS / 2][4];
+                const int r = 8 * nn + (lane & 7);
+#pragma unroll
+                for (int k2 = 0; k2 < KS / 2; k2++) ldsm4(ks + r * ROW + (((4 * k2 + (lane >> 3)) ^ (r & 7)) << 4), b[k2]);
+#pragma unroll
+                for (int k = 0; k < KS; k++) mma_f16((k & 1) ? c1 : c0, ql[k], b[k >> 1][2 * (k & 1)], b[k >> 1][2 * (k & 1) + 1]);
+#pragma unroll
+                for (int k = 0; k < KS; k++) mma_f16((k & 1) ? c1 : c0, qh[k], b[k >> 1][2 * (k & 1)], b[k >> 1][2 * (k & 1) + 1]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    sc[nn][e] = (c0[e] + c1[e]) * cexp[e >> 1];
+                    if (p0 + 8 * nn + 2 * t4 + (e & 1) > vis[e >> 1]) sc[nn][e] = -INFINITY;
+                }
+            }
+            float resc[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float mt = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+                const float m_new = fmaxf(m[h], mt), base = m_new == -INFINITY ? 0.f : m_new;
+                resc[h] = ex2(m[h] - base);
+                m[h] = m_new;
+                float ps = 0.f;
+#pragma unroll
+                for (int nn = 0; nn < 2; nn++)
+#pragma unroll
+                    for (int e = 2 * h; e < 2 * h + 2; e++) {
+                        const float p = ex2(sc[nn][e] - base);
+                        ps += p;
+                        sc[nn][e] = p * 4096.f;
+                    }
+                l[h] = l[h] * resc[h] + ps;  // (this lane's positions only)
+            }
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) split2(sc[e >> 1][2 * (e & 1)], sc[e >> 1][2 * (e & 1) + 1], ph[e], pl[e]);
+#pragma unroll
+            for (int n2 = 0; n2 < NT8 / 2; n2++) {
+                float d0[4] = {}, d1[4] = {};
+                uint32_t b[4];
+                const int r = lane & 15;
+                ldsm4t(vs + r * ROW + (((2 * n2 + (lane >> 4)) ^ (r & 7)) << 4), b);
+                mma_f16(d0, pl, b[0], b[1]);
+                mma_f16(d1, pl, b[2], b[3]);
+                mma_f16(d0, ph, b[0], b[1]);
+                mma_f16(d1, ph, b[2], b[3]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    acc[2 * n2][e] = fmaf(acc[2 * n2][e], resc[e >> 1], d0[e]);
+                    acc[2 * n2 + 1][e] = fmaf(acc[2 * n2 + 1][e], resc[e >> 1], d1[e]);
+                }
+            }
+            __syncwarp();  // the stage is requested again next round
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            if (t4 == 0) ml_s[warp][g + 8 * h] = make_float2(m[h], l[h]);
+        }
+        // the warps' sums meet where the stages were (each in its own ring)
+        float* so = reinterpret_cast<float*>(few_sm);
+        constexpr int WF = FS * STAGE / 4;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < NT8; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                *reinterpret_cast<float2*>(so + warp * WF + (g + 8 * h) * HS + 8 * i + 2 * t4) = make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
+        if (tid == 0) bad = 0;
+        __syncthreads();
+        const size_t slot = ((size_t)s.me * 2 + (unit == 0)) * A.tile_rows;
+        for (int i = tid; i < t.rows * (hs / 4); i += FT) {
+            const int r = i / (hs / 4), d = 4 * (i - r * (hs / 4));
+            float M = -INFINITY, den = 0.f, num[4] = {};
+#pragma unroll
+            for (int w = 0; w < FW; w++) M = fmaxf(M, ml_s[w][r].x);
+#pragma unroll
+            for (int w = 0; w < FW; w++) {
+                const float2 x = ml_s[w][r];
+                const float f = x.x == -INFINITY ? 0.f : ex2(x.x - M);
+                const float4 o = *reinterpret_cast<const float4*>(so + w * WF + r * HS + d);
+                den = fmaf(f, x.y, den);
+                num[0] = fmaf(f, o.x, num[0]); num[1] = fmaf(f, o.y, num[1]); num[2] = fmaf(f, o.z, num[2]); num[3] = fmaf(f, o.w, num[3]);
+            }
+            const float sum = num[0] + num[1] + num[2] + num[3] + den;
+            if (!(fabsf(sum) < INFINITY)) atomicOr(&bad, 1u << r);
+            const float f = whole ? 1.f / (den * 4096.f) : 1.f / 4096.f;
+            const int pr = t.first + r, tok = pr / c.group;
+            float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs + d : A.part + (slot + r) * hs + d;
+            if (!whole || A.qvec) {
+                *reinterpret_cast<float4*>(o) = make_float4(num[0] * f, num[1] * f, num[2] * f, num[3] * f);
+            } else {
+                for (int e = 0; e < 4; e++) o[e] = num[e] * f;
+            }
+            if (!whole && d == 0) *reinterpret_cast<float2*>(A.part_ml + (slot + r) * 2) = make_float2(M, den);
+        }
+        __syncthreads();
+        if (bad) {
+            for (int r = warp; r < t.rows; r += FW)
+                if (bad >> r & 1) {
+                    const int pr = t.first + r, tok = pr / c.group;
+                    float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs : A.part + (slot + r) * hs;
+                    row_again<__half>(A, t, head, r, lo, hi, o, whole ? nullptr : A.part_ml + (slot + r) * 2);
+                }
+            __syncthreads();
+        }
+        if (!whole) {
+            const long long at = (long long)t.line + (long long)head * t.units;
+            const int first = block_of(s, at), end = block_of(s, at + t.units - 1);
+            if (last_to_come(A.tickets + first, end - first + 1, &flag)) join<FT>(A, t, head, first, end);
+        }
+        left -= n;
+        unit = 0;
+        if (left > 0 && ++head == c.n_kv) {
+            head = 0;
+            t = load_tile(c.plan, s.tiles, ++tile);
+        }
+    }
+}
+
+template <int HS>
+int launch_few(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
+    auto kern = paged_attn_few_kernel<HS>;
+    static PerDeviceOnce attr;
+    if (attr.need(ctx->device)) {
+        SLAI_CHECK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem<HS>()));
+        attr.set(ctx->device);
+    }
+    return launch_dependent(ctx, kern, dim3((unsigned)blocks), FT, few_smem<HS>(), pdl, A);
+}
+
 }  // namespace
 
+// Whether a handle's few-row launches can take the matrix instructions (with rows that can be read in 16-byte pieces).
+bool paged_attention_few(int kv_dtype, int hs) { return kv_dtype == SLAI_KV_F16 && hs % 8 == 0 && hs <= 128; }
+
 int paged_attention_launch(slai_ctx* ctx, AttnArgs& A, int kv_dtype, int lane, int blocks, bool pdl) {
-    (void)lane;
     if (blocks <= 0) return SLAI_OK;
+    if (lane == 0 && A.vec && paged_attention_few(kv_dtype, A.c.hs)) return A.c.hs <= 64 ? launch_few<64>(ctx, A, blocks, pdl) : launch_few<128>(ctx, A, blocks, pdl);
     return kv_dtype == SLAI_KV_F16 ? launch_any<__half>(ctx, A, blocks, pdl) : launch_any<float>(ctx, A, blocks, pdl);
 }
