@@ -69,11 +69,7 @@ namespace {
 int make_handle(slai_ctx* ctx, slai_paged* p) {
     const Config& c = p->cfg;
     const int sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
-    Lane few, many;
-    few.rows = 16;
-    few.unit = 64;
-    few.blocks = (paged_attention_few(c.kv_dtype, c.head_size) ? 2 : 4) * sms;
-    few.least = 2;
+    const Lane few = paged_attention_lane(c.kv_dtype, c.head_size, sms), many;
     p->planner.init(c, few, many, 0);
     const size_t bytes = (size_t)p->planner.lay().total * 4;
     SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_plan, bytes));

@@ -166,11 +166,11 @@ __global__ void __launch_bounds__(GT) paged_attn_any_kernel(const __grid_constan
             }
         }
         if (!whole) {
-            const long long at = (long long)t.line + (long long)head * t.units;
+            const long long at = (long long)t.line + PAIR_COST + (long long)head * (t.units + PAIR_COST);
             const int first = block_of(s, at), end = block_of(s, at + t.units - 1);
-            if (last_to_come(A.tickets + first, end - first + 1, &flag)) join<GT>(A, t, head, first, end);
+            if (last_to_come(A.tickets + first, end - first + 1, &flag)) join<GT>(A, t, head, first, end, reinterpret_cast<float2*>(k_s), GP * (hsp + 4) / 2);
         }
-        left -= n;
+        left -= n + PAIR_COST;
         unit = 0;
         if (left > 0 && ++head == c.n_kv) {
             head = 0;
@@ -262,22 +262,29 @@ __device__ __forceinline__ float power_up(float largest, float& unit) {
 }
 
 // ---- f16 caches, few rows: tokens of sequences that answer ---------------------------------------------------------------------
-// Up to 16 rows (a token's or a few tokens' query heads of one cache head) are one operand of the matrix instruction.  What such a call costs is reading the
-// cache: each of the block's four warps has a ring of its own of three stages of 16 positions, brought in by asynchronous copies that go around the registers
-// (two stages ahead; the page numbers one stage further), and takes every fourth 16 positions of the block's share with a running maximum and sum of its own;
-// they are joined in shared memory at the end.  Queries and weights are pairs of halves (22 bits), two products each; sums end every 16 positions (the matrix
-// unit truncates when it adds) and go on in registers.
-constexpr int FT = 128, FW = FT / 32, FP = 16, FS = 3;
+// Up to 8 rows (a token's or a few tokens' query heads of one cache head).  Queries and weights are pairs of halves (22 bits); the 16 rows of the matrix
+// instruction are the 8 high parts and, below them, the 8 low ones, so one product does both and a lane holds both results of its row.  Sums end every 16
+// positions (the matrix unit truncates when it adds) and go on in registers.
+// What such a call costs is reading the cache: each of the block's warps has a ring of its own of stages of 16 positions, brought in by asynchronous
+// copies that go around the registers, and takes every FW-th 16 positions of the block's share with a running maximum and sum of its own; they are joined in shared
+// memory at the end.
+#ifndef FEW_W
+#define FEW_W 4
+#define FEW_S 3
+#define FEW_B 2
+#endif
+constexpr int FW = FEW_W, FT = 32 * FW, FP = 16, FS = FEW_S, FR = 8;
 template <int HS>
-constexpr int few_smem() { return FW * FS * 2 * FP * HS * 2; }
+constexpr int FEW_SMEM = FW * FS * 2 * FP * HS * 2;
 
-template <int HS>
-__global__ void __launch_bounds__(FT, 2) paged_attn_few_kernel(const __grid_constant__ AttnArgs A) {
+// ALIGNED: pages hold a multiple of 16 positions, so 16 of them have one page.
+template <int HS, bool ALIGNED>
+__global__ void __launch_bounds__(FT, FEW_B) paged_attn_few_kernel(const __grid_constant__ AttnArgs A) {
     constexpr int ROW = HS * 2, CH = HS / 8, TILE = FP * ROW, STAGE = 2 * TILE, KS = HS / 16, NT8 = HS / 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     extern __shared__ __align__(128) unsigned char few_sm[];
-    __shared__ float2 ml_s[FW][16];
+    __shared__ float2 ml_s[FW][FR];
     __shared__ unsigned int bad;
     __shared__ int flag;
     const Cache& c = A.c;
@@ -293,87 +300,83 @@ __global__ void __launch_bounds__(FT, 2) paged_attn_few_kernel(const __grid_cons
         const bool whole = n == t.units;
         const int lo = unit * A.unit, hi = min((unit + n) * A.unit, t.pos0 + (t.first + t.rows - 1) / c.group + 1);  // positions [lo, hi)
         const int subs = (hi - lo + FP - 1) / FP, mine = subs > warp ? (subs - warp + FW - 1) / FW : 0;
-        // place of position (lane & 15) of this warp's i-th 16, in bytes; -1 behind the end
+        // Where this warp's i-th 16 positions are, in bytes: of the first of them (ALIGNED), or of position (lane & 15).
         auto place = [&](int i) -> long long {
-            const int p = lo + (warp + i * FW) * FP + (lane & 15);
-            return i < mine && p < hi ? 2 * place_of(c, t.table, p, head) : -1;
+            const int p = lo + (warp + i * FW) * FP + (ALIGNED ? 0 : lane & 15);
+            return i < mine && p < hi ? 2 * place_of(c, t.table, p, head) : 0;
         };
         auto request = [&](int i, long long at) {
             if (i < mine) {
                 const uint32_t dst = ring + (i % FS) * STAGE;
+                const int valid = hi - (lo + (warp + i * FW) * FP), ch = lane % CH, r0 = lane / CH;
+                constexpr int STEP = 32 / CH;  // rows a pass of the warp covers
+                const char *k0 = keys + at + 16 * ch, *v0 = values + at + 16 * ch;
 #pragma unroll
-                for (int k = 0; k < FP * CH / 32; k++) {
-                    const int r = (lane + 32 * k) / CH, ch = lane % CH;
-                    const long long a = __shfl_sync(0xffffffffu, at, r);
-                    const uint32_t off = r * ROW + ((ch ^ (r & 7)) << 4), bytes = a >= 0 && ch < chunks ? 16u : 0u;
-                    const long long src = bytes ? a + 16 * ch : 0;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + off), "l"(__cvta_generic_to_global(keys + src)), "r"(bytes) : "memory");
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + TILE + off), "l"(__cvta_generic_to_global(values + src)), "r"(bytes) : "memory");
+                for (int k = 0; k < FP / STEP; k++) {
+                    const int r = r0 + STEP * k;
+                    const uint32_t off = r * ROW + ((ch ^ (r & 7)) << 4), bytes = r < valid && ch < chunks ? 16u : 0u;  // (none: zeros, nothing is read)
+                    long long a = r * 2 * c.pos_stride;
+                    if (!ALIGNED) a = __shfl_sync(0xffffffffu, at, r) - at;
+                    if (bytes == 0) a = -at - 16 * ch;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + off), "l"(__cvta_generic_to_global(k0 + a)), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + TILE + off), "l"(__cvta_generic_to_global(v0 + a)), "r"(bytes) : "memory");
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         {
-            const long long a0 = place(0), a1 = place(1);
-            request(0, a0);
-            request(1, a1);
-        }
-        long long next = place(2);
-
-        // queries: rows g and g + 8
-        uint32_t qh[KS][4], ql[KS][4];
-        float cexp[2];  // the row's scores to powers of two
-        int vis[2];     // last position the row sees
-        {
-            float2 v[KS][4];
-            float mx[2] = {0.f, 0.f};
-            const float* qr[2];
+            long long at[FS - 1];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int r = g + 8 * h, pr = t.first + r, tok = pr / c.group;
-                vis[h] = r < t.rows ? t.pos0 + tok : -1;
-                qr[h] = A.q + (r < t.rows ? (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs : 0);
-            }
+            for (int i = 0; i < FS - 1; i++) at[i] = place(i);
+#pragma unroll
+            for (int i = 0; i < FS - 1; i++) request(i, at[i]);
+        }
+        long long next = place(FS - 1);
+
+        // queries of row g: high parts in the instruction's row g, low ones in row g + 8
+        uint32_t qf[KS][4];
+        float cexp;  // the row's scores to powers of two
+        const int pr_g = t.first + g, tok_g = pr_g / c.group, vis = g < t.rows ? t.pos0 + tok_g : -1;  // last position the row sees
+        {
+            float2 v[KS][2];
+            float mx = 0.f;
+            const float* qr = A.q + (g < t.rows ? (t.row0 + tok_g) * A.q_ld + (long long)(head * c.group + pr_g % c.group) * hs : 0);
 #pragma unroll
             for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int d = 16 * k + 2 * t4 + 8 * (i >> 1);
+                for (int i = 0; i < 2; i++) {
+                    const int d = 16 * k + 2 * t4 + 8 * i;
                     v[k][i] = make_float2(0.f, 0.f);
-                    if (vis[i & 1] >= 0 && d < hs) {
-                        if (A.qvec) v[k][i] = __ldcg(reinterpret_cast<const float2*>(qr[i & 1] + d));
-                        else v[k][i] = make_float2(__ldcg(qr[i & 1] + d), __ldcg(qr[i & 1] + d + 1));
+                    if (vis >= 0 && d < hs) {
+                        if (A.qvec) v[k][i] = __ldcg(reinterpret_cast<const float2*>(qr + d));
+                        else v[k][i] = make_float2(__ldcg(qr + d), __ldcg(qr + d + 1));
                     }
                     v[k][i].x *= A.scale;
                     v[k][i].y *= A.scale;
-                    mx[i & 1] = fmaxf(mx[i & 1], fmaxf(fabsf(v[k][i].x), fabsf(v[k][i].y)));
+                    mx = fmaxf(mx, fmaxf(fabsf(v[k][i].x), fabsf(v[k][i].y)));
                 }
-            float up[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                up[h] = power_up(mx[h], cexp[h]);
-                cexp[h] *= LOG2E;
-            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float up = power_up(mx, cexp);
+            cexp *= LOG2E;
 #pragma unroll
             for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) split2(v[k][i].x * up[i & 1], v[k][i].y * up[i & 1], qh[k][i], ql[k][i]);
+                for (int i = 0; i < 2; i++) split2(v[k][i].x * up, v[k][i].y * up, qf[k][2 * i], qf[k][2 * i + 1]);
         }
-        float acc[NT8][4];
+        float acc[NT8][2];
 #pragma unroll
-        for (int i = 0; i < NT8; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m: largest score so far, as a power of two's exponent
+        for (int i = 0; i < NT8; i++) acc[i][0] = acc[i][1] = 0.f;
+        float m = -INFINITY, l = 0.f;  // m: largest score so far, as a power of two's exponent
 
         for (int i = 0; i < mine; i++) {
-            request(i + 2, next);
-            next = place(i + 3);
-            asm volatile("cp.async.wait_group 2;" ::: "memory");
+            request(i + FS - 1, next);
+            next = place(i + FS);
+            asm volatile("cp.async.wait_group %0;" ::"n"(FS - 1) : "memory");
             __syncwarp();
             const uint32_t ks = ring + (i % FS) * STAGE, vs = ks + TILE;
             const int p0 = lo + (warp + i * FW) * FP;
-            float sc[2][4];
+            float sc[4];
 #pragma unroll
             for (int nn = 0; nn < 2; nn++) {
                 float c0[4] = {}, c1[4] = {};
@@ -382,72 +385,55 @@ __global__ void __launch_bounds__(FT, 2) paged_attn_few_kernel(const __grid_cons
 #pragma unroll
                 for (int k2 = 0; k2 < KS / 2; k2++) ldsm4(ks + r * ROW + (((4 * k2 + (lane >> 3)) ^ (r & 7)) << 4), b[k2]);
 #pragma unroll
-                for (int k = 0; k < KS; k++) mma_f16((k & 1) ? c1 : c0, ql[k], b[k >> 1][2 * (k & 1)], b[k >> 1][2 * (k & 1) + 1]);
+                for (int k = 0; k < KS; k++) mma_f16((k & 1) ? c1 : c0, qf[k], b[k >> 1][2 * (k & 1)], b[k >> 1][2 * (k & 1) + 1]);
 #pragma unroll
-                for (int k = 0; k < KS; k++) mma_f16((k & 1) ? c1 : c0, qh[k], b[k >> 1][2 * (k & 1)], b[k >> 1][2 * (k & 1) + 1]);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    sc[nn][e] = (c0[e] + c1[e]) * cexp[e >> 1];
-                    if (p0 + 8 * nn + 2 * t4 + (e & 1) > vis[e >> 1]) sc[nn][e] = -INFINITY;
+                for (int e = 0; e < 2; e++) {
+                    const float x = ((c0[e] + c1[e]) + (c0[e + 2] + c1[e + 2])) * cexp;
+                    sc[2 * nn + e] = p0 + 8 * nn + 2 * t4 + e > vis ? -INFINITY : x;
                 }
             }
-            float resc[2];
+            float mt = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+            const float m_new = fmaxf(m, mt), base = m_new == -INFINITY ? 0.f : m_new, resc = ex2(m - base);
+            m = m_new;
+            float ps = 0.f;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float mt = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-                const float m_new = fmaxf(m[h], mt), base = m_new == -INFINITY ? 0.f : m_new;
-                resc[h] = ex2(m[h] - base);
-                m[h] = m_new;
-                float ps = 0.f;
-#pragma unroll
-                for (int nn = 0; nn < 2; nn++)
-#pragma unroll
-                    for (int e = 2 * h; e < 2 * h + 2; e++) {
-                        const float p = ex2(sc[nn][e] - base);
-                        ps += p;
-                        sc[nn][e] = p * 4096.f;
-                    }
-                l[h] = l[h] * resc[h] + ps;  // (this lane's positions only)
+            for (int e = 0; e < 4; e++) {
+                const float p = ex2(sc[e] - base);
+                ps += p;
+                sc[e] = p * 4096.f;
             }
-            uint32_t ph[4], pl[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) split2(sc[e >> 1][2 * (e & 1)], sc[e >> 1][2 * (e & 1) + 1], ph[e], pl[e]);
+            l = l * resc + ps;  // (this lane's positions only)
+            uint32_t pf[4];
+            split2(sc[0], sc[1], pf[0], pf[1]);
+            split2(sc[2], sc[3], pf[2], pf[3]);
 #pragma unroll
             for (int n2 = 0; n2 < NT8 / 2; n2++) {
                 float d0[4] = {}, d1[4] = {};
                 uint32_t b[4];
                 const int r = lane & 15;
                 ldsm4t(vs + r * ROW + (((2 * n2 + (lane >> 4)) ^ (r & 7)) << 4), b);
-                mma_f16(d0, pl, b[0], b[1]);
-                mma_f16(d1, pl, b[2], b[3]);
-                mma_f16(d0, ph, b[0], b[1]);
-                mma_f16(d1, ph, b[2], b[3]);
+                mma_f16(d0, pf, b[0], b[1]);
+                mma_f16(d1, pf, b[2], b[3]);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    acc[2 * n2][e] = fmaf(acc[2 * n2][e], resc[e >> 1], d0[e]);
-                    acc[2 * n2 + 1][e] = fmaf(acc[2 * n2 + 1][e], resc[e >> 1], d1[e]);
+                for (int e = 0; e < 2; e++) {
+                    acc[2 * n2][e] = fmaf(acc[2 * n2][e], resc, d0[e] + d0[e + 2]);
+                    acc[2 * n2 + 1][e] = fmaf(acc[2 * n2 + 1][e], resc, d1[e] + d1[e + 2]);
                 }
             }
             __syncwarp();  // the stage is requested again next round
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            if (t4 == 0) ml_s[warp][g + 8 * h] = make_float2(m[h], l[h]);
-        }
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t4 == 0) ml_s[warp][g] = make_float2(m, l);
         // the warps' sums meet where the stages were (each in its own ring)
         float* so = reinterpret_cast<float*>(few_sm);
         constexpr int WF = FS * STAGE / 4;
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < NT8; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-                *reinterpret_cast<float2*>(so + warp * WF + (g + 8 * h) * HS + 8 * i + 2 * t4) = make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
+        for (int i = 0; i < NT8; i++) *reinterpret_cast<float2*>(so + warp * WF + g * HS + 8 * i + 2 * t4) = make_float2(acc[i][0], acc[i][1]);
         if (tid == 0) bad = 0;
         __syncthreads();
         const size_t slot = ((size_t)s.me * 2 + (unit == 0)) * A.tile_rows;
@@ -464,8 +450,7 @@ __global__ void __launch_bounds__(FT, 2) paged_attn_few_kernel(const __grid_cons
                 den = fmaf(f, x.y, den);
                 num[0] = fmaf(f, o.x, num[0]); num[1] = fmaf(f, o.y, num[1]); num[2] = fmaf(f, o.z, num[2]); num[3] = fmaf(f, o.w, num[3]);
             }
-            const float sum = num[0] + num[1] + num[2] + num[3] + den;
-            if (!(fabsf(sum) < INFINITY)) atomicOr(&bad, 1u << r);
+            if (!(fabsf(num[0] + num[1] + num[2] + num[3] + den) < INFINITY)) atomicOr(&bad, 1u << r);
             const float f = whole ? 1.f / (den * 4096.f) : 1.f / 4096.f;
             const int pr = t.first + r, tok = pr / c.group;
             float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs + d : A.part + (slot + r) * hs + d;
@@ -487,11 +472,12 @@ __global__ void __launch_bounds__(FT, 2) paged_attn_few_kernel(const __grid_cons
             __syncthreads();
         }
         if (!whole) {
-            const long long at = (long long)t.line + (long long)head * t.units;
+            const long long at = (long long)t.line + PAIR_COST + (long long)head * (t.units + PAIR_COST);
             const int first = block_of(s, at), end = block_of(s, at + t.units - 1);
-            if (last_to_come(A.tickets + first, end - first + 1, &flag)) join<FT>(A, t, head, first, end);
+            if (last_to_come(A.tickets + first, end - first + 1, &flag))
+                join<FT>(A, t, head, first, end, reinterpret_cast<float2*>(few_sm), FEW_SMEM<HS> / 8);
         }
-        left -= n;
+        left -= n + PAIR_COST;
         unit = 0;
         if (left > 0 && ++head == c.n_kv) {
             head = 0;
@@ -500,24 +486,40 @@ __global__ void __launch_bounds__(FT, 2) paged_attn_few_kernel(const __grid_cons
     }
 }
 
-template <int HS>
+template <int HS, bool ALIGNED>
 int launch_few(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
-    auto kern = paged_attn_few_kernel<HS>;
+    auto kern = paged_attn_few_kernel<HS, ALIGNED>;
     static PerDeviceOnce attr;
     if (attr.need(ctx->device)) {
-        SLAI_CHECK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem<HS>()));
+        SLAI_CHECK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM<HS>));
         attr.set(ctx->device);
     }
-    return launch_dependent(ctx, kern, dim3((unsigned)blocks), FT, few_smem<HS>(), pdl, A);
+    return launch_dependent(ctx, kern, dim3((unsigned)blocks), FT, FEW_SMEM<HS>, pdl, A);
 }
 
 }  // namespace
 
 // Whether a handle's few-row launches can take the matrix instructions (with rows that can be read in 16-byte pieces).
 bool paged_attention_few(int kv_dtype, int hs) { return kv_dtype == SLAI_KV_F16 && hs % 8 == 0 && hs <= 128; }
+Lane paged_attention_lane(int kv_dtype, int hs, int sms) {
+    Lane l;
+    l.unit = 64;
+    l.least = 2;
+    if (paged_attention_few(kv_dtype, hs)) {
+        l.rows = FR;
+        l.blocks = FEW_B * sms;
+    } else {
+        l.rows = GR;
+        l.blocks = 4 * sms;
+    }
+    return l;
+}
 
 int paged_attention_launch(slai_ctx* ctx, AttnArgs& A, int kv_dtype, int lane, int blocks, bool pdl) {
     if (blocks <= 0) return SLAI_OK;
-    if (lane == 0 && A.vec && paged_attention_few(kv_dtype, A.c.hs)) return A.c.hs <= 64 ? launch_few<64>(ctx, A, blocks, pdl) : launch_few<128>(ctx, A, blocks, pdl);
+    if (lane == 0 && A.vec && paged_attention_few(kv_dtype, A.c.hs)) {
+        if (A.c.page_size % FP == 0) return A.c.hs <= 64 ? launch_few<64, true>(ctx, A, blocks, pdl) : launch_few<128, true>(ctx, A, blocks, pdl);
+        return A.c.hs <= 64 ? launch_few<64, false>(ctx, A, blocks, pdl) : launch_few<128, false>(ctx, A, blocks, pdl);
+    }
     return kv_dtype == SLAI_KV_F16 ? launch_any<__half>(ctx, A, blocks, pdl) : launch_any<float>(ctx, A, blocks, pdl);
 }

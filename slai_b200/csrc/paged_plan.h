@@ -3,7 +3,8 @@
 // A sequence's rows of the step's attention are (token, query head of the group) pairs, one cache head at a time: rows [R i, R i + R) of them are a
 // tile.  A tile's work is its positions, 0 .. the last one its last row sees, in units of `unit` positions; the units of all (tile, cache head) pairs stand
 // in one line, tile by tile and head by head, and a block takes an equal share of that line, from somewhere in one pair to somewhere in another.  So
-// one long sequence and many short ones keep all SMs equally long; a pair that lies on several blocks leaves partial results (two a block at most),
+// one long sequence and many short ones keep all SMs equally long.  To begin and end a pair costs a block about as much as PAIR_COST units, which stand in the
+// line in front of the pair's own.  A pair that lies on several blocks leaves partial results (two a block at most),
 // which the block that comes last joins in the order of their positions.
 #pragma once
 #include <stdint.h>
@@ -13,6 +14,8 @@
 #include <vector>
 
 namespace paged {
+
+constexpr int PAIR_COST = 2;
 
 struct Config {
     int n_q_heads, n_kv_heads, head_size, page_size, n_pages, kv_dtype;
@@ -27,14 +30,14 @@ struct Tile {
     int rows;     // packed rows of the tile
     int table;    // page table of the sequence
     int units;    // of one cache head
-    int line;     // place in the line of the tile's first unit
+    int line;     // place in the line of the tile's first pair
     int pad;
 };
 struct Start {  // where a block begins
-    int tile, head, unit, count;   // count: units of the block
+    int tile, head, unit, count;   // count: places of the line from there to the end of the block's share
     Tile t;                        // tiles[tile]
     int tiles;                     // offset of the tiles
-    int units, blocks, me;         // of the whole line; blocks that share it
+    int units, blocks, me;         // places of the whole line; blocks that share it
 };
 struct Row {  // a token of the step
     int pos, slot;  // slot: page * page_size + place in the page
@@ -119,7 +122,7 @@ class Planner {
             if (rows > cfg_.max_tokens) return "more new tokens than max_tokens (" + std::to_string(cfg_.max_tokens) + ")";
             if (entries > cfg_.max_table) return "more pages than max_table (" + std::to_string(cfg_.max_table) + ")";
             const int k = lane_of(n_new[b]);
-            for_tiles(b, pos0[b], n_new[b], group, [&](const Tile& t) { line[k] += (long long)t.units * cfg_.n_kv_heads; });
+            for_tiles(b, pos0[b], n_new[b], group, [&](const Tile& t) { line[k] += (long long)(t.units + PAIR_COST) * cfg_.n_kv_heads; });
         }
         if (line[0] > 0x7fffffffll || line[1] > 0x7fffffffll) return "the step's attention is too large";
         // Every page exists; one that gets new tokens belongs to its sequence alone, and to one place of it (pages that are only read may be shared).
@@ -172,7 +175,7 @@ class Planner {
                         t.row0 = r0;
                         t.table = tab_at[b];
                         t.line = so_far;
-                        so_far += t.units * cfg_.n_kv_heads;
+                        so_far += (t.units + PAIR_COST) * cfg_.n_kv_heads;
                         tiles[n++] = t;
                     });
                 r0 += n_new[b];
@@ -187,12 +190,12 @@ class Planner {
                 Start s = {};
                 if (c < C) {
                     const long long lo = U * c / C, hi = U * (c + 1) / C;
-                    while (lo >= tiles[tile].line + (long long)tiles[tile].units * cfg_.n_kv_heads) tile++;
-                    const int in = (int)(lo - tiles[tile].line);
+                    while (lo >= tiles[tile].line + (long long)(tiles[tile].units + PAIR_COST) * cfg_.n_kv_heads) tile++;
+                    const int in = (int)(lo - tiles[tile].line), pair = tiles[tile].units + PAIR_COST, skip = std::max(0, PAIR_COST - in % pair);
                     s.tile = tile;
-                    s.head = in / tiles[tile].units;
-                    s.unit = in % tiles[tile].units;
-                    s.count = (int)(hi - lo);
+                    s.head = in / pair;
+                    s.unit = std::max(0, in % pair - PAIR_COST);
+                    s.count = (int)(hi - lo) - skip;  // (none is left where the share ends in front of the pair's first unit)
                     s.t = tiles[tile];
                     s.tiles = tiles_at;
                     s.units = (int)U;

@@ -6,6 +6,7 @@ import subprocess
 import numpy as np
 import pytest
 
+COST = 2  # places of the line in front of a pair
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
@@ -107,8 +108,8 @@ def walk(p, k):
         s = words(p.starts[k] + 16 * c, 16)
         tile, head, unit, left = (int(x) for x in s[:4])
         t, tiles, U, blocks, me = s[4:12], int(s[12]), int(s[13]), int(s[14]), int(s[15])
-        assert (left > 0) == (c < p.step[1 + k])
-        if left:
+        assert left <= 0 or c < p.step[1 + k]
+        if c < p.step[1 + k]:
             assert me == c and blocks == p.step[1 + k] and (t == words(tiles + 8 * tile, 8)).all()
         began = unit
         while left > 0:
@@ -116,12 +117,12 @@ def walk(p, k):
             assert n > 0
             got += [(tile, head, u) for u in range(unit, unit + n)]
             if n < t[5]:
-                at = int(t[6]) + head * int(t[5])
+                at = int(t[6]) + COST + head * (int(t[5]) + COST)
                 block = lambda x: ((x + 1) * blocks - 1) // U  # noqa: E731
                 first, last = block(at), block(at + int(t[5]) - 1)
                 parts.setdefault((tile, head), (first, last, []))[2].append((c, int(unit == 0)))
                 assert unit == 0 or unit == began
-            left -= n
+            left -= n + COST
             unit = began = 0
             if left > 0:
                 head += 1
