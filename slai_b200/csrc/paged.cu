@@ -49,7 +49,6 @@ struct slai_paged {
     cudaEvent_t copied[SLOTS] = {};
     int slot = 0;
     float *d_part[2] = {}, *d_ml[2] = {};
-    unsigned int* d_tickets = nullptr;
     ~slai_paged() {
         cudaFree(d_plan);
         for (int i = 0; i < SLOTS; i++) {
@@ -60,7 +59,6 @@ struct slai_paged {
             cudaFree(d_part[k]);
             cudaFree(d_ml[k]);
         }
-        cudaFree(d_tickets);
     }
 };
 
@@ -77,16 +75,12 @@ int make_handle(slai_ctx* ctx, slai_paged* p) {
         SLAI_CHECK_CUDA(ctx, cudaMallocHost(&p->h_plan[i], bytes));
         SLAI_CHECK_CUDA(ctx, cudaEventCreateWithFlags(&p->copied[i], cudaEventDisableTiming));
     }
-    int blocks = 0;
     for (int k = 0; k < 2; k++) {
         const Lane& l = p->planner.lane(k);
-        blocks += l.blocks;
         if (l.blocks == 0) continue;
         SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_part[k], sizeof(float) * 2 * l.blocks * l.rows * c.head_size));
         SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_ml[k], sizeof(float) * 2 * l.blocks * l.rows * 2));
     }
-    SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_tickets, sizeof(unsigned int) * blocks));
-    SLAI_CHECK_CUDA(ctx, cudaMemsetAsync(p->d_tickets, 0, sizeof(unsigned int) * blocks, ctx->stream));
     return SLAI_OK;
 }
 
@@ -253,19 +247,17 @@ SLAI_API int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, 
     A.err_flag = ctx->d_counters + CNT_ERR_FLAG;
     A.wait_limit = ctx->wait_limit;
     const bool recording = capturing(ctx);
-    unsigned int* tickets = p->d_tickets;
     for (int k = 0; k < 2; k++) {
         const Lane& l = p->planner.lane(k);
         if (l.blocks == 0) continue;
-        A.lane = k;
         A.starts_at = p->planner.lay().starts[k];
+        A.joins_at = p->planner.lay().joins[k];
+        A.count_at = p->planner.lay().count + 1 + k;
         A.tile_rows = l.rows;
         A.unit = l.unit;
         A.part = p->d_part[k];
         A.part_ml = p->d_ml[k];
-        A.tickets = tickets;
-        tickets += l.blocks;
-        if ((rc = paged_attention_launch(ctx, A, c.kv_dtype, k, recording ? l.blocks : p->step.blocks[k], ctx->use_pdl))) return rc;
+        if ((rc = paged_attention_launch(ctx, A, c.kv_dtype, k, recording ? l.blocks : p->step.blocks[k], recording ? l.blocks : p->step.joins[k], ctx->use_pdl))) return rc;
     }
     return SLAI_OK;
 }

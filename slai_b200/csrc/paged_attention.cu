@@ -58,7 +58,6 @@ __global__ void __launch_bounds__(GT) paged_attn_any_kernel(const __grid_constan
     float* v_s = k_s + GP * ks;     // [32][hsp]
     float* p_s = v_s + GP * hsp;    // [16][32]
     __shared__ long long place[GP];
-    __shared__ int flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     Tile t = s.t;
@@ -165,11 +164,6 @@ __global__ void __launch_bounds__(GT) paged_attn_any_kernel(const __grid_constan
                 if (!whole && lane == 0) *reinterpret_cast<float2*>(A.part_ml + (slot + g0 + r) * 2) = make_float2(m[i] * LOG2E, l[i]);
             }
         }
-        if (!whole) {
-            const long long at = (long long)t.line + PAIR_COST + (long long)head * (t.units + PAIR_COST);
-            const int first = block_of(s, at), end = block_of(s, at + t.units - 1);
-            if (last_to_come(A.tickets + first, end - first + 1, &flag)) join<GT>(A, t, head, first, end, reinterpret_cast<float2*>(k_s), GP * (hsp + 4) / 2);
-        }
         left -= n + PAIR_COST;
         unit = 0;
         if (left > 0 && ++head == c.n_kv) {
@@ -190,6 +184,88 @@ int launch_any(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
         attr.set(ctx->device);
     }
     return launch_dependent(ctx, kern, dim3((unsigned)blocks), GT, smem, pdl, A);
+}
+
+// ---- pairs that lie on several blocks ------------------------------------------------------------------------------------------
+// Rows of a tile: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the blocks' results in the order of their positions (a block that saw nothing of a row
+// has m = -inf, l = 0, o = 0).  A launch of its own behind the other's end, whose blocks read all results at once: done by the block that comes last, a
+// token over 32750 positions (37 blocks a pair) took 12 us from its loop's end to the result, and over 515 positions 5.
+constexpr int JT = 128, JW = JT / 32;
+// SPLIT: a block takes one row, its warps every JW-th result; else a warp takes a row.
+template <bool SPLIT>
+__global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs A) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hs = A.c.hs;
+    const int4* g = reinterpret_cast<const int4*>(A.c.plan + A.joins_at) + 2 * blockIdx.x;
+    const int4 j0 = __ldcg(g), j1 = __ldcg(g + 1);  // row0, first, rows, head; begin, end
+    const bool none = (int)blockIdx.x >= __ldcg(A.c.plan + A.count_at);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (none) return;
+    const int r = SPLIT ? (int)blockIdx.y : (int)blockIdx.y * JW + warp, nb = j1.y - j1.x + 1;
+    if (r >= j0.z) return;
+    auto slot = [&](int i) { return ((size_t)(j1.x + i) * 2 + (i == 0)) * A.tile_rows + r; };
+    const float2* ml = reinterpret_cast<const float2*>(A.part_ml);
+    constexpr int STEP = SPLIT ? JW : 1;
+    const int b_first = SPLIT ? warp : 0;
+    const bool quads = hs % 4 == 0;
+    __shared__ float num_s[SPLIT ? JW : 1][256];
+    __shared__ float den_s[JW];
+    float M = -INFINITY;
+    for (int b = lane; b < nb; b += 32) M = fmaxf(M, __ldcg(ml + slot(b)).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const int pr = j0.y + r, tok = pr / A.c.group;
+    float* out = A.out + (j0.x + tok) * A.out_ld + (long long)(j0.w * A.c.group + pr % A.c.group) * hs;
+    for (int d0 = 0; d0 < hs; d0 += quads ? 128 : 32) {
+        const int d = d0 + (quads ? 4 * lane : lane);
+        float num[4] = {}, den = 0.f;
+        for (int b0 = b_first; b0 < nb; b0 += 8 * STEP) {
+            float4 o[8];
+            float2 y[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int b = b0 + u * STEP;
+                o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                y[u] = make_float2(-INFINITY, 0.f);
+                if (b < nb) {
+                    y[u] = __ldcg(ml + slot(b));
+                    const float* p = A.part + slot(b) * hs + d;
+                    if (quads && d < hs) o[u] = __ldcg(reinterpret_cast<const float4*>(p));
+                    else if (d < hs) o[u].x = __ldcg(p);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float f = y[u].x == -INFINITY ? 0.f : exp2f(y[u].x - M);
+                den = fmaf(f, y[u].y, den);
+                num[0] = fmaf(f, o[u].x, num[0]); num[1] = fmaf(f, o[u].y, num[1]); num[2] = fmaf(f, o[u].z, num[2]); num[3] = fmaf(f, o[u].w, num[3]);
+            }
+        }
+        if (!SPLIT) {
+            for (int e = 0; e < (quads ? 4 : 1) && d < hs; e++) out[d + e] = num[e] / den;
+        } else {
+            for (int e = 0; e < (quads ? 4 : 1) && d < hs; e++) num_s[warp][d + e] = num[e];
+            if (lane == 0) den_s[warp] = den;
+        }
+    }
+    if (SPLIT) {
+        __syncthreads();
+        for (int d = threadIdx.x; d < hs; d += JT) {
+            float n = 0.f, den = 0.f;
+#pragma unroll
+            for (int w = 0; w < JW; w++) {
+                n += num_s[w][d];
+                den += den_s[w];
+            }
+            out[d] = n / den;
+        }
+    }
+}
+
+int launch_join(slai_ctx* ctx, const AttnArgs& A, int joins, bool pdl) {
+    if (joins <= 0) return SLAI_OK;
+    if (A.tile_rows <= 16) return launch_dependent(ctx, paged_join_kernel<true>, dim3((unsigned)joins, (unsigned)A.tile_rows), JT, 0, pdl, A);
+    return launch_dependent(ctx, paged_join_kernel<false>, dim3((unsigned)joins, (unsigned)((A.tile_rows + JW - 1) / JW)), JT, 0, pdl, A);
 }
 
 // ---- what the matrix units cannot carry ----------------------------------------------------------------------------------
@@ -282,17 +358,17 @@ template <int HS, bool ALIGNED>
 __global__ void __launch_bounds__(FT, FEW_B) paged_attn_few_kernel(const __grid_constant__ AttnArgs A) {
     constexpr int ROW = HS * 2, CH = HS / 8, TILE = FP * ROW, STAGE = 2 * TILE, KS = HS / 16, NT8 = HS / 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     extern __shared__ __align__(128) unsigned char few_sm[];
     __shared__ float2 ml_s[FW][FR];
     __shared__ unsigned int bad;
-    __shared__ int flag;
     const Cache& c = A.c;
     const Start s = load_start(c.plan, A.starts_at, blockIdx.x);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, hs = c.hs, chunks = hs / 8;
     const uint32_t sm = (uint32_t)__cvta_generic_to_shared(few_sm), ring = sm + warp * FS * STAGE;
     const char *keys = c.keys, *values = c.values;
 
+    bool behind = false;
+    if (s.count <= 0) asm volatile("griddepcontrol.wait;" ::: "memory");
     Tile t = s.t;
     int head = s.head, unit = s.unit, tile = s.tile;
     for (int left = s.count; left > 0;) {
@@ -328,6 +404,9 @@ __global__ void __launch_bounds__(FT, FEW_B) paged_attn_few_kernel(const __grid_
             long long at[FS - 1];
 #pragma unroll
             for (int i = 0; i < FS - 1; i++) at[i] = place(i);
+            // The plan is there before any kernel of its step starts (it comes by a copy, which no launch overtakes); all else is the kernel before's.
+            if (!behind) asm volatile("griddepcontrol.wait;" ::: "memory");
+            behind = true;
 #pragma unroll
             for (int i = 0; i < FS - 1; i++) request(i, at[i]);
         }
@@ -471,12 +550,6 @@ __global__ void __launch_bounds__(FT, FEW_B) paged_attn_few_kernel(const __grid_
                 }
             __syncthreads();
         }
-        if (!whole) {
-            const long long at = (long long)t.line + PAIR_COST + (long long)head * (t.units + PAIR_COST);
-            const int first = block_of(s, at), end = block_of(s, at + t.units - 1);
-            if (last_to_come(A.tickets + first, end - first + 1, &flag))
-                join<FT>(A, t, head, first, end, reinterpret_cast<float2*>(few_sm), FEW_SMEM<HS> / 8);
-        }
         left -= n + PAIR_COST;
         unit = 0;
         if (left > 0 && ++head == c.n_kv) {
@@ -515,11 +588,15 @@ Lane paged_attention_lane(int kv_dtype, int hs, int sms) {
     return l;
 }
 
-int paged_attention_launch(slai_ctx* ctx, AttnArgs& A, int kv_dtype, int lane, int blocks, bool pdl) {
-    if (blocks <= 0) return SLAI_OK;
+static int launch_lane(slai_ctx* ctx, const AttnArgs& A, int kv_dtype, int lane, int blocks, bool pdl) {
     if (lane == 0 && A.vec && paged_attention_few(kv_dtype, A.c.hs)) {
         if (A.c.page_size % FP == 0) return A.c.hs <= 64 ? launch_few<64, true>(ctx, A, blocks, pdl) : launch_few<128, true>(ctx, A, blocks, pdl);
         return A.c.hs <= 64 ? launch_few<64, false>(ctx, A, blocks, pdl) : launch_few<128, false>(ctx, A, blocks, pdl);
     }
     return kv_dtype == SLAI_KV_F16 ? launch_any<__half>(ctx, A, blocks, pdl) : launch_any<float>(ctx, A, blocks, pdl);
+}
+int paged_attention_launch(slai_ctx* ctx, AttnArgs& A, int kv_dtype, int lane, int blocks, int joins, bool pdl) {
+    if (blocks <= 0) return SLAI_OK;
+    const int rc = launch_lane(ctx, A, kv_dtype, lane, blocks, pdl);
+    return rc ? rc : launch_join(ctx, A, joins, pdl);
 }

@@ -5,7 +5,7 @@
 // in one line, tile by tile and head by head, and a block takes an equal share of that line, from somewhere in one pair to somewhere in another.  So
 // one long sequence and many short ones keep all SMs equally long.  To begin and end a pair costs a block about as much as PAIR_COST units, which stand in the
 // line in front of the pair's own.  A pair that lies on several blocks leaves partial results (two a block at most),
-// which the block that comes last joins in the order of their positions.
+// which a launch behind it joins in the order of their positions.
 #pragma once
 #include <stdint.h>
 
@@ -39,10 +39,15 @@ struct Start {  // where a block begins
     int tiles;                     // offset of the tiles
     int units, blocks, me;         // places of the whole line; blocks that share it
 };
+struct Join {  // a pair that lies on several blocks
+    int row0, first, rows, head;  // as in Tile
+    int begin, end;               // the blocks; of `begin` the second slot, of the others the first
+    int pad[2];
+};
 struct Row {  // a token of the step
     int pos, slot;  // slot: page * page_size + place in the page
 };
-static_assert(sizeof(Tile) == 32 && sizeof(Start) == 64 && sizeof(Row) == 8, "read as words by the kernels");
+static_assert(sizeof(Tile) == 32 && sizeof(Start) == 64 && sizeof(Join) == 32 && sizeof(Row) == 8, "read as words by the kernels");
 
 struct Lane {  // one of the two kinds of kernel
     int rows = 0, unit = 0;    // tile height, positions of a unit
@@ -51,7 +56,7 @@ struct Lane {  // one of the two kinds of kernel
 };
 
 struct Layout {  // of the device copy, in ints
-    int starts[2], count, rows, dynamic, total;  // count: rows of the step
+    int starts[2], joins[2], count, rows, dynamic, total;  // count: numbers of the step's rows and of each lane's joins
 };
 inline int tiles_cap(const Config& c, const Lane& l) {
     return l.blocks ? (int)std::min<long long>(((long long)c.max_tokens * (c.n_q_heads / c.n_kv_heads)) / l.rows + c.max_seqs, 1ll << 30) : 0;
@@ -60,7 +65,9 @@ inline Layout layout(const Config& c, const Lane (&lanes)[2]) {
     Layout L;
     L.starts[0] = 0;
     L.starts[1] = L.starts[0] + lanes[0].blocks * (int)(sizeof(Start) / 4);
-    L.count = L.starts[1] + lanes[1].blocks * (int)(sizeof(Start) / 4);
+    L.joins[0] = L.starts[1] + lanes[1].blocks * (int)(sizeof(Start) / 4);
+    L.joins[1] = L.joins[0] + lanes[0].blocks * (int)(sizeof(Join) / 4);
+    L.count = L.joins[1] + lanes[1].blocks * (int)(sizeof(Join) / 4);
     L.rows = L.count + 8;
     L.dynamic = (L.rows + 2 * c.max_tokens + 7) & ~7;
     L.total = L.dynamic + ((c.max_table + 7) & ~7) + (tiles_cap(c, lanes[0]) + tiles_cap(c, lanes[1])) * (int)(sizeof(Tile) / 4);
@@ -70,6 +77,7 @@ inline Layout layout(const Config& c, const Lane (&lanes)[2]) {
 struct Step {
     int n_rows = -1;          // -1: there has been no step
     int blocks[2] = {0, 0};   // blocks with work
+    int joins[2] = {0, 0};
     int used = 0;             // ints of the dynamic part
 };
 
@@ -185,7 +193,8 @@ class Planner {
             const int C = (int)std::min<long long>(lanes_[k].blocks, (U + lanes_[k].least - 1) / std::max(1, lanes_[k].least));
             step->blocks[k] = C;
             Start* st = reinterpret_cast<Start*>(out + lay_.starts[k]);
-            int tile = 0;
+            Join* jo = reinterpret_cast<Join*>(out + lay_.joins[k]);
+            int tile = 0, joins = 0, known = -1;  // known: the line's place of the last pair in `jo`
             for (int c = 0; c < lanes_[k].blocks; c++) {
                 Start s = {};
                 if (c < C) {
@@ -201,9 +210,23 @@ class Planner {
                     s.units = (int)U;
                     s.blocks = C;
                     s.me = c;
+                    const int at = tiles[tile].line + s.head * pair;
+                    if (s.unit > 0 && at != known) {
+                        auto block = [&](long long x) { return (int)(((x + 1) * C - 1) / U); };
+                        Join j = {};
+                        j.row0 = s.t.row0;
+                        j.first = s.t.first;
+                        j.rows = s.t.rows;
+                        j.head = s.head;
+                        j.begin = block(at + PAIR_COST);
+                        j.end = block(at + pair - 1);
+                        jo[joins++] = j;
+                        known = at;
+                    }
                 }
                 st[c] = s;
             }
+            step->joins[k] = out[lay_.count + 1 + k] = joins;
         }
         step->used = at - lay_.dynamic;
         return "";

@@ -32,17 +32,17 @@ Host* host_paged_create(const int* cfg, const int* lanes, int few, char* why, in
     return h;
 }
 void host_paged_destroy(Host* h) { delete h; }
-// total ints; offsets of starts[0], starts[1], count, rows, dynamic
+// total ints; offsets of starts, joins, count, rows, dynamic
 void host_paged_layout(Host* h, int* out) {
     const Layout& L = h->p.lay();
-    const int v[6] = {L.total, L.starts[0], L.starts[1], L.count, L.rows, L.dynamic};
+    const int v[8] = {L.total, L.starts[0], L.starts[1], L.joins[0], L.joins[1], L.count, L.rows, L.dynamic};
     memcpy(out, v, sizeof(v));
 }
-// out: total ints; step: n_rows, blocks[0], blocks[1], used.  Returns the reason ("" = fine).
+// out: total ints; step: n_rows, blocks of each lane, used, joins of each lane.  Returns the reason ("" = fine).
 const char* host_paged_plan(Host* h, int n, const int* pos0, const int* n_new, const int* tables, long long ld, int* out, int* step) {
     Step s;
     h->why = h->p.plan(n, pos0, n_new, tables, ld, out, &s);
-    const int v[4] = {s.n_rows, s.blocks[0], s.blocks[1], s.used};
+    const int v[6] = {s.n_rows, s.blocks[0], s.blocks[1], s.used, s.joins[0], s.joins[1]};
     memcpy(step, v, sizeof(v));
     return h->why.c_str();
 }

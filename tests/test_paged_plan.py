@@ -33,14 +33,15 @@ class Plan:
         self.h = lib.host_paged_create(cfg, flat, few, why, 300)
         self.why = why.value.decode()
         if self.h:
-            lay = (C.c_int * 6)()
+            lay = (C.c_int * 8)()
             lib.host_paged_layout(self.h, lay)
-            self.total, *self.starts, self.count, self.rows, self.dynamic = lay
+            self.total, *at, self.count, self.rows, self.dynamic = lay
+            self.starts, self.joins = at[:2], at[2:]
             self.out = np.full(self.total, -7, np.int32)
 
     def __call__(self, pos0, n_new, tables):
         pos0, n_new, tables = (np.ascontiguousarray(x, np.int32) for x in (pos0, n_new, tables))
-        step = (C.c_int * 4)()
+        step = (C.c_int * 6)()
         why = self.lib.host_paged_plan(self.h, len(pos0), pos0.ctypes.data, n_new.ctypes.data, tables.ctypes.data, tables.shape[1], self.out.ctypes.data, step)
         self.step = list(step)
         return why.decode()
@@ -119,8 +120,7 @@ def walk(p, k):
             if n < t[5]:
                 at = int(t[6]) + COST + head * (int(t[5]) + COST)
                 block = lambda x: ((x + 1) * blocks - 1) // U  # noqa: E731
-                first, last = block(at), block(at + int(t[5]) - 1)
-                parts.setdefault((tile, head), (first, last, []))[2].append((c, int(unit == 0)))
+                parts.setdefault((tile, head), ([int(x) for x in t[[0, 2, 3]]] + [head, block(at), block(at + int(t[5]) - 1)], []))[1].append((c, int(unit == 0)))
                 assert unit == 0 or unit == began
             left -= n + COST
             unit = began = 0
@@ -129,8 +129,10 @@ def walk(p, k):
                 if head == p.kv:
                     head, tile = 0, tile + 1
                     t = words(tiles + 8 * tile, 8)
-    for first, last, blocks in parts.values():
+    for (*_, first, last), blocks in parts.values():
         assert blocks == [(b, int(b == first)) for b in range(first, last + 1)]
+    joins = [words(p.joins[k] + 8 * i, 6).tolist() for i in range(p.step[4 + k])]
+    assert p.out[p.count + 1 + k] == p.step[4 + k] == len(parts) and joins == [j for j, _ in parts.values()]
     return got
 
 
