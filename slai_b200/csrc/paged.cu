@@ -7,6 +7,10 @@
 using namespace paged;
 
 namespace {
+#ifndef FEW_ROWS_DEF
+#define FEW_ROWS_DEF 32
+#endif
+constexpr int FEW_ROWS = FEW_ROWS_DEF;  // rows of a cache head that a sequence may bring and still go to the kernel for few
 constexpr int SLOTS = 2;  // pinned copies of a plan: the next step is planned while the last one's copy is on its way
 
 bool capturing(slai_ctx* ctx) {
@@ -67,8 +71,10 @@ namespace {
 int make_handle(slai_ctx* ctx, slai_paged* p) {
     const Config& c = p->cfg;
     const int sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
-    const Lane few = paged_attention_lane(c.kv_dtype, c.head_size, sms), many;
-    p->planner.init(c, few, many, 0);
+    const Lane few = paged_attention_lane(c.kv_dtype, c.head_size, sms);
+    Lane many;
+    if (paged_attention_few(c.kv_dtype, c.head_size) && (long long)c.max_tokens * (c.n_q_heads / c.n_kv_heads) > FEW_ROWS) many = paged_prompt_lane(sms);
+    p->planner.init(c, few, many, FEW_ROWS);
     const size_t bytes = (size_t)p->planner.lay().total * 4;
     SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_plan, bytes));
     for (int i = 0; i < SLOTS; i++) {

@@ -62,6 +62,10 @@ paged::Lane paged_attention_lane(int kv_dtype, int hs, int sms);
 // One lane's kernel with `blocks` blocks, and the joins of at most `joins` pairs.
 int paged_attention_launch(slai_ctx* ctx, paged::AttnArgs& A, int kv_dtype, int lane, int blocks, int joins, bool pdl);
 
+// paged_prompt.cu
+paged::Lane paged_prompt_lane(int sms);
+int paged_prompt_launch(slai_ctx* ctx, const paged::AttnArgs& A, int blocks, bool pdl);
+
 // paged_append.cu
 struct QkArgs {
     int rows, counted;            // counted: there are as many rows as the step has when the kernel runs, `rows` at most

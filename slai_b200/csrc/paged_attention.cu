@@ -1,7 +1,7 @@
 // Causal attention of a step's new tokens to the keys and values that their sequences hold in pages: out = softmax(q K^T scale) V, each token over the
 // positions up to its own, a cache head shared by `group` query heads.  (The reference's operator has one token and one dense cache:
 // crates/slai/src/ops/batched_multiquery_attention.rs:32-156.)  Who computes what: paged_plan.h.
-#include "paged.cuh"
+#include "paged_rows.cuh"
 
 using namespace paged;
 
@@ -11,11 +11,6 @@ namespace {
 // 16 rows at a time, positions in tiles of 32 brought into shared memory as f32; warp w has rows 4w .. 4w + 3; scores: lane = position, sums of values:
 // lane = dimensions.  Plain f32 arithmetic, one pass with the running maximum and sum of each row.
 constexpr int GT = 128, GR = 16, GP = 32;
-
-template <typename T>
-__device__ __forceinline__ float to_float(T x);
-template <> __device__ __forceinline__ float to_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 
 template <typename T>
 __device__ __forceinline__ void load_rows(const T* base, const long long* place, int rows, int hs, int hsp, bool vec, float* s, int stride, int tid) {
@@ -268,43 +263,6 @@ int launch_join(slai_ctx* ctx, const AttnArgs& A, int joins, bool pdl) {
     return launch_dependent(ctx, paged_join_kernel<false>, dim3((unsigned)joins, (unsigned)((A.tile_rows + JW - 1) / JW)), JT, 0, pdl, A);
 }
 
-// ---- what the matrix units cannot carry ----------------------------------------------------------------------------------
-// The kernels below multiply whole tiles: a weight of zero times an infinite value that its row does not see would be NaN.  A row whose sums are not finite (this,
-// or the formula's own infinities and NaN) is computed again by one warp, position by position: [lo, hi) of the positions, as the formula says.
-template <typename T>
-__device__ __noinline__ void row_again(const AttnArgs& A, const Tile& t, int head, int r, int lo, int hi, float* out, float* ml) {
-    const Cache& c = A.c;
-    const int lane = threadIdx.x & 31, pr = t.first + r, tok = pr / c.group;
-    const float* q = A.q + (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * c.hs;
-    hi = min(hi, t.pos0 + tok + 1);
-    float m = -INFINITY, l = 0.f, acc[8] = {};
-    for (int p0 = lo; p0 < hi; p0 += 32) {
-        const bool seen = p0 + lane < hi;
-        const long long at = seen ? place_of(c, t.table, p0 + lane, head) : 0;
-        float s = 0.f;
-        if (seen)
-            for (int d = 0; d < c.hs; d++) s = fmaf(__ldcg(q + d) * A.scale, to_float<T>(reinterpret_cast<const T*>(c.keys)[at + d]), s);
-        float mt = seen ? s : -INFINITY;
-        for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-        const float m_new = fmaxf(m, mt), resc = m == -INFINITY ? 1.f : expf(m - m_new);
-        const float w = !seen || s == -INFINITY ? 0.f : expf(s - m_new);
-        float ws = w;
-        for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
-        l = l * resc + ws;
-        m = m_new;
-        for (int j = 0; j < 8; j++) acc[j] *= resc;
-        for (int i = 0; i < min(32, hi - p0); i++) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            const long long ai = __shfl_sync(0xffffffffu, at, i);
-            for (int j = 0; j < 8; j++)
-                if (lane + 32 * j < c.hs) acc[j] = fmaf(wi, to_float<T>(reinterpret_cast<const T*>(c.values)[ai + lane + 32 * j]), acc[j]);
-        }
-    }
-    for (int j = 0; j < 8; j++)
-        if (lane + 32 * j < c.hs) out[lane + 32 * j] = ml ? acc[j] : acc[j] / l;
-    if (ml && lane == 0) *reinterpret_cast<float2*>(ml) = make_float2(m * LOG2E, l);
-}
-
 // ---- PTX wrappers --------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -317,26 +275,6 @@ __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// v = hi + lo, 22 bits
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const __half2 l = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-}
-// 2^x, of the sizes weights have
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// The power of two that puts a row's largest query below 2^15, and its inverse: whatever their size they fit a pair of halves.
-__device__ __forceinline__ float power_up(float largest, float& unit) {
-    const int e = max((int)(__float_as_uint(largest) >> 23), 15);  // biased by 127
-    unit = __uint_as_float((uint32_t)(e - 14) << 23);
-    return __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
-}
-
 // ---- f16 caches, few rows: tokens of sequences that answer ---------------------------------------------------------------------
 // Up to 8 rows (a token's or a few tokens' query heads of one cache head).  Queries and weights are pairs of halves (22 bits); the 16 rows of the matrix
 // instruction are the 8 high parts and, below them, the 8 low ones, so one product does both and a lane holds both results of its row.  Sums end every 16
@@ -589,6 +527,7 @@ Lane paged_attention_lane(int kv_dtype, int hs, int sms) {
 }
 
 static int launch_lane(slai_ctx* ctx, const AttnArgs& A, int kv_dtype, int lane, int blocks, bool pdl) {
+    if (lane == 1 && A.vec) return paged_prompt_launch(ctx, A, blocks, pdl);
     if (lane == 0 && A.vec && paged_attention_few(kv_dtype, A.c.hs)) {
         if (A.c.page_size % FP == 0) return A.c.hs <= 64 ? launch_few<64, true>(ctx, A, blocks, pdl) : launch_few<128, true>(ctx, A, blocks, pdl);
         return A.c.hs <= 64 ? launch_few<64, false>(ctx, A, blocks, pdl) : launch_few<128, false>(ctx, A, blocks, pdl);
