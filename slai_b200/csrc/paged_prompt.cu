@@ -5,23 +5,26 @@
 // (22 bits), two products each: one rounding of either to f16 would put 1e-4 into the result, the pairs leave 3e-7.  The tensor core truncates when it adds:
 // both sums end with their 128 positions, and a half's output goes on in its threads' registers, times the factor by which the running maximum moved.
 //
-//   warps 0-1    keys, warps 2-3 values into a ring of three tiles of shared memory (asynchronous 16-byte copies that write the swizzle themselves: pages of any
-//                size, strides and order; positions behind the last are zeros)
-//   warps 4-7    half A: softmax, a row a thread: S out of tensor memory once for its maximum and once more for the weights, which take its columns' place as the
-//   warps 8-11   half B  next product's operand; then the product's result
-//   warp 12      issues the products: QK_A(j), PV_B(j-1), QK_B(j), PV_A(j): while one half's threads are at its softmax the tensor cores are at the other's
+//   warp 0       issues the products: QK_A(j), PV_B(j-1), QK_B(j), PV_A(j): while one half's threads are at its softmax the tensor cores are at the other's
 //                products.  Three regions of 128 columns of tensor memory hold scores and weights in turn, one the outputs.
+//   warps 1-3    keys and values of 128 positions, in turn, into a tile of shared memory each (asynchronous 16-byte copies that write the swizzle themselves:
+//                pages of any size, strides and order; positions behind the last are zeros)
+//   warps 4-11   half A, warps 12-19 half B: softmax, two threads a row, 64 positions and then 64 dimensions each: S out of tensor memory once for its maximum and once
+//                more for the weights, which take its columns' place as the next product's operand; then the product's result.  (With one thread a row its
+//                chain of latencies was 2.1 us a unit, twice what the other half's products hide.)
 // A region is written again by the third QK after its own; by then the PV that read it is complete: before each PV its issuer waits until the output of the PV
 // before has been read (one region for all of them), so that only the last PV issued can be under way.
 //
 // Every wait is bounded (common.cuh, bounded_wait).
+#include <type_traits>
+
 #include "paged_rows.cuh"
 
 using namespace paged;
 
 namespace {
 
-constexpr int PT = 512, PR = 128, PU = 128, PSLOTS = 3;  // threads, rows of a half, positions of a unit, tiles of keys or values in shared memory
+constexpr int PT = 640, PR = 128, PU = 128, PSLOTS = 3;  // threads, rows of a half, positions of a unit, tiles of keys or values in shared memory
 constexpr int ERR_PAGED = 7;
 constexpr float WEIGHT = 16.f;  // weights are carried 16 times their size: their low parts keep their bits, and the exponent's rounding stays below 2^-23
 
@@ -56,24 +59,41 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-#define R32(r) "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), \
-                "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),      \
-                "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-#define W32(r) "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),   \
-               "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),     \
-               "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-__device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
-                 "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : R32(r)
-                 : "r"(a)
-                 : "memory");
+#define R16(r) "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), \
+                "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+__device__ __forceinline__ void tmem_ld16(uint32_t a, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];" : R16(r) : "r"(a) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&r)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
-                 "%24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
-                 W32(r)
-                 : "memory");
+__device__ __forceinline__ void tmem_st4(uint32_t a, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+// Two f32 at a time
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 pack2(uint32_t a, uint32_t b) { return pack2(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -83,7 +103,14 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 template <int HS>
 struct Smem {
     static constexpr int BLOCK = 128 * 128, BLOCKS = HS / 64, Q = BLOCKS * BLOCK, TILE = BLOCKS * BLOCK;
-    static constexpr int RING = 4 * Q, TOTAL = RING + PSLOTS * TILE;
+    struct Rest {
+        unsigned long long bars[2 * PSLOTS + 10];
+        float max_s[4 * PR];  // what the two threads of a row tell one another
+        unsigned int bad_s[2][2][4];
+        uint32_t tmem_slot;
+    };
+    static constexpr int RING = 4 * Q, REST = RING + PSLOTS * TILE, TOTAL = REST + (int)sizeof(Rest);
+    static_assert(TOTAL <= 227 * 1024, "a block's shared memory");
 };
 
 // A block's part of one (tile, head) pair.
@@ -125,10 +152,17 @@ __device__ __forceinline__ void for_parts(const Start& s, const Cache& c, F f) {
 template <int HS>
 __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_constant__ AttnArgs A) {
     using L = Smem<HS>;
-    extern __shared__ unsigned char smem_dyn[];
-    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) unsigned long long bars[2 * PSLOTS + 10];
-    __shared__ uint32_t tmem_slot;
+    extern __shared__ __align__(1024) unsigned char smem_dyn[];  // (the kernel has no other shared memory: the operands begin on the swizzle's boundary)
+    unsigned char* smem = smem_dyn;
+    typename L::Rest& rest = *reinterpret_cast<typename L::Rest*>(smem + L::REST);
+    unsigned long long* bars = rest.bars;
+    uint32_t& tmem_slot = rest.tmem_slot;
+    float* max_s = rest.max_s;
+    auto& bad_s = rest.bad_s;
+    if (smem_u32(smem) & 1023) {
+        if (threadIdx.x == 0) atomicExch(A.err_flag, (unsigned int)ERR_PAGED);
+        return;
+    }
     const uint32_t sb = smem_u32(smem), ring = sb + L::RING;
     const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * PSLOTS, q_full = kv_empty + 8 * PSLOTS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
                    o_free = o_full + 16, all_done = o_free + 8;
@@ -136,21 +170,21 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hs = c.hs;
     if (tid == 0) {
         for (int i = 0; i < PSLOTS; i++) {
-            mbar_init(kv_full + 8 * i, 2);   // the two warps that fill a tile
+            mbar_init(kv_full + 8 * i, 1);
             mbar_init(kv_empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(q_full + 8 * i, 4);
+            mbar_init(q_full + 8 * i, 8);
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 4);
+            mbar_init(p_full + 8 * i, 8);
             mbar_init(o_full + 8 * i, 1);
         }
-        mbar_init(o_free, 4);
+        mbar_init(o_free, 8);
         mbar_init(all_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
     }
-    if (warp == 12) {
+    if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -165,49 +199,42 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
     auto wait = [&](uint32_t bar, uint32_t parity) { return bounded_wait<false, true, ERR_PAGED>(bar, parity & 1, limit, A.err_flag); };
 
     if (warp < 4) {
-        // ---- keys (warps 0, 1) and values (2, 3): tiles 0, 2, .. and 1, 3, .. of the ring's sequence ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        const bool value = warp >= 2;
-        const char* base = value ? c.values : c.keys;
-        const int r0 = 64 * (warp & 1);
-        constexpr int CH = HS / 8, STEP = 32 / CH;  // 16-byte pieces of a row, rows a pass of the warp covers
-        const int ch = lane % CH, rl = lane / CH, chunks = hs / 8;
-        int tile = value;  // of the sequence keys 0, values 0, keys 1, ..
-        for_parts(s, c, [&](const Tile& t, int head, const Part& p) {
-            const int hi = t.pos0 + (t.first + t.rows - 1) / c.group + 1;
-            auto place = [&](int j, int i) -> long long {  // of position 32 i + lane of this warp's 64, -1 behind the last
-                const int at = (p.unit + j) * PU + r0 + 32 * i + lane;
-                return at < hi ? 2 * place_of(c, t.table, at, head) : -1;
-            };
-            long long a0 = place(0, 0), a1 = place(0, 1);
-            for (int j = 0; j < p.n; j++, tile += 2) {
-                const int slot = tile % PSLOTS, round = tile / PSLOTS;
-                if (round > 0) wait(kv_empty + 8 * slot, round - 1);
-                if (!__any_sync(0xffffffffu, limit == 0)) {
-                    const uint32_t dst = ring + slot * L::TILE;
-#pragma unroll 8
-                    for (int k = 0; k < 64 / STEP; k++) {
-                        const int r = STEP * k + rl;  // of the warp's 64
-                        const long long a = __shfl_sync(0xffffffffu, k < 32 / STEP ? a0 : a1, r & 31);
-                        const int row = r0 + r;
-                        const uint32_t off = (ch >> 3) * L::BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4), bytes = a >= 0 && ch < chunks ? 16u : 0u;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + off), "l"(__cvta_generic_to_global(base + (bytes ? a + 16 * ch : 0))), "r"(bytes) : "memory");
-                    }
-                    if (j + 1 < p.n) {
-                        a0 = place(j + 1, 0);
-                        a1 = place(j + 1, 1);
-                    }
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp > 0) {
+            // ---- keys and values: tile i of the sequence keys 0, values 0, keys 1, .. is warp i % 3 + 1's, in its slot ----
+            const int slot = warp - 1;
+            constexpr int CH = HS / 8, STEP = 32 / CH;  // 16-byte pieces of a row, rows a pass of the warp covers
+            const int ch = lane % CH, rl = lane / CH, chunks = hs / 8;
+            const uint32_t dst0 = ring + slot * L::TILE + (ch >> 3) * L::BLOCK;
+            int next = slot, base = 0, round = 0;  // number of this warp's next tile, of the part's first
+            for_parts(s, c, [&](const Tile& t, int head, const Part& p) {
+                const int hi = t.pos0 + (t.first + t.rows - 1) / c.group + 1;
+                for (; next < base + 2 * p.n; next += PSLOTS, round++) {
+                    const int j = (next - base) >> 1, p0 = (p.unit + j) * PU;
+                    const char* from = (next - base) & 1 ? c.values : c.keys;
+                    long long at[4];  // places of positions 32 i + lane, -1 behind the last
+#pragma unroll
+                    for (int i = 0; i < 4; i++) at[i] = p0 + 32 * i + lane < hi ? 2 * place_of(c, t.table, p0 + 32 * i + lane, head) : -1;
+                    if (round > 0) wait(kv_empty + 8 * slot, round - 1);
+                    if (__any_sync(0xffffffffu, limit == 0)) continue;
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll 4
+                        for (int k = 0; k < 32 / STEP; k++) {
+                            const int r = STEP * k + rl, row = 32 * i + r;
+                            const long long a = __shfl_sync(0xffffffffu, at[i], r);
+                            const uint32_t off = row * 128 + (((ch & 7) ^ (row & 7)) << 4), bytes = a >= 0 && ch < chunks ? 16u : 0u;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst0 + off), "l"(__cvta_generic_to_global(from + (bytes ? a + 16 * ch : 0))), "r"(bytes) : "memory");
+                        }
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     fence_async();  // before the tensor core's reads
                     __syncwarp();
                     if (lane == 0) mbar_arrive(kv_full + 8 * slot);
                 }
-            }
-        });
-        asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 12) {
+                base += 2 * p.n;
+            });
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
             // ---- products ----
             const uint32_t id_qk = idesc(128, false), id_pv = idesc(HS, true);
             uint32_t n_q[2] = {0, 0}, n_s[2] = {0, 0}, n_pv = 0, qk = 0;  // phases: queries, scores of each half; outputs; scores of both
@@ -254,7 +281,7 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
                         for (int w = 1; w >= 0; w--)
 #pragma unroll
                             for (int k = 0; k < PU / 16; k++)
-                                umma_ts(out_cols, a + 32 * (k / 2) + 16 * w + 8 * (k % 2), desc_mn(b + 2048 * k, L::BLOCK), id_pv, w == 0 || k > 0);
+                                umma_ts(out_cols, a + 16 * k + 8 * w, desc_mn(b + 2048 * k, L::BLOCK), id_pv, w == 0 || k > 0);
                         umma_commit(o_full + 8 * h);
                         if (h == 1 || j >= p.nb) umma_commit(kv_empty + 8 * (vt % PSLOTS));
                     }
@@ -276,94 +303,129 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
             __syncwarp();
         }
     } else {
-        // ---- softmax: a row a thread ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int h = warp >= 8, q4 = warp & 3, r = 32 * q4 + lane;
-        const uint32_t lanes = (uint32_t)(32 * q4) << 16, mine = sb + h * 2 * L::Q;
-        unsigned char* mine_p = smem + h * 2 * L::Q;
+        // ---- softmax: two threads a row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int h = warp >= 12, q4 = warp & 3, g = (warp - 4) >> 2 & 1, r = 32 * q4 + lane, pair = 1 + 4 * h + q4;  // pair: the barrier of a quarter's two warps
+        constexpr int DH = HS / 2;  // dimensions a thread
+        const uint32_t lanes = (uint32_t)(32 * q4) << 16;
+        unsigned char* mine = smem + h * 2 * L::Q;
+        float* other = max_s + (2 * h + (g ^ 1)) * PR + r;
+        float* own = max_s + (2 * h + g) * PR + r;
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory"); };
         uint32_t n_s = 0, qk = 0;
         for_parts(s, c, [&](const Tile& t, int head, const Part& p) {
             const int n = h ? p.nb : p.na, rows = h ? p.rb : p.ra, row_first = t.first + PR * h;
-            float acc[HS];
-#pragma unroll
-            for (int d = 0; d < HS; d++) acc[d] = 0.f;
-            float m = -INFINITY, l = 0.f, cexp = 0.f;
-            const int vis = r < rows ? t.pos0 + (row_first + r) / c.group : -1;
+            const int pr = row_first + min(r, rows - 1), tok = pr / c.group, vis = r < rows ? t.pos0 + tok : -1;  // last position the row sees
+            const long long col = (long long)(head * c.group + pr % c.group) * hs;
+            float cexp = 0.f;
             if (n > 0) {
-                // queries: a warp brings one row after the other, 4 elements a lane
-#pragma unroll 4
-                for (int i = 0; i < 32; i++) {
-                    const int rr = 32 * q4 + i, pr = row_first + rr, tok = pr / c.group;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (rr < rows && 4 * lane < hs) {
-                        const float* q = A.q + (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs + 4 * lane;
-                        if (A.qvec) v = __ldcg(reinterpret_cast<const float4*>(q));
-                        else v = make_float4(__ldcg(q), __ldcg(q + 1), __ldcg(q + 2), __ldcg(q + 3));
-                    }
-                    v.x *= A.scale; v.y *= A.scale; v.z *= A.scale; v.w *= A.scale;
-                    float mx = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+                // queries: a warp brings 16 rows, 8 at a time, 4 elements a lane
+                const long long q_at = (t.row0 + tok) * A.q_ld + col;
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                    float unit;
-                    const float up = power_up(mx, unit);
-                    if (lane == i) cexp = unit * LOG2E;
-                    uint2 hi, lo;
-                    split2(v.x * up, v.y * up, hi.x, lo.x);
-                    split2(v.z * up, v.w * up, hi.y, lo.y);
-                    if (4 * lane < HS) {
-                        const int ch = (lane % 16) / 2, off = (lane / 16) * L::BLOCK + rr * 128 + ((ch ^ (rr & 7)) << 4) + 8 * (lane & 1);
-                        *reinterpret_cast<uint2*>(mine_p + off) = hi;
-                        *reinterpret_cast<uint2*>(mine_p + L::Q + off) = lo;
+                for (int i0 = 0; i0 < 16; i0 += 8) {
+                    float4 v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int rl = 16 * g + i0 + i;
+                        const float* q = A.q + __shfl_sync(0xffffffffu, q_at, rl) + 4 * lane;
+                        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (32 * q4 + rl < rows && 4 * lane < hs) {
+                            if (A.qvec) v[i] = __ldcg(reinterpret_cast<const float4*>(q));
+                            else v[i] = make_float4(__ldcg(q), __ldcg(q + 1), __ldcg(q + 2), __ldcg(q + 3));
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int rl = 16 * g + i0 + i, rr = 32 * q4 + rl;
+                        v[i].x *= A.scale; v[i].y *= A.scale; v[i].z *= A.scale; v[i].w *= A.scale;
+                        float mx = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        float unit;
+                        const float up = power_up(mx, unit);
+                        if (lane == rl) cexp = unit * LOG2E;
+                        uint2 hi, lo;
+                        split2(v[i].x * up, v[i].y * up, hi.x, lo.x);
+                        split2(v[i].z * up, v[i].w * up, hi.y, lo.y);
+                        if (4 * lane < HS) {
+                            const int ch = (lane % 16) / 2, off = (lane / 16) * L::BLOCK + rr * 128 + ((ch ^ (rr & 7)) << 4) + 8 * (lane & 1);
+                            *reinterpret_cast<uint2*>(mine + off) = hi;
+                            *reinterpret_cast<uint2*>(mine + L::Q + off) = lo;
+                        }
                     }
                 }
                 fence_async();
-                __syncwarp();
+                if (lane >> 4 == g) {  // the rows' units to both of their threads
+                    *own = cexp;
+                    *other = cexp;
+                }
+                meet();
+                cexp = *own;
                 if (lane == 0 && limit) mbar_arrive(q_full + 8 * h);
             }
+            f32x2 acc[DH / 2];
+#pragma unroll
+            for (int d = 0; d < DH / 2; d++) acc[d] = 0;
+            float m = -INFINITY, l = 0.f;
             for (int j = 0; j < n; j++) {
-                const uint32_t reg = tmem + 128 * ((qk + j + (h == 0 ? min(j, p.nb) : min(j + 1, p.na))) % 3) + lanes;
-                const int p0 = (p.unit + j) * PU;
+                const uint32_t reg = tmem + 128 * ((qk + j + (h == 0 ? min(j, p.nb) : min(j + 1, p.na))) % 3) + lanes + 64 * g;
+                const int p0 = (p.unit + j) * PU + 64 * g;
                 wait(s_full + 8 * h, n_s);
                 __syncwarp();
                 tc_after();
-                const bool all_seen = __all_sync(0xffffffffu, vis >= p0 + PU - 1);
-                float mx = -INFINITY;
+                float resc;
+                auto weights = [&](auto all_seen) {
+                    constexpr bool ALL = decltype(all_seen)::value;
+                    const int seen = vis - p0;  // positions 0 .. seen of this thread's 64
+                    float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    uint32_t x[32];
-                    tmem_ld32(reg + 32 * k, x);
-                    tmem_wait_ld();
-                    if (all_seen) {
+                    for (int k = 0; k < 2; k++) {
+                        uint32_t x[2][16];
+                        tmem_ld16(reg + 32 * k, x[0]);
+                        tmem_ld16(reg + 32 * k + 16, x[1]);
+                        tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(x[i]));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) mx = fmaxf(mx, p0 + 32 * k + i <= vis ? __uint_as_float(x[i]) : -INFINITY);
-                    }
-                }
-                const float m_new = fmaxf(m, mx * cexp), base = m_new == -INFINITY ? 0.f : m_new, resc = ex2(m - base);
-                m = m_new;
-                const float shift = 4.f - base;  // log2(WEIGHT)
-                float ps[4] = {};
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    uint32_t x[32], y[32];
-                    tmem_ld32(reg + 32 * k, x);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float e0 = ex2(fmaf(__uint_as_float(x[i]), cexp, shift)), e1 = ex2(fmaf(__uint_as_float(x[i + 1]), cexp, shift));
-                        if (!all_seen) {
-                            e0 = p0 + 32 * k + i <= vis ? e0 : 0.f;
-                            e1 = p0 + 32 * k + i + 1 <= vis ? e1 : 0.f;
+                        for (int i = 0; i < 32; i += 2) {
+                            const float a = __uint_as_float(x[i >> 4][i & 15]), b = __uint_as_float(x[i >> 4][(i & 15) + 1]);
+                            mx[(i >> 1) & 1] = max3(mx[(i >> 1) & 1], ALL || 32 * k + i <= seen ? a : -INFINITY, ALL || 32 * k + i + 1 <= seen ? b : -INFINITY);
                         }
-                        ps[(i >> 1) & 3] += e0 + e1;
-                        const int at = (i >> 4) * 8 + ((i & 15) >> 1);  // 16 positions: 8 columns of high parts; 16 further on the low ones
-                        split2(e0, e1, y[at], y[16 + at]);
                     }
-                    tmem_st32(reg + 32 * k, y);
-                }
-                l = l * resc + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
+                    *own = fmaxf(mx[0], mx[1]);
+                    meet();
+                    const float m_new = fmaxf(m, fmaxf(*own, *other) * cexp), base = m_new == -INFINITY ? 0.f : m_new;
+                    resc = ex2(m - base);
+                    m = m_new;
+                    const f32x2 shift = pack2(4.f - base, 4.f - base), slope = pack2(cexp, cexp);  // log2(WEIGHT)
+                    f32x2 ps[2] = {0, 0};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t x[16];
+                        tmem_ld16(reg + 16 * k, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            uint32_t hi[4], lo[4];  // of 16 positions: 8 columns of high parts, 8 of low ones
+#pragma unroll
+                            for (int i = 0; i < 8; i += 2) {
+                                const float2 e = unpack2(fma2(pack2(x[8 * u + i], x[8 * u + i + 1]), slope, shift));
+                                const int at = 16 * k + 8 * u + i;
+                                const float a = ALL || at <= seen ? ex2(e.x) : 0.f, b = ALL || at + 1 <= seen ? ex2(e.y) : 0.f;
+                                ps[(i >> 1) & 1] = add2(ps[(i >> 1) & 1], pack2(a, b));
+                                // the high part: the upper 11 bits, exactly an f16; the low part: the rest, rounded to one
+                                const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+                                const __half2 hh = __floats2half2_rn(ah, bh), ll = __floats2half2_rn(a - ah, b - bh);
+                                hi[i >> 1] = *reinterpret_cast<const uint32_t*>(&hh);
+                                lo[i >> 1] = *reinterpret_cast<const uint32_t*>(&ll);
+                            }
+                            tmem_st4(reg + 16 * k + 4 * u, hi);
+                            tmem_st4(reg + 16 * k + 8 + 4 * u, lo);
+                        }
+                    }
+                    const float2 sum = unpack2(add2(ps[0], ps[1]));
+                    l = l * resc + (sum.x + sum.y);  // (this thread's positions)
+                };
+                if (__all_sync(0xffffffffu, vis >= p0 + 63)) weights(std::true_type());
+                else weights(std::false_type());
                 tmem_wait_st();
                 tc_before();
                 __syncwarp();
@@ -371,13 +433,15 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
                 wait(o_full + 8 * h, n_s);
                 __syncwarp();
                 tc_after();
+                const f32x2 by = pack2(resc, resc);
 #pragma unroll
-                for (int k = 0; k < HS / 32; k++) {
-                    uint32_t x[32];
-                    tmem_ld32(out_cols + lanes + 32 * k, x);
+                for (int k = 0; k < DH / 32; k++) {
+                    uint32_t o[2][16];
+                    tmem_ld16(out_cols + lanes + DH * g + 32 * k, o[0]);
+                    tmem_ld16(out_cols + lanes + DH * g + 32 * k + 16, o[1]);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; i++) acc[32 * k + i] = fmaf(acc[32 * k + i], resc, __uint_as_float(x[i]));
+                    for (int i = 0; i < 16; i++) acc[16 * k + i] = fma2(acc[16 * k + i], by, pack2(o[i >> 3][2 * i & 15], o[i >> 3][(2 * i & 15) + 1]));
                 }
                 tc_before();
                 __syncwarp();
@@ -386,46 +450,67 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
             }
             qk += p.na + p.nb;
             // ---- results: through shared memory (the queries' place), so that a row leaves in one piece ----
-            const float f = p.whole ? 1.f / l : 1.f / WEIGHT;
+            meet();  // (both have read the last maxima)
+            *own = l;
+            meet();
+            l += *other;
             float sum = l;
 #pragma unroll
-            for (int d = 0; d < HS; d++) sum += acc[d];
+            for (int d = 0; d < DH / 2; d++) {
+                const float2 v = unpack2(acc[d]);
+                sum += v.x + v.y;
+            }
             const unsigned int bad = __ballot_sync(0xffffffffu, r < rows && !(fabsf(sum) < INFINITY));
-            float4* so = reinterpret_cast<float4*>(mine_p) + r * (HS / 4);
-            __syncwarp();
+            const float f = p.whole ? 1.f / l : 1.f / WEIGHT;
+            float4* so = reinterpret_cast<float4*>(mine) + r * (HS / 4);
 #pragma unroll
-            for (int d = 0; d < HS / 4; d++) so[d ^ (lane & (HS / 4 - 1))] = make_float4(acc[4 * d] * f, acc[4 * d + 1] * f, acc[4 * d + 2] * f, acc[4 * d + 3] * f);
-            __syncwarp();
+            for (int d = 0; d < DH / 4; d++) {
+                const float2 v = unpack2(acc[2 * d]), w = unpack2(acc[2 * d + 1]);
+                so[(DH / 4 * g + d) ^ (lane & (HS / 4 - 1))] = make_float4(v.x * f, v.y * f, w.x * f, w.y * f);
+            }
+            if (lane == 0) bad_s[h][g][q4] = bad;
             const size_t slot = ((size_t)s.me * 2 + (p.unit == 0)) * A.tile_rows + PR * h;
-            if (!p.whole && r < rows) *reinterpret_cast<float2*>(A.part_ml + (slot + r) * 2) = make_float2(m, l / WEIGHT);
-            for (int i = 0; i < 32 && 32 * q4 + i < rows; i++) {
-                const int rr = 32 * q4 + i, pr = row_first + rr, tok = pr / c.group;
-                float* o = p.whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs : A.part + (slot + rr) * hs;
-                if (bad >> i & 1) {
-                    row_again<__half>(A, t, head, PR * h + rr, p.unit * PU, (p.unit + p.n) * PU, o, p.whole ? nullptr : A.part_ml + (slot + rr) * 2);
-                } else if (4 * lane < hs) {
-                    const float4 v = reinterpret_cast<const float4*>(mine_p)[rr * (HS / 4) + (lane ^ (i & (HS / 4 - 1)))];
-                    if (!p.whole || A.qvec) {
-                        *reinterpret_cast<float4*>(o + 4 * lane) = v;
+            if (!p.whole && g == 0 && r < rows) *reinterpret_cast<float2*>(A.part_ml + (slot + r) * 2) = make_float2(m, l / WEIGHT);
+            meet();
+            float* o_at = p.whole ? A.out + (t.row0 + tok) * A.out_ld + col : A.part + (slot + min(r, rows - 1)) * hs;
+            const bool vec = !p.whole || A.qvec;
+#pragma unroll 8
+            for (int i = 0; i < 16; i++) {
+                const int rl = 16 * g + i, rr = 32 * q4 + rl;
+                float* o = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o_at), rl)) + 4 * lane;
+                if (rr < rows && 4 * lane < hs) {
+                    const float4 v = reinterpret_cast<const float4*>(mine)[rr * (HS / 4) + (lane ^ (rl & (HS / 4 - 1)))];
+                    if (vec) {
+                        *reinterpret_cast<float4*>(o) = v;
                     } else {
-                        o[4 * lane] = v.x; o[4 * lane + 1] = v.y; o[4 * lane + 2] = v.z; o[4 * lane + 3] = v.w;
+                        o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
                     }
                 }
             }
-            if (h) asm volatile("bar.sync 2, 128;" ::: "memory");  // the next queries lie across the four warps' results
-            else asm volatile("bar.sync 1, 128;" ::: "memory");
+            const unsigned int again = bad_s[h][0][q4] | bad_s[h][1][q4];
+            if (again) {
+                __syncwarp();
+                for (int i = 16 * g; i < 16 * g + 16; i++)
+                    if (again >> i & 1) {
+                        float* o = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o_at), i));
+                        row_again<__half>(A, t, head, PR * h + 32 * q4 + i, p.unit * PU, (p.unit + p.n) * PU, o,
+                                          p.whole ? nullptr : A.part_ml + (slot + 32 * q4 + i) * 2);
+                    }
+            }
+            if (h) asm volatile("bar.sync 10, 256;" ::: "memory");  // the next queries lie across the eight warps' results
+            else asm volatile("bar.sync 9, 256;" ::: "memory");
         });
     }
     __syncwarp();
     tc_before();
     __syncthreads();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 template <int HS>
 int launch(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
     auto kern = paged_attn_prompt_kernel<HS>;
-    constexpr int bytes = Smem<HS>::TOTAL + 1024;
+    constexpr int bytes = Smem<HS>::TOTAL;
     static PerDeviceOnce attr;
     if (attr.need(ctx->device)) {
         SLAI_CHECK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
