@@ -245,6 +245,7 @@ SLAI_API int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, 
     A.scale = scale == 0.f ? (float)(1.0 / sqrt((double)c.head_size)) : scale;
     A.q = d_q;
     A.out = d_out;
+    A.n_pages = c.n_pages;
     const int esz = c.kv_dtype == SLAI_KV_F16 ? 2 : 4;
     const uintptr_t bits = (uintptr_t)layer->d_keys | (uintptr_t)layer->d_values | (uintptr_t)(layer->page_stride * esz) | (uintptr_t)(layer->head_stride * esz) |
                            (uintptr_t)(layer->pos_stride * esz) | (uintptr_t)(c.head_size * esz);

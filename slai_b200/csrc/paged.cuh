@@ -21,6 +21,7 @@ struct AttnArgs {
     float* out;
     long long q_ld, out_ld;  // floats between tokens
     float scale;
+    int n_pages;
     int tile_rows, unit;     // of the lane
     int vec;                 // rows of the cache can be read in 16-byte pieces
     int qvec;                // ... and rows of q and out

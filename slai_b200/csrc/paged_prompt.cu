@@ -7,8 +7,10 @@
 //
 //   warp 0       issues the products: QK_A(j), PV_B(j-1), QK_B(j), PV_A(j): while one half's threads are at its softmax the tensor cores are at the other's
 //                products.  Three regions of 128 columns of tensor memory hold scores and weights in turn, one the outputs.
-//   warps 1-3    keys and values of 128 positions, in turn, into a tile of shared memory each (asynchronous 16-byte copies that write the swizzle themselves:
-//                pages of any size, strides and order; positions behind the last are zeros)
+//   warps 1-3    keys and values of 128 positions, in turn, into a tile of shared memory each: by TMA, a box per page, where pages divide 128 positions or are
+//                divided by them, else (and where a sequence ends inside the tile: positions behind the last are zeros, whatever the page holds there) by
+//                asynchronous 16-byte copies that write the swizzle themselves.  (All by the latter, a tile took as long as the two products that hide it: 522 us for
+//                1023 tokens of 64 heads on 8 at position 7001.)
 //   warps 4-11   half A, warps 12-19 half B: softmax, two threads a row, 64 positions and then 64 dimensions each: S out of tensor memory once for its maximum and once
 //                more for the weights, which take its columns' place as the next product's operand; then the product's result.  (With one thread a row its
 //                chain of latencies was 2.1 us a unit, twice what the other half's products hide.)
@@ -17,6 +19,8 @@
 //
 // Every wait is bounded (common.cuh, bounded_wait).
 #include <type_traits>
+
+#include <cuda.h>
 
 #include "paged_rows.cuh"
 
@@ -32,6 +36,14 @@ constexpr float WEIGHT = 16.f;  // weights are carried 16 times their size: thei
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t a, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(a), "r"(count) : "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint32_t a) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory"); }
+__device__ __forceinline__ void mbar_expect_tx(uint32_t a, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t mbar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(mbar), "r"(x),
+                 "r"(y), "r"(z), "r"(w)
+                 : "memory");
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -150,7 +162,8 @@ __device__ __forceinline__ void for_parts(const Start& s, const Cache& c, F f) {
 }
 
 template <int HS>
-__global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap map_k,
+                                                                  const __grid_constant__ CUtensorMap map_v, const int box) {
     using L = Smem<HS>;
     extern __shared__ __align__(1024) unsigned char smem_dyn[];  // (the kernel has no other shared memory: the operands begin on the swizzle's boundary)
     unsigned char* smem = smem_dyn;
@@ -212,6 +225,26 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
                 for (; next < base + 2 * p.n; next += PSLOTS, round++) {
                     const int j = (next - base) >> 1, p0 = (p.unit + j) * PU;
                     const char* from = (next - base) & 1 ? c.values : c.keys;
+                    if (box > 0 && p0 + PU <= hi) {
+                        // a page is a box of `box` rows and 64 dimensions; lane i has the number of the tile's i-th
+                        const int i_page = p0 / c.page_size, boxes = PU / box;
+                        const int id = lane < boxes ? __ldcg(c.plan + t.table + i_page + (lane * box) / c.page_size) : 0;
+                        if (round > 0) wait(kv_empty + 8 * slot, round - 1);
+                        if (__any_sync(0xffffffffu, limit == 0)) continue;
+                        if (elect_one()) mbar_expect_tx(kv_full + 8 * slot, L::TILE);
+                        __syncwarp();
+                        for (int i = 0; i < boxes; i++) {
+                            const int page = __shfl_sync(0xffffffffu, id, i);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int d = 0; d < L::BLOCKS; d++)
+                                    tma_load_4d(ring + slot * L::TILE + d * L::BLOCK + i * box * 128, (next - base) & 1 ? &map_v : &map_k, 64 * d, (p0 + i * box) % c.page_size, head, page,
+                                                kv_full + 8 * slot);
+                            }
+                            __syncwarp();
+                        }
+                        continue;
+                    }
                     long long at[4];  // places of positions 32 i + lane, -1 behind the last
 #pragma unroll
                     for (int i = 0; i < 4; i++) at[i] = p0 + 32 * i + lane < hi ? 2 * place_of(c, t.table, p0 + 32 * i + lane, head) : -1;
@@ -234,6 +267,8 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
                 base += 2 * p.n;
             });
             asm volatile("cp.async.wait_all;" ::: "memory");
+            limit = LAST_POLLS;
+            if (round > 0) wait(kv_full + 8 * slot, round - 1);  // the last copy lands before the block ends
         } else {
             // ---- products ----
             const uint32_t id_qk = idesc(128, false), id_pv = idesc(HS, true);
@@ -507,6 +542,29 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
+// ---- host side -----------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled() {
+    static EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
+}
+// Pages as [page][head][position][dimension], whatever their order in memory, in boxes of 64 dimensions of `rows` positions.
+bool make_map(CUtensorMap* map, const AttnArgs& A, const void* base, int rows) {
+    const EncodeTiledFn enc = encode_tiled();
+    const Cache& c = A.c;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.hs, (cuuint64_t)c.page_size, (cuuint64_t)c.n_kv, (cuuint64_t)A.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.pos_stride * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)rows, 1, 1}, elem[4] = {1, 1, 1, 1};
+    return enc && enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int HS>
 int launch(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
     auto kern = paged_attn_prompt_kernel<HS>;
@@ -516,7 +574,12 @@ int launch(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
         SLAI_CHECK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
         attr.set(ctx->device);
     }
-    return launch_dependent(ctx, kern, dim3((unsigned)blocks), PT, bytes, pdl, A);
+    // (a stride that the copy engine does not take, 2^40 bytes and more: by 16-byte copies)
+    const int ps = A.c.page_size;
+    int box = ps % PU == 0 ? PU : ps >= 8 && PU % ps == 0 ? ps : 0;
+    CUtensorMap k = {}, v = {};
+    if (box > 0 && !(make_map(&k, A, A.c.keys, box) && make_map(&v, A, A.c.values, box))) box = 0;
+    return launch_dependent(ctx, kern, dim3((unsigned)blocks), PT, bytes, pdl, A, k, v, box);
 }
 
 }  // namespace
