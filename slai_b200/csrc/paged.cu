@@ -264,7 +264,8 @@ SLAI_API int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, 
         A.unit = l.unit;
         A.part = p->d_part[k];
         A.part_ml = p->d_ml[k];
-        if ((rc = paged_attention_launch(ctx, A, c.kv_dtype, k, recording ? l.blocks : p->step.blocks[k], recording ? l.blocks : p->step.joins[k], ctx->use_pdl))) return rc;
+        if ((rc = paged_attention_launch(ctx, A, c.kv_dtype, k, recording ? l.blocks : p->step.blocks[k], recording ? l.blocks : p->step.joins[k],
+                                         recording ? l.blocks : p->step.longest[k], ctx->use_pdl))) return rc;
     }
     return SLAI_OK;
 }

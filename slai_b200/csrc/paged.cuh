@@ -60,8 +60,8 @@ __device__ __forceinline__ long long place_of(const Cache& c, int table, int p, 
 
 bool paged_attention_few(int kv_dtype, int hs);
 paged::Lane paged_attention_lane(int kv_dtype, int hs, int sms);
-// One lane's kernel with `blocks` blocks, and the joins of at most `joins` pairs.
-int paged_attention_launch(slai_ctx* ctx, paged::AttnArgs& A, int kv_dtype, int lane, int blocks, int joins, bool pdl);
+// One lane's kernel with `blocks` blocks, and the joins of at most `joins` pairs of at most `longest` results.
+int paged_attention_launch(slai_ctx* ctx, paged::AttnArgs& A, int kv_dtype, int lane, int blocks, int joins, int longest, bool pdl);
 
 // paged_prompt.cu
 paged::Lane paged_prompt_lane(int sms);

@@ -185,82 +185,164 @@ int launch_any(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
 // Rows of a tile: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the blocks' results in the order of their positions (a block that saw nothing of a row
 // has m = -inf, l = 0, o = 0).  A launch of its own behind the other's end, whose blocks read all results at once: done by the block that comes last, a
 // token over 32750 positions (37 blocks a pair) took 12 us from its loop's end to the result, and over 515 positions 5.
-constexpr int JT = 128, JW = JT / 32;
-// SPLIT: a block takes one row, its warps every JW-th result; else a warp takes a row.
-template <bool SPLIT>
-__global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs A) {
+__device__ __forceinline__ float join_weight(float m, float M) { return m == -INFINITY ? 0.f : exp2f(m - M); }
+struct JoinOf {  // one pair
+    int row0, first, rows, head, begin, nb;
+};
+__device__ __forceinline__ bool load_join(const AttnArgs& A, JoinOf& j) {
+    const int4* g = reinterpret_cast<const int4*>(A.c.plan + A.joins_at) + 2 * blockIdx.x;
+    const int4 a = __ldcg(g), b = __ldcg(g + 1);
+    j = {a.x, a.y, a.z, a.w, b.x, b.y - b.x + 1};
+    return (int)blockIdx.x < __ldcg(A.c.plan + A.count_at);
+}
+__device__ __forceinline__ size_t part_slot(const AttnArgs& A, const JoinOf& j, int i, int r) { return ((size_t)(j.begin + i) * 2 + (i == 0)) * A.tile_rows + r; }
+__device__ __forceinline__ float* join_out(const AttnArgs& A, const JoinOf& j, int r) {
+    const int pr = j.first + r, tok = pr / A.c.group;
+    return A.out + (j.row0 + tok) * A.out_ld + (long long)(j.head * A.c.group + pr % A.c.group) * A.c.hs;
+}
+// elements d .. d + 3 of a result where heads are whole quads, else d
+__device__ __forceinline__ float4 join_load(const AttnArgs& A, size_t slot, int d, bool quads) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (d >= A.c.hs) return o;
+    if (quads) return __ldcg(reinterpret_cast<const float4*>(A.part + slot * A.c.hs + d));
+    o.x = __ldcg(A.part + slot * A.c.hs + d);
+    return o;
+}
+__device__ __forceinline__ void join_add(float4& a, float f, float4 o) {
+    a.x = fmaf(f, o.x, a.x); a.y = fmaf(f, o.y, a.y); a.z = fmaf(f, o.z, a.z); a.w = fmaf(f, o.w, a.w);
+}
+
+// A few results to a pair: a warp takes four rows; eight lanes of it have a row's weights.
+constexpr int JT = 64, JR = 4, JROWS = JT / 32 * JR;
+__global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ AttnArgs A) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hs = A.c.hs;
-    const int4* g = reinterpret_cast<const int4*>(A.c.plan + A.joins_at) + 2 * blockIdx.x;
-    const int4 j0 = __ldcg(g), j1 = __ldcg(g + 1);  // row0, first, rows, head; begin, end
-    const bool none = (int)blockIdx.x >= __ldcg(A.c.plan + A.count_at);
+    JoinOf j;
+    const bool on = load_join(A, j);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (none) return;
-    const int r = SPLIT ? (int)blockIdx.y : (int)blockIdx.y * JW + warp, nb = j1.y - j1.x + 1;
-    if (r >= j0.z) return;
-    auto slot = [&](int i) { return ((size_t)(j1.x + i) * 2 + (i == 0)) * A.tile_rows + r; };
+    const int r0 = (int)blockIdx.y * JROWS + warp * JR, n = min(JR, j.rows - r0);
+    if (!on || n <= 0) return;
     const float2* ml = reinterpret_cast<const float2*>(A.part_ml);
-    constexpr int STEP = SPLIT ? JW : 1;
-    const int b_first = SPLIT ? warp : 0;
+    const int mine = min(lane >> 3, n - 1), b8 = lane & 7;
     const bool quads = hs % 4 == 0;
-    __shared__ float num_s[SPLIT ? JW : 1][256];
-    __shared__ float den_s[JW];
-    float M = -INFINITY;
-    for (int b = lane; b < nb; b += 32) M = fmaxf(M, __ldcg(ml + slot(b)).x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const int pr = j0.y + r, tok = pr / A.c.group;
-    float* out = A.out + (j0.x + tok) * A.out_ld + (long long)(j0.w * A.c.group + pr % A.c.group) * hs;
     for (int d0 = 0; d0 < hs; d0 += quads ? 128 : 32) {
         const int d = d0 + (quads ? 4 * lane : lane);
-        float num[4] = {}, den = 0.f;
-        for (int b0 = b_first; b0 < nb; b0 += 8 * STEP) {
-            float4 o[8];
-            float2 y[8];
+        float4 num[JR];
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const int b = b0 + u * STEP;
-                o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                y[u] = make_float2(-INFINITY, 0.f);
-                if (b < nb) {
-                    y[u] = __ldcg(ml + slot(b));
-                    const float* p = A.part + slot(b) * hs + d;
-                    if (quads && d < hs) o[u] = __ldcg(reinterpret_cast<const float4*>(p));
-                    else if (d < hs) o[u].x = __ldcg(p);
+        for (int r = 0; r < JR; r++) num[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.f, M = -INFINITY;
+        for (int c0 = 0; c0 < j.nb; c0 += 8) {  // eight results at a time, with a running maximum; loads first, all at once
+            const float2 y = c0 + b8 < j.nb ? __ldcg(ml + part_slot(A, j, c0 + b8, r0 + mine)) : make_float2(-INFINITY, 0.f);
+            const int m = min(8, j.nb - c0);
+            float4 o[2][JR];
+            auto load = [&](int u) {
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int r = 0; r < JR; r++) o[k][r] = join_load(A, part_slot(A, j, c0 + min(u + k, m - 1), r0 + min(r, n - 1)), d, quads);
+            };
+            load(0);
+            float Mn = y.x;
+#pragma unroll
+            for (int i = 4; i > 0; i >>= 1) Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, i));
+            Mn = fmaxf(M, Mn);
+            const float f = join_weight(y.x, Mn), resc = join_weight(M, Mn);
+            M = Mn;
+            den = fmaf(den, resc, f * y.y);
+            if (c0 > 0) {
+#pragma unroll
+                for (int r = 0; r < JR; r++) {
+                    const float by = __shfl_sync(0xffffffffu, resc, 8 * r);
+                    num[r].x *= by; num[r].y *= by; num[r].z *= by; num[r].w *= by;
                 }
             }
+            for (int u = 0; u < m; u += 2) {
+                if (u > 0) load(u);
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const float f = y[u].x == -INFINITY ? 0.f : exp2f(y[u].x - M);
-                den = fmaf(f, y[u].y, den);
-                num[0] = fmaf(f, o[u].x, num[0]); num[1] = fmaf(f, o[u].y, num[1]); num[2] = fmaf(f, o[u].z, num[2]); num[3] = fmaf(f, o[u].w, num[3]);
+                for (int k = 0; k < 2; k++)
+                    if (u + k < m) {
+#pragma unroll
+                        for (int r = 0; r < JR; r++) join_add(num[r], __shfl_sync(0xffffffffu, f, 8 * r + u + k), o[k][r]);
+                    }
             }
         }
-        if (!SPLIT) {
-            for (int e = 0; e < (quads ? 4 : 1) && d < hs; e++) out[d + e] = num[e] / den;
-        } else {
-            for (int e = 0; e < (quads ? 4 : 1) && d < hs; e++) num_s[warp][d + e] = num[e];
-            if (lane == 0) den_s[warp] = den;
-        }
-    }
-    if (SPLIT) {
-        __syncthreads();
-        for (int d = threadIdx.x; d < hs; d += JT) {
-            float n = 0.f, den = 0.f;
 #pragma unroll
-            for (int w = 0; w < JW; w++) {
-                n += num_s[w][d];
-                den += den_s[w];
+        for (int i = 4; i > 0; i >>= 1) den += __shfl_xor_sync(0xffffffffu, den, i);
+#pragma unroll
+        for (int r = 0; r < JR; r++) {
+            const float by = 1.f / __shfl_sync(0xffffffffu, den, 8 * r);
+            if (r < n && d < hs) {
+                float* o = join_out(A, j, r0 + r) + d;
+                if (quads && A.qvec) {
+                    *reinterpret_cast<float4*>(o) = make_float4(num[r].x * by, num[r].y * by, num[r].z * by, num[r].w * by);
+                } else {
+                    const float v[4] = {num[r].x, num[r].y, num[r].z, num[r].w};
+                    for (int e = 0; e < (quads ? 4 : 1); e++) o[e] = v[e] * by;
+                }
             }
-            out[d] = n / den;
         }
     }
 }
 
-int launch_join(slai_ctx* ctx, const AttnArgs& A, int joins, bool pdl) {
+// Many results to a pair (one long sequence over many blocks): a block takes a row, its warps every LW-th result.
+constexpr int LT = 128, LW = LT / 32, JOIN_MANY = 8;
+__global__ void __launch_bounds__(LT) paged_join_many_kernel(const __grid_constant__ AttnArgs A) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hs = A.c.hs, r = (int)blockIdx.y;
+    JoinOf j;
+    const bool on = load_join(A, j);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!on || r >= j.rows) return;
+    const float2* ml = reinterpret_cast<const float2*>(A.part_ml);
+    __shared__ float num_s[LW][256];
+    __shared__ float den_s[LW];
+    float M = -INFINITY;
+    for (int b = lane; b < j.nb; b += 32) M = fmaxf(M, __ldcg(ml + part_slot(A, j, b, r)).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const bool quads = hs % 4 == 0;
+    for (int d0 = 0; d0 < hs; d0 += quads ? 128 : 32) {
+        const int d = d0 + (quads ? 4 * lane : lane);
+        float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.f;
+        for (int b0 = warp; b0 < j.nb; b0 += 8 * LW) {
+            float4 o[8];
+            float2 y[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int b = b0 + u * LW;
+                y[u] = b < j.nb ? __ldcg(ml + part_slot(A, j, b, r)) : make_float2(-INFINITY, 0.f);
+                o[u] = join_load(A, part_slot(A, j, min(b, j.nb - 1), r), b < j.nb ? d : hs, quads);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float f = join_weight(y[u].x, M);
+                den = fmaf(f, y[u].y, den);
+                join_add(num, f, o[u]);
+            }
+        }
+        const float v[4] = {num.x, num.y, num.z, num.w};
+        for (int e = 0; e < (quads ? 4 : 1) && d < hs; e++) num_s[warp][d + e] = v[e];
+        if (lane == 0) den_s[warp] = den;
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < hs; d += LT) {
+        float n = 0.f, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < LW; w++) {
+            n += num_s[w][d];
+            den += den_s[w];
+        }
+        join_out(A, j, r)[d] = n / den;
+    }
+}
+
+// `longest`: most results of a pair.  us of the call, a warp for four rows / a block for each: 272 pairs of 2 or 3 results of 8 rows 98.8 / 102; 8 pairs of 37 results
+// 38.8 / 32.5; 141 pairs of 2 or 3 of 256 rows 475 / 494.
+int launch_join(slai_ctx* ctx, const AttnArgs& A, int joins, int longest, bool pdl) {
     if (joins <= 0) return SLAI_OK;
-    if (A.tile_rows <= 16) return launch_dependent(ctx, paged_join_kernel<true>, dim3((unsigned)joins, (unsigned)A.tile_rows), JT, 0, pdl, A);
-    return launch_dependent(ctx, paged_join_kernel<false>, dim3((unsigned)joins, (unsigned)((A.tile_rows + JW - 1) / JW)), JT, 0, pdl, A);
+    if (longest > JOIN_MANY && A.tile_rows <= 16) return launch_dependent(ctx, paged_join_many_kernel, dim3((unsigned)joins, (unsigned)A.tile_rows), LT, 0, pdl, A);
+    return launch_dependent(ctx, paged_join_kernel, dim3((unsigned)joins, (unsigned)((A.tile_rows + JROWS - 1) / JROWS)), JT, 0, pdl, A);
 }
 
 // ---- PTX wrappers --------------------------------------------------------------------------------------------------------
@@ -534,8 +616,8 @@ static int launch_lane(slai_ctx* ctx, const AttnArgs& A, int kv_dtype, int lane,
     }
     return kv_dtype == SLAI_KV_F16 ? launch_any<__half>(ctx, A, blocks, pdl) : launch_any<float>(ctx, A, blocks, pdl);
 }
-int paged_attention_launch(slai_ctx* ctx, AttnArgs& A, int kv_dtype, int lane, int blocks, int joins, bool pdl) {
+int paged_attention_launch(slai_ctx* ctx, AttnArgs& A, int kv_dtype, int lane, int blocks, int joins, int longest, bool pdl) {
     if (blocks <= 0) return SLAI_OK;
     const int rc = launch_lane(ctx, A, kv_dtype, lane, blocks, pdl);
-    return rc ? rc : launch_join(ctx, A, joins, pdl);
+    return rc ? rc : launch_join(ctx, A, joins, longest, pdl);
 }

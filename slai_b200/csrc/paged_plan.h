@@ -77,7 +77,8 @@ inline Layout layout(const Config& c, const Lane (&lanes)[2]) {
 struct Step {
     int n_rows = -1;          // -1: there has been no step
     int blocks[2] = {0, 0};   // blocks with work
-    int joins[2] = {0, 0};
+    int joins[2] = {0, 0};    // pairs on several blocks
+    int longest[2] = {0, 0};  // most blocks of one
     int used = 0;             // ints of the dynamic part
 };
 
@@ -221,6 +222,7 @@ class Planner {
                         j.begin = block(at + PAIR_COST);
                         j.end = block(at + pair - 1);
                         jo[joins++] = j;
+                        step->longest[k] = std::max(step->longest[k], j.end - j.begin + 1);
                         known = at;
                     }
                 }

@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
         uint32_t n_s = 0, qk = 0;
         for_parts(s, c, [&](const Tile& t, int head, const Part& p) {
             const int n = h ? p.nb : p.na, rows = h ? p.rb : p.ra, row_first = t.first + PR * h;
-            const int pr = row_first + min(r, rows - 1), tok = pr / c.group, vis = r < rows ? t.pos0 + tok : -1;  // last position the row sees
+            const int pr = row_first + min(r, rows - 1), tok = pr / c.group, vis = r < rows ? t.pos0 + tok : 0x7fffffff;  // last position the row sees (rows behind the last: all, so that they need no mask)
             const long long col = (long long)(head * c.group + pr % c.group) * hs;
             float cexp = 0.f;
             if (n > 0) {
