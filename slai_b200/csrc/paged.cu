@@ -71,10 +71,13 @@ namespace {
 int make_handle(slai_ctx* ctx, slai_paged* p) {
     const Config& c = p->cfg;
     const int sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
-    const Lane few = paged_attention_lane(c.kv_dtype, c.head_size, sms);
+    const int group = c.n_q_heads / c.n_kv_heads;
+    const bool f16 = c.kv_dtype == SLAI_KV_F16, fast = paged_attention_few(c.kv_dtype, c.head_size);
+    const Lane few = paged_attention_lane(c.kv_dtype, c.head_size, group, sms);
+    const int few_rows = f16 ? FEW_ROWS : few.rows;
     Lane many;
-    if (paged_attention_few(c.kv_dtype, c.head_size) && (long long)c.max_tokens * (c.n_q_heads / c.n_kv_heads) > FEW_ROWS) many = paged_prompt_lane(sms);
-    p->planner.init(c, few, many, FEW_ROWS);
+    if (fast && (long long)c.max_tokens * group > few_rows) many = f16 ? paged_prompt_lane(sms) : paged_attention_any_lane(sms);
+    p->planner.init(c, few, many, few_rows);
     const size_t bytes = (size_t)p->planner.lay().total * 4;
     SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_plan, bytes));
     for (int i = 0; i < SLOTS; i++) {

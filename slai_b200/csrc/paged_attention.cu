@@ -357,6 +357,59 @@ __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// ---- few rows: the end of a block's part of a pair ------------------------------------------------------------------------------
+// Each of the block's FW warps has a maximum, a sum and an output of every row for its own positions: `so` [warp][rows][HS] (WF floats apart), ml_s; outputs and sums are
+// `carried` times their size apart.  They become the result, or the block's slot of `part`.
+#ifndef FEW_W
+#define FEW_W 4
+#define FEW_S 3
+#define FEW_B 2
+#endif
+constexpr int FW = FEW_W, FT = 32 * FW, FR = 8;
+template <int HS, typename T>
+__device__ __forceinline__ void few_end(const AttnArgs& A, const Start& s, const Tile& t, int head, int unit, bool whole, int lo, int hi, const float* so, int WF,
+                                        const float2 (*ml_s)[FR], unsigned int& bad, float carried) {
+    const Cache& c = A.c;
+    const int tid = threadIdx.x, warp = tid >> 5, hs = c.hs;
+    if (tid == 0) bad = 0;
+    __syncthreads();
+    const size_t slot = ((size_t)s.me * 2 + (unit == 0)) * A.tile_rows;
+    for (int i = tid; i < t.rows * (hs / 4); i += FT) {
+        const int r = i / (hs / 4), d = 4 * (i - r * (hs / 4));
+        float M = -INFINITY, den = 0.f, num[4] = {};
+#pragma unroll
+        for (int w = 0; w < FW; w++) M = fmaxf(M, ml_s[w][r].x);
+#pragma unroll
+        for (int w = 0; w < FW; w++) {
+            const float2 x = ml_s[w][r];
+            const float f = x.x == -INFINITY ? 0.f : ex2(x.x - M);
+            const float4 o = *reinterpret_cast<const float4*>(so + w * WF + r * HS + d);
+            den = fmaf(f, x.y, den);
+            num[0] = fmaf(f, o.x, num[0]); num[1] = fmaf(f, o.y, num[1]); num[2] = fmaf(f, o.z, num[2]); num[3] = fmaf(f, o.w, num[3]);
+        }
+        if (!(fabsf(num[0] + num[1] + num[2] + num[3] + den) < INFINITY)) atomicOr(&bad, 1u << r);
+        const float f = whole ? carried / den : carried;
+        const int pr = t.first + r, tok = pr / c.group;
+        float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs + d : A.part + (slot + r) * hs + d;
+        if (!whole || A.qvec) {
+            *reinterpret_cast<float4*>(o) = make_float4(num[0] * f, num[1] * f, num[2] * f, num[3] * f);
+        } else {
+            for (int e = 0; e < 4; e++) o[e] = num[e] * f;
+        }
+        if (!whole && d == 0) *reinterpret_cast<float2*>(A.part_ml + (slot + r) * 2) = make_float2(M, den);
+    }
+    __syncthreads();
+    if (bad) {
+        for (int r = warp; r < t.rows; r += FW)
+            if (bad >> r & 1) {
+                const int pr = t.first + r, tok = pr / c.group;
+                float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs : A.part + (slot + r) * hs;
+                row_again<T>(A, t, head, r, lo, hi, o, whole ? nullptr : A.part_ml + (slot + r) * 2);
+            }
+        __syncthreads();
+    }
+}
+
 // ---- f16 caches, few rows: tokens of sequences that answer ---------------------------------------------------------------------
 // Up to 8 rows (a token's or a few tokens' query heads of one cache head).  Queries and weights are pairs of halves (22 bits); the 16 rows of the matrix
 // instruction are the 8 high parts and, below them, the 8 low ones, so one product does both and a lane holds both results of its row.  Sums end every 16
@@ -364,12 +417,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
 // What such a call costs is reading the cache: each of the block's warps has a ring of its own of stages of 16 positions, brought in by asynchronous
 // copies that go around the registers, and takes every FW-th 16 positions of the block's share with a running maximum and sum of its own; they are joined in shared
 // memory at the end.
-#ifndef FEW_W
-#define FEW_W 4
-#define FEW_S 3
-#define FEW_B 2
-#endif
-constexpr int FW = FEW_W, FT = 32 * FW, FP = 16, FS = FEW_S, FR = 8;
+constexpr int FP = 16, FS = FEW_S;
 template <int HS>
 constexpr int FEW_SMEM = FW * FS * 2 * FP * HS * 2;
 
@@ -533,43 +581,7 @@ __global__ void __launch_bounds__(FT, FEW_B) paged_attn_few_kernel(const __grid_
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < NT8; i++) *reinterpret_cast<float2*>(so + warp * WF + g * HS + 8 * i + 2 * t4) = make_float2(acc[i][0], acc[i][1]);
-        if (tid == 0) bad = 0;
-        __syncthreads();
-        const size_t slot = ((size_t)s.me * 2 + (unit == 0)) * A.tile_rows;
-        for (int i = tid; i < t.rows * (hs / 4); i += FT) {
-            const int r = i / (hs / 4), d = 4 * (i - r * (hs / 4));
-            float M = -INFINITY, den = 0.f, num[4] = {};
-#pragma unroll
-            for (int w = 0; w < FW; w++) M = fmaxf(M, ml_s[w][r].x);
-#pragma unroll
-            for (int w = 0; w < FW; w++) {
-                const float2 x = ml_s[w][r];
-                const float f = x.x == -INFINITY ? 0.f : ex2(x.x - M);
-                const float4 o = *reinterpret_cast<const float4*>(so + w * WF + r * HS + d);
-                den = fmaf(f, x.y, den);
-                num[0] = fmaf(f, o.x, num[0]); num[1] = fmaf(f, o.y, num[1]); num[2] = fmaf(f, o.z, num[2]); num[3] = fmaf(f, o.w, num[3]);
-            }
-            if (!(fabsf(num[0] + num[1] + num[2] + num[3] + den) < INFINITY)) atomicOr(&bad, 1u << r);
-            const float f = whole ? 1.f / (den * 4096.f) : 1.f / 4096.f;
-            const int pr = t.first + r, tok = pr / c.group;
-            float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs + d : A.part + (slot + r) * hs + d;
-            if (!whole || A.qvec) {
-                *reinterpret_cast<float4*>(o) = make_float4(num[0] * f, num[1] * f, num[2] * f, num[3] * f);
-            } else {
-                for (int e = 0; e < 4; e++) o[e] = num[e] * f;
-            }
-            if (!whole && d == 0) *reinterpret_cast<float2*>(A.part_ml + (slot + r) * 2) = make_float2(M, den);
-        }
-        __syncthreads();
-        if (bad) {
-            for (int r = warp; r < t.rows; r += FW)
-                if (bad >> r & 1) {
-                    const int pr = t.first + r, tok = pr / c.group;
-                    float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs : A.part + (slot + r) * hs;
-                    row_again<__half>(A, t, head, r, lo, hi, o, whole ? nullptr : A.part_ml + (slot + r) * 2);
-                }
-            __syncthreads();
-        }
+        few_end<HS, __half>(A, s, t, head, unit, whole, lo, hi, so, WF, ml_s, bad, 1.f / 4096.f);
         left -= n + PAIR_COST;
         unit = 0;
         if (left > 0 && ++head == c.n_kv) {
@@ -590,16 +602,230 @@ int launch_few(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
     return launch_dependent(ctx, kern, dim3((unsigned)blocks), FT, FEW_SMEM<HS>, pdl, A);
 }
 
+// ---- f32 caches, few rows ----------------------------------------------------------------------------------------------------------
+// The same with f32 arithmetic: stages of 8 positions; four lanes take a position's score (a quarter of the dimensions each, the queries from shared memory), a lane
+// four dimensions of the output.  R: rows that there is room for (4 or 8).  Reading the cache bounds it: 8 rows take about half of the instructions that
+// there is time for meanwhile.
+constexpr int EP = 8;
+template <int HS, int R>
+constexpr int FEW32_SMEM = FW * FS * 2 * EP * HS * 4 + R * HS * 4 + FW * EP * R * 4;
+
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+template <int HS, int R, bool ALIGNED>
+__global__ void __launch_bounds__(FT, FEW_B) paged_attn_few32_kernel(const __grid_constant__ AttnArgs A) {
+    constexpr int ROW = HS * 4, CH = HS / 4, TILE = EP * ROW, STAGE = 2 * TILE, STEP = 32 / CH;  // STEP: rows a pass of the warp covers
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    extern __shared__ __align__(128) unsigned char few_sm[];
+    float* q_s = reinterpret_cast<float*>(few_sm + FW * FS * STAGE);  // [R][HS]
+    __shared__ float2 ml_s[FW][FR];
+    __shared__ unsigned int bad;
+    const Cache& c = A.c;
+    const Start s = load_start(c.plan, A.starts_at, blockIdx.x);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, p8 = lane >> 2, c4 = lane & 3, hs = c.hs, chunks = hs / 4, ch = lane % CH, rl = lane / CH;
+    float* p_s = q_s + R * HS + warp * EP * R;                         // [8][R], this warp's
+    unsigned char* ring = few_sm + warp * FS * STAGE;
+    const uint32_t ring_a = (uint32_t)__cvta_generic_to_shared(ring);
+    const char *keys = c.keys, *values = c.values;
+    // a piece's place in its row: rows of odd positions lie the other way round, so that two rows' pieces share no bank
+    auto piece = [](int r, int i) { return 4 * (i ^ ((r & 1) << 2)); };
+
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Tile t = s.t;
+    int head = s.head, unit = s.unit, tile = s.tile;
+    for (int left = s.count; left > 0;) {
+        const int n = min(left, t.units - unit);
+        const bool whole = n == t.units;
+        const int lo = unit * A.unit, hi = min((unit + n) * A.unit, t.pos0 + (t.first + t.rows - 1) / c.group + 1);  // positions [lo, hi)
+        const int subs = (hi - lo + EP - 1) / EP, mine = subs > warp ? (subs - warp + FW - 1) / FW : 0;
+        auto place = [&](int i) -> long long {
+            const int p = lo + (warp + i * FW) * EP + (ALIGNED ? 0 : lane & 7);
+            return i < mine && p < hi ? 4 * place_of(c, t.table, p, head) : 0;
+        };
+        auto request = [&](int i, long long at) {
+            if (i < mine) {
+                const uint32_t dst = ring_a + (i % FS) * STAGE;
+                const int valid = hi - (lo + (warp + i * FW) * EP);
+#pragma unroll
+                for (int k = 0; k < EP / STEP; k++) {
+                    const int r = rl + STEP * k;
+                    const uint32_t off = r * ROW + 4 * piece(r, ch), bytes = r < valid && ch < chunks ? 16u : 0u;  // (none: zeros, nothing is read)
+                    const long long a = ALIGNED ? at + r * 4 * c.pos_stride : __shfl_sync(0xffffffffu, at, r);
+                    const long long src = bytes ? a + 16 * ch : 0;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + off), "l"(__cvta_generic_to_global(keys + src)), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + TILE + off), "l"(__cvta_generic_to_global(values + src)), "r"(bytes) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        {
+            long long at[FS - 1];
+#pragma unroll
+            for (int i = 0; i < FS - 1; i++) at[i] = place(i);
+#pragma unroll
+            for (int i = 0; i < FS - 1; i++) request(i, at[i]);
+        }
+        long long next = place(FS - 1);
+        const float by = A.scale * LOG2E;  // scores as powers of two's exponents
+        for (int i = tid; i < R * HS; i += FT) {
+            const int r = i / HS, d = i % HS, pr = t.first + r, tok = pr / c.group;
+            q_s[i] = r < t.rows && d < hs ? __ldcg(A.q + (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs + d) * by : 0.f;
+        }
+        int vis[R];  // last position a row sees
+#pragma unroll
+        for (int r = 0; r < R; r++) vis[r] = r < t.rows ? t.pos0 + (t.first + r) / c.group : -1;
+        __syncthreads();
+        f32x2 acc[R][2];
+        float m[R], l[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            acc[r][0] = acc[r][1] = 0;
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+        }
+        for (int i = 0; i < mine; i++) {
+            request(i + FS - 1, next);
+            next = place(i + FS);
+            asm volatile("cp.async.wait_group %0;" ::"n"(FS - 1) : "memory");
+            __syncwarp();
+            const float* ks = reinterpret_cast<const float*>(ring + (i % FS) * STAGE);
+            const float* vs = ks + TILE / 4;
+            const int p = lo + (warp + i * FW) * EP + p8;
+            f32x2 sc[R][2];
+#pragma unroll
+            for (int r = 0; r < R; r++) sc[r][0] = sc[r][1] = 0;
+#pragma unroll
+            for (int j = 0; j < HS / 16; j++) {
+                const ulonglong2 k2 = *reinterpret_cast<const ulonglong2*>(ks + p8 * HS + piece(p8, 4 * j + c4));
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q_s + r * HS + 4 * (4 * j + c4));
+                    sc[r][0] = fma2(k2.x, q2.x, sc[r][0]);
+                    sc[r][1] = fma2(k2.y, q2.y, sc[r][1]);
+                }
+            }
+            float w[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const float2 a = unpack2(sc[r][0]), b = unpack2(sc[r][1]);
+                float x = (a.x + a.y) + (b.x + b.y);
+                x += __shfl_xor_sync(0xffffffffu, x, 1);
+                x += __shfl_xor_sync(0xffffffffu, x, 2);
+                w[r] = p > vis[r] ? -INFINITY : x;
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float mt = w[r];
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
+                const float m_new = fmaxf(m[r], mt), base = m_new == -INFINITY ? 0.f : m_new, resc = ex2(m[r] - base);
+                m[r] = m_new;
+                w[r] = ex2(w[r] - base);
+                l[r] = l[r] * resc + w[r];  // (this lane's positions only)
+                const f32x2 f = pack2(resc, resc);
+                acc[r][0] = mul2(acc[r][0], f);
+                acc[r][1] = mul2(acc[r][1], f);
+            }
+#pragma unroll
+            for (int r0 = 0; r0 < R; r0 += 4) {  // of the four lanes of a position, each writes one row of four
+                const float x = c4 == 0 ? w[r0] : c4 == 1 ? w[r0 + 1] : c4 == 2 ? w[r0 + 2] : w[r0 + 3];
+                p_s[p8 * R + r0 + c4] = x;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < EP; k += STEP) {
+                const int pos = k + rl;
+                const ulonglong2 v2 = *reinterpret_cast<const ulonglong2*>(vs + pos * HS + piece(pos, ch));
+#pragma unroll
+                for (int r0 = 0; r0 < R; r0 += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(p_s + pos * R + r0);
+                    const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const f32x2 f = pack2(xs[r], xs[r]);
+                        acc[r0 + r][0] = fma2(f, v2.x, acc[r0 + r][0]);
+                        acc[r0 + r][1] = fma2(f, v2.y, acc[r0 + r][1]);
+                    }
+                }
+            }
+            __syncwarp();  // the stage is requested, the weights written again next round
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        float* so = reinterpret_cast<float*>(few_sm);
+        constexpr int WF = FS * STAGE / 4;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+            const float2 a = unpack2(acc[r][0]), b = unpack2(acc[r][1]);
+            float4 v = make_float4(a.x, a.y, b.x, b.y);
+            if (STEP == 2) {
+                v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
+                v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+                v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
+                v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+            }
+            if (rl == 0) *reinterpret_cast<float4*>(so + warp * WF + r * HS + 4 * ch) = v;
+            if (lane == 0) ml_s[warp][r] = make_float2(m[r], l[r]);
+        }
+        few_end<HS, float>(A, s, t, head, unit, whole, lo, hi, so, WF, ml_s, bad, 1.f);
+        left -= n + PAIR_COST;
+        unit = 0;
+        if (left > 0 && ++head == c.n_kv) {
+            head = 0;
+            t = load_tile(c.plan, s.tiles, ++tile);
+        }
+    }
+}
+
+template <int HS, int R, bool ALIGNED>
+int launch_few32(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
+    auto kern = paged_attn_few32_kernel<HS, R, ALIGNED>;
+    static PerDeviceOnce attr;
+    if (attr.need(ctx->device)) {
+        SLAI_CHECK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW32_SMEM<HS, R>));
+        attr.set(ctx->device);
+    }
+    return launch_dependent(ctx, kern, dim3((unsigned)blocks), FT, FEW32_SMEM<HS, R>, pdl, A);
+}
+template <int HS>
+int launch_few32_of(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
+    if (A.c.page_size % EP == 0) return A.tile_rows <= 4 ? launch_few32<HS, 4, true>(ctx, A, blocks, pdl) : launch_few32<HS, 8, true>(ctx, A, blocks, pdl);
+    return A.tile_rows <= 4 ? launch_few32<HS, 4, false>(ctx, A, blocks, pdl) : launch_few32<HS, 8, false>(ctx, A, blocks, pdl);
+}
+
 }  // namespace
 
-// Whether a handle's few-row launches can take the matrix instructions (with rows that can be read in 16-byte pieces).
-bool paged_attention_few(int kv_dtype, int hs) { return kv_dtype == SLAI_KV_F16 && hs % 8 == 0 && hs <= 128; }
-Lane paged_attention_lane(int kv_dtype, int hs, int sms) {
+// Whether a handle's few-row launches can take the kernels above (with rows that can be read in 16-byte pieces).
+bool paged_attention_few(int kv_dtype, int hs) { return hs % (kv_dtype == SLAI_KV_F16 ? 8 : 4) == 0 && hs <= 128; }
+Lane paged_attention_lane(int kv_dtype, int hs, int group, int sms) {
     Lane l;
     l.unit = 64;
     l.least = 2;
     if (paged_attention_few(kv_dtype, hs)) {
-        l.rows = FR;
+        l.rows = kv_dtype == SLAI_KV_F16 || group > 4 ? FR : 4;
         l.blocks = FEW_B * sms;
     } else {
         l.rows = GR;
@@ -607,10 +833,18 @@ Lane paged_attention_lane(int kv_dtype, int hs, int sms) {
     }
     return l;
 }
-
+Lane paged_attention_any_lane(int sms) {
+    Lane l;
+    l.rows = GR;
+    l.unit = 64;
+    l.least = 2;
+    l.blocks = 4 * sms;
+    return l;
+}
 static int launch_lane(slai_ctx* ctx, const AttnArgs& A, int kv_dtype, int lane, int blocks, bool pdl) {
-    if (lane == 1 && A.vec) return paged_prompt_launch(ctx, A, blocks, pdl);
+    if (lane == 1 && A.vec && kv_dtype == SLAI_KV_F16) return paged_prompt_launch(ctx, A, blocks, pdl);
     if (lane == 0 && A.vec && paged_attention_few(kv_dtype, A.c.hs)) {
+        if (kv_dtype == SLAI_KV_F32) return A.c.hs <= 64 ? launch_few32_of<64>(ctx, A, blocks, pdl) : launch_few32_of<128>(ctx, A, blocks, pdl);
         if (A.c.page_size % FP == 0) return A.c.hs <= 64 ? launch_few<64, true>(ctx, A, blocks, pdl) : launch_few<128, true>(ctx, A, blocks, pdl);
         return A.c.hs <= 64 ? launch_few<64, false>(ctx, A, blocks, pdl) : launch_few<128, false>(ctx, A, blocks, pdl);
     }
