@@ -76,7 +76,7 @@ int make_handle(slai_ctx* ctx, slai_paged* p) {
     const Lane few = paged_attention_lane(c.kv_dtype, c.head_size, group, sms);
     const int few_rows = f16 ? FEW_ROWS : few.rows;
     Lane many;
-    if (fast && (long long)c.max_tokens * group > few_rows) many = f16 ? paged_prompt_lane(sms) : paged_attention_any_lane(sms);
+    if (fast && (long long)c.max_tokens * group > few_rows) many = f16 ? paged_prompt_lane(sms) : paged_attention_block_lane(sms);
     p->planner.init(c, few, many, few_rows);
     const size_t bytes = (size_t)p->planner.lay().total * 4;
     SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_plan, bytes));

@@ -60,7 +60,7 @@ __device__ __forceinline__ long long place_of(const Cache& c, int table, int p, 
 
 bool paged_attention_few(int kv_dtype, int hs);
 paged::Lane paged_attention_lane(int kv_dtype, int hs, int group, int sms);
-paged::Lane paged_attention_any_lane(int sms);  // f32 caches, many rows
+paged::Lane paged_attention_block_lane(int sms);  // f32 caches, many rows
 // One lane's kernel with `blocks` blocks, and the joins of at most `joins` pairs of at most `longest` results.
 int paged_attention_launch(slai_ctx* ctx, paged::AttnArgs& A, int kv_dtype, int lane, int blocks, int joins, int longest, bool pdl);
 
