@@ -687,8 +687,9 @@ __global__ void __launch_bounds__(FT, FEW_B) paged_attn_few32_kernel(const __gri
         }
         long long next = place(FS - 1);
         const float by = A.scale * LOG2E;  // scores as powers of two's exponents
-        for (int i = tid; i < R * HS; i += FT) {
-            const int r = i / HS, d = i % HS, pr = t.first + r, tok = pr / c.group;
+#pragma unroll
+        for (int k = 0; k < R * HS / FT; k++) {
+            const int i = tid + k * FT, r = i / HS, d = i % HS, pr = t.first + r, tok = pr / c.group;
             q_s[i] = r < t.rows && d < hs ? __ldcg(A.q + (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs + d) * by : 0.f;
         }
         int vis[R];  // last position a row sees
@@ -832,13 +833,13 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
     constexpr int CH = HS / 4, STEP = 32 / CH, KS = L::KS, DV = HS / 64;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(128) unsigned char few_sm[];
-    float* q_s = reinterpret_cast<float*>(few_sm);   // [64][HS + 4], times the scale
+    float* q_s = reinterpret_cast<float*>(few_sm);   // [64][HS + 4]
     float* kv_s = q_s + L::Q;                        // two of: keys [32][HS + 4], values [32][HS]
     float* p_s = kv_s + 2 * (L::K + L::V);           // [32][64 + 4]: weights
     const Cache& c = A.c;
     const Start s = load_start(c.plan, A.starts_at, blockIdx.x);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tx = tid & 15, ty = tid >> 4, hs = c.hs, chunks = hs / 4, ch = lane % CH, rl = lane / CH;
-    const uint32_t kv_a = (uint32_t)__cvta_generic_to_shared(kv_s);
+    const uint32_t kv_a = (uint32_t)__cvta_generic_to_shared(kv_s), q_a = (uint32_t)__cvta_generic_to_shared(q_s);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     Tile t = s.t;
     int head = s.head, unit = s.unit, tile = s.tile;
@@ -861,15 +862,26 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(vd + 4 * (r * HS + 4 * ch)), "l"(__cvta_generic_to_global(c.values + src)), "r"(bytes) : "memory");
             }
         };
+        // queries: all on their way at once
+        if (A.qvec) {
+#pragma unroll
+            for (int k = 0; k < BR / 4; k += STEP) {
+                const int r = 4 * k + 4 * rl + warp, pr = t.first + min(r, t.rows - 1), tok = pr / c.group;
+                const uint32_t bytes = r < t.rows && ch < chunks ? 16u : 0u;
+                const float* q = A.q + (bytes ? (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs + 4 * ch : 0);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_a + 4 * (r * KS + 4 * ch)), "l"(__cvta_generic_to_global(q)), "r"(bytes) : "memory");
+            }
+        } else {
+            for (int r = warp; r < BR; r += BT / 32) {
+                const int pr = t.first + min(r, t.rows - 1), tok = pr / c.group;
+                const float* q = A.q + (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs;
+#pragma unroll
+                for (int d = lane; d < HS; d += 32) q_s[r * KS + d] = r < t.rows && d < hs ? __ldcg(q + d) : 0.f;
+            }
+        }
         request(0);
         asm volatile("cp.async.commit_group;" ::: "memory");
         const float by = A.scale * LOG2E;  // scores as powers of two's exponents
-        for (int r = warp; r < BR; r += BT / 32) {
-            const int pr = t.first + min(r, t.rows - 1), tok = pr / c.group;
-            const float* q = A.q + (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs;
-#pragma unroll
-            for (int d = lane; d < HS; d += 32) q_s[r * KS + d] = r < t.rows && d < hs ? __ldcg(q + d) * by : 0.f;
-        }
         const bool on = 16 * warp < t.rows;  // this warp has rows
         int vis[8];  // last position a row sees
 #pragma unroll
@@ -912,7 +924,7 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
                     for (int u = 0; u < 2; u++) {
                         const float2 x = unpack2(sc[r][u]);
                         // (rows behind the tile's last see the positions that are not there too: nothing of theirs is kept)
-                        w[r][u] = p0 + tx + 16 * u > min(vis[r], hi - 1) ? -INFINITY : x.x + x.y;
+                        w[r][u] = p0 + tx + 16 * u > min(vis[r], hi - 1) ? -INFINITY : (x.x + x.y) * by;
                     }
                     float mt = fmaxf(w[r][0], w[r][1]);
 #pragma unroll

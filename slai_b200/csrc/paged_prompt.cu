@@ -354,39 +354,36 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
             const long long col = (long long)(head * c.group + pr % c.group) * hs;
             float cexp = 0.f;
             if (n > 0) {
-                // queries: a warp brings 16 rows, 8 at a time, 4 elements a lane
+                // queries: a warp brings 16 rows, 4 elements a lane, all on their way at once
                 const long long q_at = (t.row0 + tok) * A.q_ld + col;
+                float4 v[16];
 #pragma unroll
-                for (int i0 = 0; i0 < 16; i0 += 8) {
-                    float4 v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int rl = 16 * g + i0 + i;
-                        const float* q = A.q + __shfl_sync(0xffffffffu, q_at, rl) + 4 * lane;
-                        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (32 * q4 + rl < rows && 4 * lane < hs) {
-                            if (A.qvec) v[i] = __ldcg(reinterpret_cast<const float4*>(q));
-                            else v[i] = make_float4(__ldcg(q), __ldcg(q + 1), __ldcg(q + 2), __ldcg(q + 3));
-                        }
+                for (int i = 0; i < 16; i++) {
+                    const int rl = 16 * g + i;
+                    const float* q = A.q + __shfl_sync(0xffffffffu, q_at, rl) + 4 * lane;
+                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (32 * q4 + rl < rows && 4 * lane < hs) {
+                        if (A.qvec) v[i] = __ldcg(reinterpret_cast<const float4*>(q));
+                        else v[i] = make_float4(__ldcg(q), __ldcg(q + 1), __ldcg(q + 2), __ldcg(q + 3));
                     }
+                }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int rl = 16 * g + i0 + i, rr = 32 * q4 + rl;
-                        v[i].x *= A.scale; v[i].y *= A.scale; v[i].z *= A.scale; v[i].w *= A.scale;
-                        float mx = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+                for (int i = 0; i < 16; i++) {
+                    const int rl = 16 * g + i, rr = 32 * q4 + rl;
+                    v[i].x *= A.scale; v[i].y *= A.scale; v[i].z *= A.scale; v[i].w *= A.scale;
+                    float mx = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
 #pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                        float unit;
-                        const float up = power_up(mx, unit);
-                        if (lane == rl) cexp = unit * LOG2E;
-                        uint2 hi, lo;
-                        split2(v[i].x * up, v[i].y * up, hi.x, lo.x);
-                        split2(v[i].z * up, v[i].w * up, hi.y, lo.y);
-                        if (4 * lane < HS) {
-                            const int ch = (lane % 16) / 2, off = (lane / 16) * L::BLOCK + rr * 128 + ((ch ^ (rr & 7)) << 4) + 8 * (lane & 1);
-                            *reinterpret_cast<uint2*>(mine + off) = hi;
-                            *reinterpret_cast<uint2*>(mine + L::Q + off) = lo;
-                        }
+                    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    float unit;
+                    const float up = power_up(mx, unit);
+                    if (lane == rl) cexp = unit * LOG2E;
+                    uint2 hi, lo;
+                    split2(v[i].x * up, v[i].y * up, hi.x, lo.x);
+                    split2(v[i].z * up, v[i].w * up, hi.y, lo.y);
+                    if (4 * lane < HS) {
+                        const int ch = (lane % 16) / 2, off = (lane / 16) * L::BLOCK + rr * 128 + ((ch ^ (rr & 7)) << 4) + 8 * (lane & 1);
+                        *reinterpret_cast<uint2*>(mine + off) = hi;
+                        *reinterpret_cast<uint2*>(mine + L::Q + off) = lo;
                     }
                 }
                 fence_async();
