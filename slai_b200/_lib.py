@@ -129,9 +129,9 @@ SIGNATURES = {
     "slai_paged_create": (C.c_int, [_vp, C.POINTER(PagedConfig), _pp]),
     "slai_paged_destroy": (C.c_int, [_vp]),
     "slai_paged_step": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _i64]),
-    "slai_qk_norm_rope": (C.c_int, [_vp, C.POINTER(QkParams), C.c_int, _vp, _vp, _vp, _vp, _vp]),
-    "slai_paged_append": (C.c_int, [_vp, C.POINTER(PagedLayer), C.POINTER(QkParams), _vp, _vp, _vp, _vp]),
-    "slai_paged_attention": (C.c_int, [_vp, C.POINTER(PagedLayer), _vp, _i64, C.c_float, _vp, _i64]),
+    "slai_qk_norm_rope": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp]),
+    "slai_paged_append": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "slai_paged_attention": (C.c_int, [_vp, _vp, _vp, _i64, C.c_float, _vp, _i64]),
     "slai_llama_create": (C.c_int, [_vp, C.POINTER(LlamaConfig), _pp]),
     "slai_llama_destroy": (C.c_int, [_vp]),
     "slai_llama_set_matrix": (C.c_int, [_vp, C.c_int, C.c_int, _vp]),

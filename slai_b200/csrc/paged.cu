@@ -74,7 +74,7 @@ int make_handle(slai_ctx* ctx, slai_paged* p) {
     const int group = c.n_q_heads / c.n_kv_heads;
     const bool f16 = c.kv_dtype == SLAI_KV_F16, fast = paged_attention_few(c.kv_dtype, c.head_size);
     const Lane few = paged_attention_lane(c.kv_dtype, c.head_size, group, sms);
-    const int few_rows = f16 ? FEW_ROWS : few.rows;
+    const int few_rows = f16 ? FEW_ROWS : std::max(few.rows, 4);
     Lane many;
     if (fast && (long long)c.max_tokens * group > few_rows) many = f16 ? paged_prompt_lane(sms) : paged_attention_block_lane(sms);
     p->planner.init(c, few, many, few_rows);

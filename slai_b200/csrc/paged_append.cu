@@ -115,8 +115,12 @@ __global__ void __launch_bounds__(QT) qk_any_kernel(const QkArgs A) {
 
 // Heads of a multiple of 8 elements on 16-byte boundaries: LPH lanes take a head, 8 elements a lane (two 16-byte pieces that hold four whole pairs in either
 // variant), a warp 32 / LPH * U heads of one token, whose angles it needs once.
+#ifndef QK_MINB
+#define QK_MINB 3
+#define QK_U 4
+#endif
 template <int LPH, int U, bool NEOX>
-__global__ void __launch_bounds__(QT) qk_vec_kernel(const QkArgs A) {
+__global__ void __launch_bounds__(QT, QK_MINB) qk_vec_kernel(const QkArgs A) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int HPW = 32 / LPH;
@@ -128,18 +132,15 @@ __global__ void __launch_bounds__(QT) qk_vec_kernel(const QkArgs A) {
     if (ps.x < 0) return;
     const bool mine = 8 * l < A.hs;
     const int e0 = NEOX ? 4 * l : 8 * l, e1 = NEOX ? A.hs / 2 + 4 * l : 8 * l + 4;
-    Head H[U];
     float4 x[U][2];
 #pragma unroll
-    for (int u = 0; u < U; u++) {  // all loads on their way first
+    for (int u = 0; u < U; u++) {  // all loads on their way first (where they go is worked out again below: kept meanwhile, it took half of the registers)
         const int h = h0 + u * HPW + lane / LPH;
         x[u][0] = x[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (h < heads) {
-            H[u] = head_of(A, row, ps.y, h);
-            if (mine) {
-                x[u][0] = __ldcg(reinterpret_cast<const float4*>(H[u].in + e0));
-                x[u][1] = __ldcg(reinterpret_cast<const float4*>(H[u].in + e1));
-            }
+        if (h < heads && mine) {
+            const float* in = head_of(A, row, ps.y, h).in;
+            x[u][0] = __ldcg(reinterpret_cast<const float4*>(in + e0));
+            x[u][1] = __ldcg(reinterpret_cast<const float4*>(in + e1));
         }
     }
     float2 cs[4];
@@ -150,6 +151,7 @@ __global__ void __launch_bounds__(QT) qk_vec_kernel(const QkArgs A) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int h = h0 + u * HPW + lane / LPH;
+        const Head H = head_of(A, row, ps.y, min(h, heads - 1));
         float v[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
         if (A.q_norm || A.k_norm) {  // (the same for all lanes; the sum of a head that is not normalised goes unused)
             float ss = 0.f;
@@ -157,16 +159,16 @@ __global__ void __launch_bounds__(QT) qk_vec_kernel(const QkArgs A) {
             for (int i = 0; i < 8; i++) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (h < heads && mine && H[u].norm) {
+            if (h < heads && mine && H.norm) {
                 const float r = rsqrtf(ss / (float)A.hs + A.eps);
-                const float4 w0 = *reinterpret_cast<const float4*>(H[u].norm + e0), w1 = *reinterpret_cast<const float4*>(H[u].norm + e1);
+                const float4 w0 = *reinterpret_cast<const float4*>(H.norm + e0), w1 = *reinterpret_cast<const float4*>(H.norm + e1);
                 const float wn[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[i] = v[i] * r * wn[i];
             }
         }
         if (h >= heads || !mine) continue;
-        if (H[u].turn) {
+        if (H.turn) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float& a = v[NEOX ? i : 2 * i];
@@ -176,15 +178,15 @@ __global__ void __launch_bounds__(QT) qk_vec_kernel(const QkArgs A) {
                 a = y;
             }
         }
-        if (H[u].cache && A.kv_f16) {
+        if (H.cache && A.kv_f16) {
             __half2 p[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) p[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-            __half* d = reinterpret_cast<__half*>(H[u].cache);
+            __half* d = reinterpret_cast<__half*>(H.cache);
             *reinterpret_cast<uint2*>(d + e0) = *reinterpret_cast<uint2*>(p);
             *reinterpret_cast<uint2*>(d + e1) = *reinterpret_cast<uint2*>(p + 2);
         } else {
-            float* d = H[u].out ? H[u].out : reinterpret_cast<float*>(H[u].cache);
+            float* d = H.out ? H.out : reinterpret_cast<float*>(H.cache);
             *reinterpret_cast<float4*>(d + e0) = make_float4(v[0], v[1], v[2], v[3]);
             *reinterpret_cast<float4*>(d + e1) = make_float4(v[4], v[5], v[6], v[7]);
         }
@@ -196,9 +198,9 @@ int launch_vec(slai_ctx* ctx, QkArgs& A, long long heads, bool pdl) {
     constexpr int HPW = 32 / LPH;
     auto blocks = [&](int u) { return ((long long)A.rows * ((heads + HPW * u - 1) / (HPW * u)) + QT / 32 - 1) / (QT / 32); };
     // Several heads a warp where that leaves enough warps to keep the memory busy.
-    const bool many = blocks(4) >= 8 * (ctx->sm_count > 0 ? ctx->sm_count : 148);
+    const bool many = blocks(QK_U) >= 8 * (ctx->sm_count > 0 ? ctx->sm_count : 148);
     SLAI_REQUIRE(ctx, blocks(1) <= 0x7fffffffll, SLAI_ERR_SHAPE, "rows: too many (%d tokens of %lld heads)", A.rows, heads);
-    return many ? launch_dependent(ctx, qk_vec_kernel<LPH, 4, NEOX>, dim3((unsigned)blocks(4)), QT, 0, pdl, A)
+    return many ? launch_dependent(ctx, qk_vec_kernel<LPH, QK_U, NEOX>, dim3((unsigned)blocks(QK_U)), QT, 0, pdl, A)
                 : launch_dependent(ctx, qk_vec_kernel<LPH, 1, NEOX>, dim3((unsigned)blocks(1)), QT, 0, pdl, A);
 }
 

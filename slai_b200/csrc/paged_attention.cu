@@ -604,7 +604,7 @@ int launch_few(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
 
 // ---- f32 caches, few rows ----------------------------------------------------------------------------------------------------------
 // The same with f32 arithmetic: stages of 8 positions; four lanes take a position's score (a quarter of the dimensions each, the queries from shared memory), a lane
-// four dimensions of the output.  R: rows that there is room for (4 or 8).  Reading the cache bounds it: 8 rows take about half of the instructions that
+// four dimensions of the output.  R: rows that there is room for (1, 4 or 8).  Reading the cache bounds it: 8 rows take about half of the instructions that
 // there is time for meanwhile.
 constexpr int EP = 8;
 template <int HS, int R>
@@ -688,8 +688,10 @@ __global__ void __launch_bounds__(FT, FEW_B) paged_attn_few32_kernel(const __gri
         long long next = place(FS - 1);
         const float by = A.scale * LOG2E;  // scores as powers of two's exponents
 #pragma unroll
-        for (int k = 0; k < R * HS / FT; k++) {
-            const int i = tid + k * FT, r = i / HS, d = i % HS, pr = t.first + r, tok = pr / c.group;
+        for (int k = 0; k < (R * HS + FT - 1) / FT; k++) {
+            const int i = tid + k * FT;
+            if (i >= R * HS) break;
+            const int r = i / HS, d = i % HS, pr = t.first + r, tok = pr / c.group;
             q_s[i] = r < t.rows && d < hs ? __ldcg(A.q + (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs + d) * by : 0.f;
         }
         int vis[R];  // last position a row sees
@@ -750,8 +752,8 @@ __global__ void __launch_bounds__(FT, FEW_B) paged_attn_few32_kernel(const __gri
             }
 #pragma unroll
             for (int r0 = 0; r0 < R; r0 += 4) {  // of the four lanes of a position, each writes one row of four
-                const float x = c4 == 0 ? w[r0] : c4 == 1 ? w[r0 + 1] : c4 == 2 ? w[r0 + 2] : w[r0 + 3];
-                p_s[p8 * R + r0 + c4] = x;
+                const float x = R == 1 || c4 == 0 ? w[r0] : c4 == 1 ? w[(r0 + 1) % R] : c4 == 2 ? w[(r0 + 2) % R] : w[(r0 + 3) % R];
+                if (r0 + c4 < R) p_s[p8 * R + r0 + c4] = x;
             }
             __syncwarp();
 #pragma unroll
@@ -760,10 +762,11 @@ __global__ void __launch_bounds__(FT, FEW_B) paged_attn_few32_kernel(const __gri
                 const ulonglong2 v2 = *reinterpret_cast<const ulonglong2*>(vs + pos * HS + piece(pos, ch));
 #pragma unroll
                 for (int r0 = 0; r0 < R; r0 += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(p_s + pos * R + r0);
-                    const float xs[4] = {x.x, x.y, x.z, x.w};
+                    float xs[4];
+                    if (R == 1) xs[0] = p_s[pos];
+                    else *reinterpret_cast<float4*>(xs) = *reinterpret_cast<const float4*>(p_s + pos * R + r0);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
+                    for (int r = 0; r < (R < 4 ? R : 4); r++) {
                         const f32x2 f = pack2(xs[r], xs[r]);
                         acc[r0 + r][0] = fma2(f, v2.x, acc[r0 + r][0]);
                         acc[r0 + r][1] = fma2(f, v2.y, acc[r0 + r][1]);
@@ -813,6 +816,7 @@ int launch_few32(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
 }
 template <int HS>
 int launch_few32_of(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
+    if (A.tile_rows == 1) return A.c.page_size % EP == 0 ? launch_few32<HS, 1, true>(ctx, A, blocks, pdl) : launch_few32<HS, 1, false>(ctx, A, blocks, pdl);
     if (A.c.page_size % EP == 0) return A.tile_rows <= 4 ? launch_few32<HS, 4, true>(ctx, A, blocks, pdl) : launch_few32<HS, 8, true>(ctx, A, blocks, pdl);
     return A.tile_rows <= 4 ? launch_few32<HS, 4, false>(ctx, A, blocks, pdl) : launch_few32<HS, 8, false>(ctx, A, blocks, pdl);
 }
@@ -1036,7 +1040,7 @@ Lane paged_attention_lane(int kv_dtype, int hs, int group, int sms) {
     l.unit = 64;
     l.least = 2;
     if (paged_attention_few(kv_dtype, hs)) {
-        l.rows = kv_dtype == SLAI_KV_F16 || group > 4 ? FR : 4;
+        l.rows = kv_dtype == SLAI_KV_F16 || group > 4 ? FR : group == 1 ? 1 : 4;
         l.blocks = FEW_B * sms;
     } else {
         l.rows = GR;

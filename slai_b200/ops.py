@@ -299,12 +299,9 @@ class PagedLayer:
 
     def __init__(self, keys, values, page_stride: int, head_stride: int, pos_stride: int):
         self.keys, self.values = keys, values  # held: the pages outlive the layer
+        self.strides = (page_stride, head_stride, pos_stride)
         self.c = _lib.PagedLayer(keys.ptr, values.ptr, page_stride, head_stride, pos_stride)
-
-    def span(self, n_pages: int, page_size: int, n_kv_heads: int, head_size: int) -> int:
-        """Elements from the first to the last of all pages."""
-        c = self.c
-        return (n_pages - 1) * c.page_stride + (n_kv_heads - 1) * c.head_stride + (page_size - 1) * c.pos_stride + head_size
+        self.at = C.addressof(self.c)
 
 
 class PagedKv:
@@ -315,7 +312,7 @@ class PagedKv:
                  max_seqs: int = 8, max_tokens: int = 512, max_table: int | None = None):
         self.backend = backend
         self.n_q_heads, self.n_kv_heads, self.head_size, self.page_size, self.n_pages = n_q_heads, n_kv_heads, head_size, page_size, n_pages
-        self.kv_dtype, self.max_tokens = kv_dtype, max_tokens
+        self.kv_dtype, self.max_tokens, self.width = kv_dtype, max_tokens, n_q_heads * head_size
         self.rows = None  # of the current step
         cfg = _lib.PagedConfig(n_q_heads, n_kv_heads, head_size, page_size, n_pages, kv_dtype, max_seqs, max_tokens, max_table or max(1, n_pages))
         h = C.c_void_p()
@@ -334,7 +331,8 @@ class PagedKv:
         self.rows = int(n_new.sum())
 
     def check_layer(self, layer: PagedLayer):
-        need = layer.span(self.n_pages, self.page_size, self.n_kv_heads, self.head_size)
+        page, head, pos = layer.strides
+        need = (self.n_pages - 1) * page + (self.n_kv_heads - 1) * head + (self.page_size - 1) * pos + self.head_size
         if len(layer.keys) < need or len(layer.values) < need:
             raise SlaiError(_lib.ERR_SHAPE, f"paged: pages of {len(layer.keys)} and {len(layer.values)} elements, {need} needed")
 
@@ -357,16 +355,16 @@ class QkNormRope:
             if w is not None and len(w) != head_size:
                 raise SlaiError(_lib.ERR_SHAPE, f"qk: {len(w)} norm weights for heads of {head_size}")
         self.norms = (q_norm, k_norm)  # held
-        self.n_q_heads, self.n_kv_heads, self.head_size = n_q_heads, n_kv_heads, head_size
+        self.q_width, self.k_width = n_q_heads * head_size, n_kv_heads * head_size
+        self.q_ld, self.k_ld, self.v_ld = q_ld or self.q_width, k_ld or self.k_width, v_ld or self.k_width
+        self.q_out_ld, self.k_out_ld = q_out_ld or self.q_width, k_out_ld or self.k_width
         self.c = _lib.QkParams(head_size, n_q_heads, n_kv_heads, -1 if variant is None else int(variant), base_freq, eps, _ptr(q_norm).value,
                                _ptr(k_norm).value, q_ld, k_ld, v_ld, q_out_ld, k_out_ld)
+        self.at = C.addressof(self.c)
 
 
-def _check_rows(what: str, x, rows: int, width: int, ld: int):
-    """`x` holds `rows` rows of `width` floats, `ld` (0: packed) apart."""
-    need = (rows - 1) * (ld or width) + width if rows > 0 and width > 0 else 0
-    if (0 if x is None else len(x)) < need:
-        raise SlaiError(_lib.ERR_SHAPE, f"{what}: {0 if x is None else len(x)} floats for {rows} rows of {width}, {ld or width} apart")
+def _refuse_rows(what: str, x, rows: int, width: int, ld: int):
+    raise SlaiError(_lib.ERR_SHAPE, f"{what}: {0 if x is None else len(x)} floats for {rows} rows of {width}, {ld or width} apart")
 
 
 class LlmContext:
@@ -465,31 +463,60 @@ class LlmContext:
     def kv_append(self, key_cache, value_cache, k, v, kv_dim: int, pos: int, kv_dtype: int = KV_F32):
         self.backend.check(self.lib.slai_kv_append(self.h, _ptr(key_cache), _ptr(value_cache), kv_dtype, _ptr(k), _ptr(v), kv_dim, pos))
 
-    # Paged caches (the operators they stand beside: RmsNorm, RoPE, key_cache.column(pos), BatchedMultiqueryAttention)
+    # Paged caches (the operators they stand beside: RmsNorm, RoPE, key_cache.column(pos), BatchedMultiqueryAttention).  A buffer of n rows holds at least the
+    # (n - 1) * leading dimension + width floats from its first row to its last.
     def qk_norm_rope(self, how: QkNormRope, positions, q, k, q_out, k_out):
         """Norm and rotation of the rows of q and k, token t at position positions[t] (int32 on the device; negative: left as it is)."""
-        n, hs = len(positions), how.head_size
-        for what, x, heads, ld in (("q", q, how.n_q_heads, how.c.q_ld), ("q_out", q_out, how.n_q_heads, how.c.q_out_ld),
-                                   ("k", k, how.n_kv_heads, how.c.k_ld), ("k_out", k_out, how.n_kv_heads, how.c.k_out_ld)):
-            _check_rows(f"qk_norm_rope: {what}", x, n, heads * hs, ld)
-        self.backend.check(self.lib.slai_qk_norm_rope(self.h, C.byref(how.c), n, _ptr(positions), _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out)))
+        n = len(positions)
+        if n > 0:
+            m, w, k_w = n - 1, how.q_width, how.k_width
+            if w:
+                if q is None or len(q) < m * how.q_ld + w:
+                    _refuse_rows("qk_norm_rope: q", q, n, w, how.q_ld)
+                if q_out is None or len(q_out) < m * how.q_out_ld + w:
+                    _refuse_rows("qk_norm_rope: q_out", q_out, n, w, how.q_out_ld)
+            if k_w:
+                if k is None or len(k) < m * how.k_ld + k_w:
+                    _refuse_rows("qk_norm_rope: k", k, n, k_w, how.k_ld)
+                if k_out is None or len(k_out) < m * how.k_out_ld + k_w:
+                    _refuse_rows("qk_norm_rope: k_out", k_out, n, k_w, how.k_out_ld)
+        rc = self.lib.slai_qk_norm_rope(self.h, how.at, n, positions.ptr, None if q is None else q.ptr, None if k is None else k.ptr,
+                                        None if q_out is None else q_out.ptr, None if k_out is None else k_out.ptr)
+        if rc:
+            self.backend.check(rc)
 
     def paged_append(self, paged: PagedKv, layer: PagedLayer, how: QkNormRope, q, k, v, q_out):
         """The same for the rows of the current step; keys and values go into their pages, q to q_out."""
         paged.check_layer(layer)
-        n, hs = paged.rows or 0, how.head_size
-        for what, x, heads, ld in (("q", q, how.n_q_heads, how.c.q_ld), ("q_out", q_out, how.n_q_heads, how.c.q_out_ld),
-                                   ("k", k, how.n_kv_heads, how.c.k_ld), ("v", v, how.n_kv_heads, how.c.v_ld)):
-            _check_rows(f"paged_append: {what}", x, n, heads * hs, ld)
-        self.backend.check(self.lib.slai_paged_append(paged.h, C.byref(layer.c), C.byref(how.c), _ptr(q), _ptr(k), _ptr(v), _ptr(q_out)))
+        n = paged.rows
+        if n:
+            m, w, k_w = n - 1, how.q_width, how.k_width
+            if w:
+                if q is None or len(q) < m * how.q_ld + w:
+                    _refuse_rows("paged_append: q", q, n, w, how.q_ld)
+                if q_out is None or len(q_out) < m * how.q_out_ld + w:
+                    _refuse_rows("paged_append: q_out", q_out, n, w, how.q_out_ld)
+            if k is None or len(k) < m * how.k_ld + k_w:
+                _refuse_rows("paged_append: k", k, n, k_w, how.k_ld)
+            if v is None or len(v) < m * how.v_ld + k_w:
+                _refuse_rows("paged_append: v", v, n, k_w, how.v_ld)
+        rc = self.lib.slai_paged_append(paged.h, layer.at, how.at, None if q is None else q.ptr, None if k is None else k.ptr, None if v is None else v.ptr,
+                                        None if q_out is None else q_out.ptr)
+        if rc:
+            self.backend.check(rc)
 
     def paged_attention(self, paged: PagedKv, layer: PagedLayer, q, out, scale: float = 0.0, q_ld: int = 0, out_ld: int = 0):
         """Causal attention of the step's tokens to what their sequences hold (scale 0: 1 / sqrt(head_size))."""
         paged.check_layer(layer)
-        width = paged.n_q_heads * paged.head_size
-        _check_rows("paged_attention: q", q, paged.rows or 0, width, q_ld)
-        _check_rows("paged_attention: out", out, paged.rows or 0, width, out_ld)
-        self.backend.check(self.lib.slai_paged_attention(paged.h, C.byref(layer.c), _ptr(q), q_ld, scale, _ptr(out), out_ld))
+        n, width = paged.rows, paged.width
+        if n:
+            if len(q) < (n - 1) * (q_ld or width) + width:
+                _refuse_rows("paged_attention: q", q, n, width, q_ld)
+            if len(out) < (n - 1) * (out_ld or width) + width:
+                _refuse_rows("paged_attention: out", out, n, width, out_ld)
+        rc = self.lib.slai_paged_attention(paged.h, layer.at, q.ptr, q_ld, scale, out.ptr, out_ld)
+        if rc:
+            self.backend.check(rc)
 
     def sample(self, logits: GpuVector, temperature: float, topp: float, coin: float) -> int:
         """`Sampler::sample` (models/sampler.rs:33-54) on the device, the uniform number `coin` given; `logits` is
