@@ -53,6 +53,7 @@ struct Lane {  // one of the two kinds of kernel
     int rows = 0, unit = 0;    // tile height, positions of a unit
     int blocks = 0;            // most blocks
     int least = 1;             // units a block has at least, if the line allows it
+    int join = 0;              // units that the join costs: where every pair can have a block, none is cut that is longer than a share by no more than this
 };
 
 struct Layout {  // of the device copy, in ints
@@ -191,7 +192,12 @@ class Planner {
             }
             at += n * (int)(sizeof(Tile) / 4);
             const long long U = so_far;
-            const int C = (int)std::min<long long>(lanes_[k].blocks, (U + lanes_[k].least - 1) / std::max(1, lanes_[k].least));
+            int longest = 0;
+            long long pairs = (long long)n * cfg_.n_kv_heads;
+            for (int i = 0; i < n; i++) longest = std::max(longest, tiles[i].units);
+            const long long share = lanes_[k].blocks ? std::max<long long>(lanes_[k].least, U / lanes_[k].blocks) : 0;
+            const bool whole = lanes_[k].join > 0 && pairs <= lanes_[k].blocks && longest <= share + lanes_[k].join;
+            const int C = (int)(whole ? pairs : std::min<long long>(lanes_[k].blocks, (U + lanes_[k].least - 1) / std::max(1, lanes_[k].least)));
             step->blocks[k] = C;
             Start* st = reinterpret_cast<Start*>(out + lay_.starts[k]);
             Join* jo = reinterpret_cast<Join*>(out + lay_.joins[k]);
@@ -199,7 +205,12 @@ class Planner {
             for (int c = 0; c < lanes_[k].blocks; c++) {
                 Start s = {};
                 if (c < C) {
-                    const long long lo = U * c / C, hi = U * (c + 1) / C;
+                    long long lo = U * c / C, hi = U * (c + 1) / C;
+                    if (whole) {
+                        const Tile& t = tiles[c / cfg_.n_kv_heads];
+                        lo = t.line + (long long)(c % cfg_.n_kv_heads) * (t.units + PAIR_COST);
+                        hi = lo + t.units + PAIR_COST;
+                    }
                     while (lo >= tiles[tile].line + (long long)(tiles[tile].units + PAIR_COST) * cfg_.n_kv_heads) tile++;
                     const int in = (int)(lo - tiles[tile].line), pair = tiles[tile].units + PAIR_COST, skip = std::max(0, PAIR_COST - in % pair);
                     s.tile = tile;

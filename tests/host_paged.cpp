@@ -12,7 +12,7 @@ struct Host {
 };
 
 extern "C" {
-// cfg: the nine fields of Config; lanes: {rows, unit, blocks, least} twice; returns null and the reason where the configuration is refused
+// cfg: the nine fields of Config; lanes: {rows, unit, blocks, least, join} twice; returns null and the reason where the configuration is refused
 Host* host_paged_create(const int* cfg, const int* lanes, int few, char* why, int len) {
     Config c = {cfg[0], cfg[1], cfg[2], cfg[3], cfg[4], cfg[5], cfg[6], cfg[7], cfg[8]};
     const std::string w = check_config(c);
@@ -21,10 +21,11 @@ Host* host_paged_create(const int* cfg, const int* lanes, int few, char* why, in
     if (!w.empty()) return nullptr;
     Lane l[2];
     for (int i = 0; i < 2; i++) {
-        l[i].rows = lanes[4 * i];
-        l[i].unit = lanes[4 * i + 1];
-        l[i].blocks = lanes[4 * i + 2];
-        l[i].least = lanes[4 * i + 3];
+        l[i].rows = lanes[5 * i];
+        l[i].unit = lanes[5 * i + 1];
+        l[i].blocks = lanes[5 * i + 2];
+        l[i].least = lanes[5 * i + 3];
+        l[i].join = lanes[5 * i + 4];
     }
     Host* h = new Host();
     h->c = c;

@@ -25,11 +25,11 @@ def lib(tmp_path_factory):
 
 
 class Plan:
-    def __init__(self, lib, heads=8, kv=2, size=64, page=16, pages=100, dtype=1, seqs=8, tokens=200, table=400, lanes=((16, 64, 37, 1), (128, 128, 5, 1)), few=16):
+    def __init__(self, lib, heads=8, kv=2, size=64, page=16, pages=100, dtype=1, seqs=8, tokens=200, table=400, lanes=((16, 64, 37, 1, 0), (128, 128, 5, 1, 0)), few=16):
         self.lib, self.kv, self.page, self.group, self.lanes, self.few = lib, kv, page, heads // max(1, kv), lanes, few
         why = C.create_string_buffer(300)
         cfg = (C.c_int * 9)(heads, kv, size, page, pages, dtype, seqs, tokens, table)
-        flat = (C.c_int * 8)(*lanes[0], *lanes[1])
+        flat = (C.c_int * 10)(*lanes[0], *lanes[1])
         self.h = lib.host_paged_create(cfg, flat, few, why, 300)
         self.why = why.value.decode()
         if self.h:
@@ -144,7 +144,7 @@ def test_every_unit_is_taken_once(lib, seed):
     pos0 = rng.integers(0, 700, n)
     n_new = np.where(rng.random(n) < 0.3, rng.integers(1, 150, n), rng.integers(0, 3, n))
     used = [-(-int(a + b) // page) for a, b in zip(pos0, n_new)]
-    lanes = ((16, 64, int(rng.integers(1, 300)), int(rng.integers(1, 4))), (128, 128, int(rng.integers(0, 20)), 1))
+    lanes = ((16, 64, int(rng.integers(1, 300)), int(rng.integers(1, 4)), int(rng.choice([0, 3, 20]))), (128, 128, int(rng.integers(0, 20)), 1, int(rng.choice([0, 4]))))
     p = Plan(lib, heads=kv * group, kv=kv, page=page, pages=sum(used) + 1, tokens=max(1, int(n_new.sum())), table=max(1, sum(used)), lanes=lanes, few=int(rng.choice([16, 64])))
     ids = rng.permutation(sum(used) + 1)
     tab, at = np.zeros((n, max(used) + 2), np.int32), 0
@@ -180,6 +180,16 @@ def test_every_unit_is_taken_once(lib, seed):
             assert (n_new[b] * group <= p.few) == (k == 0) or lanes[1][2] == 0
     assert sorted(seen) == [(b, r) for b in range(n) for r in range(n_new[b] * group)]
     assert p.dynamic + p.step[3] <= p.total
+
+
+def test_short_pairs_are_not_cut(lib):
+    p = Plan(lib, heads=8, kv=2, pages=100, lanes=((8, 64, 40, 1, 9), (128, 128, 5, 1, 0)))
+    ids = np.arange(99, dtype=np.int32).reshape(3, 33)
+    assert p([500, 0, 300], [1, 1, 2], ids) == "" and p.step[1] == 6 and p.step[4] == 0
+    assert len(walk(p, 0)) == sum(2 * u for u in (8, 1, 5))
+    many = Plan(lib, heads=8, kv=2, pages=100, lanes=((8, 64, 5, 1, 9), (128, 128, 5, 1, 0)))  # fewer blocks than pairs: equal shares
+    assert many([500, 0, 300], [1, 1, 2], ids) == "" and many.step[1] == 5
+    walk(many, 0)
 
 
 def test_capacity_holds_any_step_of_it(lib):
