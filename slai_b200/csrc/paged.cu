@@ -111,9 +111,9 @@ int fill_cache(slai_paged* p, const slai_paged_layer* layer, Cache* out) {
     out->page_stride = layer->page_stride;
     out->head_stride = layer->head_stride;
     out->pos_stride = layer->pos_stride;
-    out->page_size = c.page_size;
+    out->page_size = Div(c.page_size);
     out->n_kv = c.n_kv_heads;
-    out->group = c.n_q_heads / c.n_kv_heads;
+    out->group = Div(c.n_q_heads / c.n_kv_heads);
     out->hs = c.head_size;
     return SLAI_OK;
 }

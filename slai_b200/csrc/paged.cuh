@@ -11,7 +11,8 @@ struct Cache {
     int count_at, rows_at;  // offsets of the number of its rows, and of these
     char *keys, *values;
     long long page_stride, head_stride, pos_stride;  // elements
-    int page_size, n_kv, group, hs;
+    Div page_size, group;
+    int n_kv, hs;
 };
 
 struct AttnArgs {

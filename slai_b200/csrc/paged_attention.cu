@@ -1054,7 +1054,7 @@ Lane paged_attention_lane(int kv_dtype, int hs, int group, int sms) {
 Lane paged_attention_block_lane(int sms) {
     Lane l;
     l.rows = BR;
-    l.unit = 64;
+    l.unit = BP;
     l.least = 1;
     l.blocks = 2 * sms;
     return l;

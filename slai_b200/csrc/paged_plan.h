@@ -13,7 +13,39 @@
 #include <string>
 #include <vector>
 
+#ifdef __CUDACC__
+#define PAGED_HD __host__ __device__ __forceinline__
+#else
+#define PAGED_HD inline
+#endif
+
 namespace paged {
+
+// A divisor 1 .. 2^30 of numbers 0 .. 2^31 - 1: with L = ceil(log2 d) and m = floor(2^(31 + L) / d) + 1, m d is above 2^(31 + L) by at most 2^L, so that
+// n m / 2^(31 + L) is above n / d by less than 1 / d.
+struct Div {
+    int d = 1;
+    uint32_t mul = 0;
+    int shift = 0;  // L - 1
+    Div() = default;
+    explicit Div(int by) : d(by) {
+        if (by <= 1) return;
+        int L = 0;
+        while ((1ll << L) < by) L++;
+        mul = (uint32_t)(((1ull << (31 + L)) / (uint64_t)by) + 1);
+        shift = L - 1;
+    }
+    PAGED_HD operator int() const { return d; }
+};
+PAGED_HD int operator/(int n, const Div& by) {
+    if (by.d == 1) return n;
+#ifdef __CUDA_ARCH__
+    return (int)(__umulhi((uint32_t)n, by.mul) >> by.shift);
+#else
+    return (int)((uint32_t)(((uint64_t)(uint32_t)n * by.mul) >> 32) >> by.shift);
+#endif
+}
+PAGED_HD int operator%(int n, const Div& by) { return n - n / by * by.d; }
 
 constexpr int PAIR_COST = 2;
 
@@ -53,7 +85,7 @@ struct Lane {  // one of the two kinds of kernel
     int rows = 0, unit = 0;    // tile height, positions of a unit
     int blocks = 0;            // most blocks
     int least = 1;             // units a block has at least, if the line allows it
-    int join = 0;              // units that the join costs: where every pair can have a block, none is cut that is longer than a share by no more than this
+    int join = 0;              // units that the join costs: where every pair can have a block, none is cut that is longer than nine eighths of a share by no more than this
 };
 
 struct Layout {  // of the device copy, in ints
@@ -196,7 +228,7 @@ class Planner {
             long long pairs = (long long)n * cfg_.n_kv_heads;
             for (int i = 0; i < n; i++) longest = std::max(longest, tiles[i].units);
             const long long share = lanes_[k].blocks ? std::max<long long>(lanes_[k].least, U / lanes_[k].blocks) : 0;
-            const bool whole = lanes_[k].join > 0 && pairs <= lanes_[k].blocks && longest <= share + lanes_[k].join;
+            const bool whole = lanes_[k].join > 0 && pairs <= lanes_[k].blocks && longest <= share + share / 8 + lanes_[k].join;
             const int C = (int)(whole ? pairs : std::min<long long>(lanes_[k].blocks, (U + lanes_[k].least - 1) / std::max(1, lanes_[k].least)));
             step->blocks[k] = C;
             Start* st = reinterpret_cast<Start*>(out + lay_.starts[k]);

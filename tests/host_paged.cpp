@@ -12,6 +12,7 @@ struct Host {
 };
 
 extern "C" {
+int host_paged_div(int n, int d) { return n / Div(d); }
 // cfg: the nine fields of Config; lanes: {rows, unit, blocks, least, join} twice; returns null and the reason where the configuration is refused
 Host* host_paged_create(const int* cfg, const int* lanes, int few, char* why, int len) {
     Config c = {cfg[0], cfg[1], cfg[2], cfg[3], cfg[4], cfg[5], cfg[6], cfg[7], cfg[8]};
