@@ -7,10 +7,10 @@
 using namespace paged;
 
 namespace {
-#ifndef FEW_ROWS_DEF
-#define FEW_ROWS_DEF 32
-#endif
-constexpr int FEW_ROWS = FEW_ROWS_DEF;  // rows of a cache head that a sequence may bring and still go to the kernel for few
+// Rows of a cache head that a sequence may bring and surely goes to the kernel for few rows, and may bring and perhaps does.  us of a call, kernel for few / for many:
+// one sequence at 300, 32 heads: 64 rows 9.7 / 17.4; at 3000, 32 rows 34 / 35, 64 rows 55 / 36; 64 heads on 8 at 3000, 64 rows 20 / 29, 128 rows 30 / 30; 16
+// sequences of 64 heads on 8 at 2000: 16 rows 43 / 56, 32 rows 87 / 56.
+constexpr int FEW_ROWS = 16, PERHAPS_ROWS = 128;
 constexpr int SLOTS = 2;  // pinned copies of a plan: the next step is planned while the last one's copy is on its way
 
 bool capturing(slai_ctx* ctx) {
@@ -77,7 +77,7 @@ int make_handle(slai_ctx* ctx, slai_paged* p) {
     const int few_rows = f16 ? FEW_ROWS : std::max(few.rows, 4);
     Lane many;
     if (fast && (long long)c.max_tokens * group > few_rows) many = f16 ? paged_prompt_lane(sms) : paged_attention_block_lane(sms);
-    p->planner.init(c, few, many, few_rows);
+    p->planner.init(c, few, many, few_rows, PERHAPS_ROWS);
     const size_t bytes = (size_t)p->planner.lay().total * 4;
     SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_plan, bytes));
     for (int i = 0; i < SLOTS; i++) {

@@ -1045,6 +1045,8 @@ Lane paged_attention_lane(int kv_dtype, int hs, int group, int sms) {
         // us a call, cut / not cut where it can be: one token, 32 heads, at position 300 8.4 / 7.0, 515 8.8 / 10.2; a token of each of 8 sequences, 32 heads, at
         // 100 10.4 / 5.3, 515 20.6 / 16.9, 1000 31.4 / 27.6; 64 heads on 8 at 300 9.9 / 8.6, 515 11.2 / 12.5.
         l.join = 5;
+        l.fixed = 5;
+        l.each = kv_dtype == SLAI_KV_F16 ? 0.0054 : 0.0126;
     } else {
         l.rows = GR;
         l.blocks = 4 * sms;
@@ -1057,6 +1059,8 @@ Lane paged_attention_block_lane(int sms) {
     l.unit = BP;
     l.least = 1;
     l.blocks = 2 * sms;
+    l.fixed = 20;
+    l.each = 0.02;
     return l;
 }
 static int launch_lane(slai_ctx* ctx, const AttnArgs& A, int kv_dtype, int lane, int blocks, bool pdl) {

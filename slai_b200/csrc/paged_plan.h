@@ -85,6 +85,7 @@ struct Lane {  // one of the two kinds of kernel
     int rows = 0, unit = 0;    // tile height, positions of a unit
     int blocks = 0;            // most blocks
     int least = 1;             // units a block has at least, if the line allows it
+    double fixed = 0, each = 0;  // us of a launch, and of a unit in a launch that fills the GPU: which lane takes the sequences that either could take
     int join = 0;              // units that the join costs: where every pair can have a block, none is cut that is longer than nine eighths of a share by no more than this
 };
 
@@ -132,12 +133,15 @@ inline std::string check_config(const Config& c) {
 
 class Planner {
   public:
-    // `few`: rows a sequence may have (tokens * group) and still go to lane 0; lane 1 may be absent (blocks 0).
-    void init(const Config& c, const Lane& a, const Lane& b, int few) {
+    // Sequences of up to `few` rows (tokens * group) go to lane 0, of more than `most` to lane 1 (it may be absent, blocks 0); those between to where the step
+    // takes less time, by the lanes' `fixed` and `each`.
+    void init(const Config& c, const Lane& a, const Lane& b, int few, int most) {
         cfg_ = c;
         lanes_[0] = a;
         lanes_[1] = b;
         few_ = b.blocks ? few : 0x7fffffff;
+        most_ = std::max(few_, most);
+        now_ = few_;
         lay_ = layout(cfg_, lanes_);
         seen_.assign((size_t)c.n_pages, 0);
     }
@@ -151,6 +155,20 @@ class Planner {
         if (n_seq < 0 || n_seq > cfg_.max_seqs) return "n_seq must be 0 .. " + std::to_string(cfg_.max_seqs) + " (" + std::to_string(n_seq) + ")";
         if (n_seq > 0 && (!pos0 || !n_new || !tables)) return "lengths and tables are missing";
         const int group = cfg_.n_q_heads / cfg_.n_kv_heads, ps = cfg_.page_size;
+        const int before = now_;
+        struct Back {  // a step that is refused leaves no trace
+            int &now, was;
+            bool keep;
+            ~Back() {
+                if (!keep) now = was;
+            }
+        } back = {now_, before, false};
+        now_ = few_;
+        if (most_ > few_ && n_seq > 0) {
+            double us[2];
+            for (int way = 0; way < 2; way++) us[way] = cost(n_seq, pos0, n_new, group, way ? most_ : few_);
+            if (us[1] < us[0]) now_ = most_;
+        }
         long long rows = 0, entries = 0, line[2] = {0, 0};
         for (int b = 0; b < n_seq; b++) {
             if (pos0[b] < 0) return say("a negative number of cached positions", b, pos0[b]);
@@ -186,6 +204,7 @@ class Planner {
                 }
             }
         // -- nothing fails from here on --
+        back.keep = true;
         step->n_rows = (int)rows;
         out[lay_.count] = (int)rows;
         int* row = out + lay_.rows;
@@ -278,7 +297,21 @@ class Planner {
     }
 
   private:
-    int lane_of(int n_new) const { return (long long)n_new * (cfg_.n_q_heads / cfg_.n_kv_heads) <= few_ ? 0 : 1; }
+    int lane_of(int n_new) const { return (long long)n_new * (cfg_.n_q_heads / cfg_.n_kv_heads) <= now_ ? 0 : 1; }
+    // Roughly the us of a step whose sequences of up to `few` rows go to lane 0.
+    double cost(int n_seq, const int32_t* pos0, const int32_t* n_new, int group, long long few) const {
+        double line[2] = {0, 0};
+        for (int b = 0; b < n_seq; b++) {
+            if (n_new[b] <= 0 || pos0[b] < 0) continue;
+            const long long all = (long long)n_new[b] * group;
+            const int k = all <= few ? 0 : 1;
+            line[k] += (double)((all + lanes_[k].rows - 1) / lanes_[k].rows) * (((double)pos0[b] + n_new[b]) / lanes_[k].unit + PAIR_COST);
+        }
+        double us = 0;
+        for (int k = 0; k < 2; k++)
+            if (line[k] > 0) us += lanes_[k].fixed + lanes_[k].each * line[k] * cfg_.n_kv_heads;
+        return us;
+    }
     template <class F>
     void for_tiles(int, int pos0, int n_new, int group, F f) const {
         const Lane& l = lanes_[lane_of(n_new)];
@@ -296,7 +329,7 @@ class Planner {
     Config cfg_ = {};
     Lane lanes_[2];
     Layout lay_ = {};
-    int few_ = 0, mark_ = 0;
+    int few_ = 0, most_ = 0, now_ = 0, mark_ = 0;
     std::vector<int> seen_, tmp_;
 };
 

@@ -586,6 +586,8 @@ Lane paged_prompt_lane(int sms) {
     l.rows = 2 * PR;
     l.unit = PU;
     l.blocks = sms;
+    l.fixed = 13;
+    l.each = 0.0223;
     l.least = 1;
     l.join = 2;  // us a call, cut / not cut where it can be: 32 heads, 511 tokens 32.7 / 28.6, 1023 58 / 46; 64 heads on 8, 511 tokens behind 2000 101 / 81
     return l;

@@ -14,7 +14,7 @@ struct Host {
 extern "C" {
 int host_paged_div(int n, int d) { return n / Div(d); }
 // cfg: the nine fields of Config; lanes: {rows, unit, blocks, least, join} twice; returns null and the reason where the configuration is refused
-Host* host_paged_create(const int* cfg, const int* lanes, int few, char* why, int len) {
+Host* host_paged_create(const int* cfg, const int* lanes, int few, int most, char* why, int len) {
     Config c = {cfg[0], cfg[1], cfg[2], cfg[3], cfg[4], cfg[5], cfg[6], cfg[7], cfg[8]};
     const std::string w = check_config(c);
     strncpy(why, w.c_str(), len - 1);
@@ -30,7 +30,11 @@ Host* host_paged_create(const int* cfg, const int* lanes, int few, char* why, in
     }
     Host* h = new Host();
     h->c = c;
-    h->p.init(c, l[0], l[1], few);
+    l[0].fixed = 5;
+    l[0].each = 0.005;
+    l[1].fixed = 13;
+    l[1].each = 0.02;
+    h->p.init(c, l[0], l[1], few, most);
     return h;
 }
 void host_paged_destroy(Host* h) { delete h; }

@@ -25,12 +25,12 @@ def lib(tmp_path_factory):
 
 
 class Plan:
-    def __init__(self, lib, heads=8, kv=2, size=64, page=16, pages=100, dtype=1, seqs=8, tokens=200, table=400, lanes=((16, 64, 37, 1, 0), (128, 128, 5, 1, 0)), few=16):
-        self.lib, self.kv, self.page, self.group, self.lanes, self.few = lib, kv, page, heads // max(1, kv), lanes, few
+    def __init__(self, lib, heads=8, kv=2, size=64, page=16, pages=100, dtype=1, seqs=8, tokens=200, table=400, lanes=((16, 64, 37, 1, 0), (128, 128, 5, 1, 0)), few=16, most=0):
+        self.lib, self.kv, self.page, self.group, self.lanes, self.few, self.most = lib, kv, page, heads // max(1, kv), lanes, few, most
         why = C.create_string_buffer(300)
         cfg = (C.c_int * 9)(heads, kv, size, page, pages, dtype, seqs, tokens, table)
         flat = (C.c_int * 10)(*lanes[0], *lanes[1])
-        self.h = lib.host_paged_create(cfg, flat, few, why, 300)
+        self.h = lib.host_paged_create(cfg, flat, few, most, why, 300)
         self.why = why.value.decode()
         if self.h:
             lay = (C.c_int * 8)()
@@ -145,7 +145,7 @@ def test_every_unit_is_taken_once(lib, seed):
     n_new = np.where(rng.random(n) < 0.3, rng.integers(1, 150, n), rng.integers(0, 3, n))
     used = [-(-int(a + b) // page) for a, b in zip(pos0, n_new)]
     lanes = ((16, 64, int(rng.integers(1, 300)), int(rng.integers(1, 4)), int(rng.choice([0, 3, 20]))), (128, 128, int(rng.integers(0, 20)), 1, int(rng.choice([0, 2]))))
-    p = Plan(lib, heads=kv * group, kv=kv, page=page, pages=sum(used) + 1, tokens=max(1, int(n_new.sum())), table=max(1, sum(used)), lanes=lanes, few=int(rng.choice([16, 64])))
+    p = Plan(lib, heads=kv * group, kv=kv, page=page, pages=sum(used) + 1, tokens=max(1, int(n_new.sum())), table=max(1, sum(used)), lanes=lanes, few=int(rng.choice([16, 64])), most=int(rng.choice([0, 128])))
     ids = rng.permutation(sum(used) + 1)
     tab, at = np.zeros((n, max(used) + 2), np.int32), 0
     for b, u in enumerate(used):
@@ -177,7 +177,7 @@ def test_every_unit_is_taken_once(lib, seed):
             assert units == (p0 + (first + rows_in - 1) // group) // unit + 1
             assert tiles[t] == {h: list(range(units)) for h in range(kv)}
             seen += [(b, r) for r in range(first, first + rows_in)]
-            assert (n_new[b] * group <= p.few) == (k == 0) or lanes[1][2] == 0
+            assert lanes[1][2] == 0 or (k == 0 and n_new[b] * group <= max(p.few, p.most)) or (k == 1 and n_new[b] * group > p.few)
     assert sorted(seen) == [(b, r) for b in range(n) for r in range(n_new[b] * group)]
     assert p.dynamic + p.step[3] <= p.total
 
@@ -190,6 +190,16 @@ def test_short_pairs_are_not_cut(lib):
     many = Plan(lib, heads=8, kv=2, pages=100, lanes=((8, 64, 5, 1, 9), (128, 128, 5, 1, 0)))  # fewer blocks than pairs: equal shares
     assert many([500, 0, 300], [1, 1, 2], ids) == "" and many.step[1] == 5
     walk(many, 0)
+
+
+def test_which_lane_takes_what_either_could(lib):
+    """A few rows more than the kernel for few surely takes: alone they go there, many such sequences to the other kernel, and beside a long chunk too."""
+    p = Plan(lib, heads=8, kv=2, pages=2000, seqs=64, tokens=2000, table=4000, lanes=((8, 64, 40, 1, 0), (256, 128, 20, 1, 0)), most=128)
+    ids = np.arange(1600, dtype=np.int32).reshape(40, 40)
+    assert p([100], [16], ids[:1]) == "" and p.step[1] > 0 and p.step[2] == 0
+    assert p([500] * 40, [16] * 40, ids) == "" and p.step[1] == 0 and p.step[2] > 0
+    assert p([500] * 40, [4] * 40, ids) == "" and p.step[1] > 0 and p.step[2] == 0
+    assert p([100, 0], [4, 600], ids[:2]) == "" and p.step[1] > 0 and p.step[2] > 0
 
 
 def test_division(lib):
