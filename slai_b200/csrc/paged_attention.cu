@@ -823,9 +823,10 @@ int launch_few32_of(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
 
 // ---- f32 caches, many rows -----------------------------------------------------------------------------------------------------------
 // 64 rows against 32 positions at a time, both in shared memory (keys and values in two buffers, asynchronous copies); f32 arithmetic, two at a time.  Thread (ty, tx) of
-// 8 x 16 has rows 8 ty .. + 7: scores of positions tx and tx + 16, and of the sums of values the dimensions 4 tx .. + 3 (and 64 + 4 tx .. + 3); a row's
-// sixteen threads are half a warp.  Per four dimensions a thread reads ten pieces of 16 bytes for 64 products, per position four: the multipliers bound it.
-constexpr int BT = 128, BR = 64, BP = 32;
+// 16 x 16 has rows 4 ty .. + 3: scores of positions tx and tx + 16, and of the sums of values the dimensions 4 tx .. + 3 (and 64 + 4 tx .. + 3); a row's
+// sixteen threads are half a warp.  Shared memory and multipliers take about the same time.  (8 x 16 threads with 8 rows each read less, but a tile of 37 rows
+// was three warps, each alone on its scheduler: 5.5 us for 32 positions.)
+constexpr int BT = 256, BR = 64, BP = 32, BN = 4;  // threads, rows, positions; rows a thread
 template <int HS>
 struct Block32 {
     static constexpr int KS = HS + 4, Q = BR * KS, K = BP * KS, V = BP * HS, PS = BR + 4;
@@ -852,13 +853,13 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
         const bool whole = n == t.units;
         const int lo = unit * A.unit, hi = min((unit + n) * A.unit, t.pos0 + (t.first + t.rows - 1) / c.group + 1);  // positions [lo, hi)
         const int tiles = (hi - lo + BP - 1) / BP;
-        auto request = [&](int i) {  // warp w brings rows 8 w .. + 7
+        auto request = [&](int i) {  // warp w brings rows 4 w .. + 3
             const int p0 = lo + i * BP;
             const long long at = p0 + lane < hi ? 4 * place_of(c, t.table, p0 + lane, head) : -1;
             const uint32_t kd = kv_a + 4 * (i & 1) * (L::K + L::V), vd = kd + 4 * L::K;
 #pragma unroll
-            for (int k = 0; k < 8; k += STEP) {
-                const int r = 8 * warp + k + rl;
+            for (int k = 0; k < 4; k += STEP) {
+                const int r = 4 * warp + k + rl;
                 const long long a = __shfl_sync(0xffffffffu, at, r);
                 const uint32_t bytes = a >= 0 && ch < chunks ? 16u : 0u;  // (none: zeros, nothing is read)
                 const long long src = bytes ? a + 16 * ch : 0;
@@ -869,8 +870,8 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
         // queries: all on their way at once
         if (A.qvec) {
 #pragma unroll
-            for (int k = 0; k < BR / 4; k += STEP) {
-                const int r = 4 * k + 4 * rl + warp, pr = t.first + min(r, t.rows - 1), tok = pr / c.group;
+            for (int k = 0; k < BR / 8; k += STEP) {
+                const int r = 8 * k + 8 * rl + warp, pr = t.first + min(r, t.rows - 1), tok = pr / c.group;
                 const uint32_t bytes = r < t.rows && ch < chunks ? 16u : 0u;
                 const float* q = A.q + (bytes ? (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs + 4 * ch : 0);
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_a + 4 * (r * KS + 4 * ch)), "l"(__cvta_generic_to_global(q)), "r"(bytes) : "memory");
@@ -886,14 +887,14 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
         request(0);
         asm volatile("cp.async.commit_group;" ::: "memory");
         const float by = A.scale * LOG2E;  // scores as powers of two's exponents
-        const bool on = 16 * warp < t.rows;  // this warp has rows
-        int vis[8];  // last position a row sees
+        const bool on = 8 * warp < t.rows;  // this warp has rows
+        int vis[BN];  // last position a row sees
 #pragma unroll
-        for (int r = 0; r < 8; r++) vis[r] = 8 * ty + r < t.rows ? t.pos0 + (t.first + 8 * ty + r) / c.group : 0x7fffffff;
-        f32x2 acc[8][2 * DV];
-        float m[8], l[8];
+        for (int r = 0; r < BN; r++) vis[r] = BN * ty + r < t.rows ? t.pos0 + (t.first + BN * ty + r) / c.group : 0x7fffffff;
+        f32x2 acc[BN][2 * DV];
+        float m[BN], l[BN];
 #pragma unroll
-        for (int r = 0; r < 8; r++) {
+        for (int r = 0; r < BN; r++) {
 #pragma unroll
             for (int d = 0; d < 2 * DV; d++) acc[r][d] = 0;
             m[r] = -INFINITY;
@@ -908,22 +909,22 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
             const float* vs = ks + L::K;
             const int p0 = lo + i * BP;
             if (on) {
-                f32x2 sc[8][2];
+                f32x2 sc[BN][2];
 #pragma unroll
-                for (int r = 0; r < 8; r++) sc[r][0] = sc[r][1] = 0;
+                for (int r = 0; r < BN; r++) sc[r][0] = sc[r][1] = 0;
 #pragma unroll 4
                 for (int d = 0; d < HS; d += 4) {
                     const ulonglong2 k0 = *reinterpret_cast<const ulonglong2*>(ks + tx * KS + d), k1 = *reinterpret_cast<const ulonglong2*>(ks + (tx + 16) * KS + d);
 #pragma unroll
-                    for (int r = 0; r < 8; r++) {
-                        const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q_s + (8 * ty + r) * KS + d);
+                    for (int r = 0; r < BN; r++) {
+                        const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q_s + (BN * ty + r) * KS + d);
                         sc[r][0] = fma2(q2.x, k0.x, fma2(q2.y, k0.y, sc[r][0]));
                         sc[r][1] = fma2(q2.x, k1.x, fma2(q2.y, k1.y, sc[r][1]));
                     }
                 }
-                float w[8][2];
+                float w[BN][2];
 #pragma unroll
-                for (int r = 0; r < 8; r++) {
+                for (int r = 0; r < BN; r++) {
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         const float2 x = unpack2(sc[r][u]);
@@ -945,8 +946,8 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int r = 0; r < 8; r += 4)
-                        *reinterpret_cast<float4*>(p_s + (tx + 16 * u) * L::PS + 8 * ty + r) = make_float4(w[r][u], w[r + 1][u], w[r + 2][u], w[r + 3][u]);
+                    for (int r = 0; r < BN; r += 4)
+                        *reinterpret_cast<float4*>(p_s + (tx + 16 * u) * L::PS + BN * ty + r) = make_float4(w[r][u], w[r + 1][u], w[r + 2][u], w[r + 3][u]);
                 __syncwarp();
 #pragma unroll 2
                 for (int j = 0; j < BP; j++) {
@@ -954,8 +955,8 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
 #pragma unroll
                     for (int d = 0; d < DV; d++) v2[d] = *reinterpret_cast<const ulonglong2*>(vs + j * HS + 64 * d + 4 * tx);
 #pragma unroll
-                    for (int r0 = 0; r0 < 8; r0 += 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(p_s + j * L::PS + 8 * ty + r0);
+                    for (int r0 = 0; r0 < BN; r0 += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(p_s + j * L::PS + BN * ty + r0);
                         const float xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
@@ -975,10 +976,10 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
         if (on) {
             unsigned int bad = 0;  // of this thread's rows
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
+            for (int r = 0; r < BN; r++) {
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
-                const int row = 8 * ty + r;
+                const int row = BN * ty + r;
                 const bool there = row < t.rows;
                 const int pr = t.first + min(row, t.rows - 1), tok = pr / c.group;
                 float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs : A.part + (slot + min(row, t.rows - 1)) * hs;
@@ -1002,10 +1003,10 @@ __global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_
             }
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
-            const unsigned int both = __shfl_sync(0xffffffffu, bad, 0) | __shfl_sync(0xffffffffu, bad, 16) << 8;  // of the warp's 16 rows
-            for (int r = 0; r < 16 && both; r++)
+            const unsigned int both = __shfl_sync(0xffffffffu, bad, 0) | __shfl_sync(0xffffffffu, bad, 16) << BN;  // of the warp's rows
+            for (int r = 0; r < 2 * BN && both; r++)
                 if (both >> r & 1) {
-                    const int row = 16 * warp + r, pr = t.first + row, tok = pr / c.group;
+                    const int row = 2 * BN * warp + r, pr = t.first + row, tok = pr / c.group;
                     float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs : A.part + (slot + row) * hs;
                     __syncwarp();
                     row_again<float>(A, t, head, row, lo, hi, o, whole ? nullptr : A.part_ml + (slot + row) * 2);
