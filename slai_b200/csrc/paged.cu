@@ -2,6 +2,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <exception>
+
 #include "paged.cuh"
 
 using namespace paged;
@@ -149,10 +151,16 @@ SLAI_API int slai_paged_create(slai_ctx* ctx, const slai_paged_config* cfg, slai
     const std::string why = check_config(c);
     SLAI_REQUIRE(ctx, why.empty(), SLAI_ERR_SHAPE, "paged: %s", why.c_str());
     SLAI_REQUIRE(ctx, !capturing(ctx), SLAI_ERR_INVALID_ARG, "paged: a handle cannot be made while a pass is recorded");
-    slai_paged* p = new slai_paged();
-    p->ctx = ctx;
-    p->cfg = c;
-    const int rc = make_handle(ctx, p);
+    slai_paged* p = nullptr;
+    int rc;
+    try {
+        p = new slai_paged();
+        p->ctx = ctx;
+        p->cfg = c;
+        rc = make_handle(ctx, p);
+    } catch (const std::exception&) {  // (the table of pages: up to 8 GB for 2^31 pages of one position)
+        rc = slai_set_error(ctx, SLAI_ERR_OOM, "paged: no host memory for %d pages and %d table entries", c.n_pages, c.max_table);
+    }
     if (rc) {
         cudaGetLastError();
         delete p;
@@ -178,7 +186,12 @@ SLAI_API int slai_paged_step(slai_paged* p, int n_seq, const int32_t* h_pos0, co
     SLAI_CHECK_CUDA(ctx, cudaEventSynchronize(p->copied[p->slot]));  // the copy that last left this slot
     int* h = p->h_plan[p->slot];
     Step st;
-    const std::string why = p->planner.plan(n_seq, h_pos0, h_n_new, h_tables, table_ld, h, &st);
+    std::string why;
+    try {
+        why = p->planner.plan(n_seq, h_pos0, h_n_new, h_tables, table_ld, h, &st);
+    } catch (const std::exception&) {
+        return slai_set_error(ctx, SLAI_ERR_OOM, "paged step: no host memory");
+    }
     SLAI_REQUIRE(ctx, why.empty(), SLAI_ERR_SHAPE, "paged step: %s", why.c_str());
     const Layout& L = p->planner.lay();
     const size_t head = (size_t)L.rows + 2 * (size_t)st.n_rows, gap = L.dynamic - head;

@@ -9,7 +9,7 @@
 
 namespace {
 
-constexpr int QT = 256;
+constexpr int QT = 256, QU = 4;  // threads; heads a warp takes one after the other where there are many
 
 // cos and sin of pair i at position p
 __device__ __forceinline__ float2 turn(const double* turns, int i, int p) {
@@ -114,13 +114,11 @@ __global__ void __launch_bounds__(QT) qk_any_kernel(const QkArgs A) {
 }
 
 // Heads of a multiple of 8 elements on 16-byte boundaries: LPH lanes take a head, 8 elements a lane (two 16-byte pieces that hold four whole pairs in either
-// variant), a warp 32 / LPH * U heads of one token, whose angles it needs once.
-#ifndef QK_MINB
-#define QK_MINB 3
-#define QK_U 4
-#endif
+// variant), a warp 32 / LPH * U heads of one token, whose angles it needs once.  Memory bounds it: 4095 tokens of 64 + 8 heads of 128, 302 MB, 52.7 us (89 % of the
+// copy rate); 1919 tokens of 64 + 8 + 8 appended, 149 MB, 29.2 us (79 %).  us of the two by U and blocks an SM: 1 x 6 70.2, 36.5; 2 x 4 60.2, 32.1; 2 x 6 63.9, 34.0;
+// 4 x 3 57.5, 31.7; 8 x 2 64.7, 40.0; 4 x 3 with loads that leave L2 first 52.7, 29.2.
 template <int LPH, int U, bool NEOX>
-__global__ void __launch_bounds__(QT, QK_MINB) qk_vec_kernel(const QkArgs A) {
+__global__ void __launch_bounds__(QT, 3) qk_vec_kernel(const QkArgs A) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int HPW = 32 / LPH;
@@ -139,8 +137,8 @@ __global__ void __launch_bounds__(QT, QK_MINB) qk_vec_kernel(const QkArgs A) {
         x[u][0] = x[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (h < heads && mine) {
             const float* in = head_of(A, row, ps.y, h).in;
-            x[u][0] = __ldcg(reinterpret_cast<const float4*>(in + e0));
-            x[u][1] = __ldcg(reinterpret_cast<const float4*>(in + e1));
+            x[u][0] = __ldcs(reinterpret_cast<const float4*>(in + e0));  // (read once: out of L2 before what the attention reads next)
+            x[u][1] = __ldcs(reinterpret_cast<const float4*>(in + e1));
         }
     }
     float2 cs[4];
@@ -198,9 +196,9 @@ int launch_vec(slai_ctx* ctx, QkArgs& A, long long heads, bool pdl) {
     constexpr int HPW = 32 / LPH;
     auto blocks = [&](int u) { return ((long long)A.rows * ((heads + HPW * u - 1) / (HPW * u)) + QT / 32 - 1) / (QT / 32); };
     // Several heads a warp where that leaves enough warps to keep the memory busy.
-    const bool many = blocks(QK_U) >= 8 * (ctx->sm_count > 0 ? ctx->sm_count : 148);
+    const bool many = blocks(QU) >= 8 * (ctx->sm_count > 0 ? ctx->sm_count : 148);
     SLAI_REQUIRE(ctx, blocks(1) <= 0x7fffffffll, SLAI_ERR_SHAPE, "rows: too many (%d tokens of %lld heads)", A.rows, heads);
-    return many ? launch_dependent(ctx, qk_vec_kernel<LPH, QK_U, NEOX>, dim3((unsigned)blocks(QK_U)), QT, 0, pdl, A)
+    return many ? launch_dependent(ctx, qk_vec_kernel<LPH, QU, NEOX>, dim3((unsigned)blocks(QU)), QT, 0, pdl, A)
                 : launch_dependent(ctx, qk_vec_kernel<LPH, 1, NEOX>, dim3((unsigned)blocks(1)), QT, 0, pdl, A);
 }
 

@@ -203,14 +203,14 @@ class Planner {
                     seen_[id] = pass ? written : read;
                 }
             }
+        std::vector<int>& tab_at = tmp_;
+        tab_at.assign((size_t)std::max(1, n_seq), 0);
         // -- nothing fails from here on --
         back.keep = true;
         step->n_rows = (int)rows;
         out[lay_.count] = (int)rows;
         int* row = out + lay_.rows;
         int at = lay_.dynamic, r0 = 0;
-        std::vector<int>& tab_at = tmp_;
-        tab_at.assign((size_t)std::max(1, n_seq), 0);
         for (int b = 0; b < n_seq; b++) {
             if (n_new[b] == 0) continue;
             const int32_t* tab = tables + (int64_t)b * ld;

@@ -223,6 +223,15 @@ CASES = [
     (2, 1, 65, 7, [20, 0], [1, 19]),                          # odd sizes
     (2, 1, 1, 1, [20, 0], [1, 3]),
     (3, 1, 20, 3, [2, 100], [3, 1]),
+    # chunks through tiles of 256 rows: heads narrower than the tile, pages that divide 128 positions, that are divided by them, neither
+    (3, 3, 48, 20, [0, 45], [150, 131]),
+    (4, 2, 56, 8, [130], [129]),
+    (2, 1, 64, 128, [100, 256], [140, 200]),
+    (3, 1, 128, 24, [111], [131]),
+    (2, 2, 104, 256, [300], [300]),
+    (2, 1, 128, 16, [9000], [150]),                           # few tiles over many blocks
+    (1, 1, 128, 512, [1000, 0], [128, 129]),
+    (40, 1, 128, 16, [77], [20]),                             # a group wider than a warp
 ]
 
 
@@ -319,6 +328,53 @@ def test_results_repeat(ctx, backend):
     for _ in range(5):
         ctx.paged_attention(P.kv, P.layer, qd, out)
         assert (out.to_numpy().reshape(first.shape) == first).all()
+
+
+@pytest.mark.parametrize("n_new", [[1, 1], [140, 1]])
+def test_a_cache_beyond_32_bits(ctx, backend, n_new):
+    """Pages 2^28 elements apart: the last lie 5 GB behind the first."""
+    hq, hk, hs, page, n_pages, stride = 4, 2, 128, 64, 11, 1 << 28
+    rng = np.random.default_rng(2)
+    free, _ = backend.mem_info()
+    assert free > 3 * n_pages * stride * 2
+
+    class Far:  # a buffer of n elements
+        def __init__(self):
+            self.n = (n_pages - 1) * stride + hk * page * hs
+            self.ptr = backend.malloc(self.n * 2)
+
+        def __len__(self):
+            return self.n
+
+    keys, values = Far(), Far()
+    try:
+        kv = PagedKv(backend, hq, hk, hs, page, n_pages, F16, max_seqs=2, max_tokens=200)
+        layer = PagedLayer(keys, values, stride, page * hs, hs)
+        tables = np.array([[10, 9, 0, 8], [7, 6, 5, -1]], np.int32)
+        pos0 = [100, 130]
+        held = [[rng.standard_normal((p + n, hk, hs)).astype(np.float16) for p, n in zip(pos0, n_new)] for _ in range(2)]
+        for w, buf in enumerate((keys, values)):
+            for b in range(2):
+                x = held[w][b]
+                for i in range(-(-len(x) // page)):
+                    block = np.zeros((hk, page, hs), np.float16)
+                    part = x[i * page:(i + 1) * page]
+                    block[:, :len(part)] = part.transpose(1, 0, 2)
+                    backend.write_buffer(buf.ptr + int(tables[b, i]) * stride * 2, block)
+        kv.step(pos0, n_new, tables)
+        rows = sum(n_new)
+        # the step's own keys and values go in by the append (no norm, no rotation)
+        k, v = (np.concatenate([held[w][b][p:] for b, p in enumerate(pos0)]).astype(np.float32) for w in range(2))
+        ctx.paged_append(kv, layer, QkNormRope(hs, 0, hk, None), None, backend.vector(k), backend.vector(v), None)
+        q, out = rng.standard_normal((rows, hq, hs)).astype(np.float32), backend.zeros(rows * hq * hs)
+        ctx.paged_attention(kv, layer, backend.vector(q), out)
+        got, at = out.to_numpy().reshape(rows, hq, hs), 0
+        for b, (p, n) in enumerate(zip(pos0, n_new)):
+            check(got[at:at + n], *R.attention(q[at:at + n], held[0][b], held[1][b], p, hs**-0.5))
+            at += n
+    finally:
+        for buf in (keys, values):
+            backend.free(buf.ptr)
 
 
 # ---- together ----------------------------------------------------------------------------------------------------------
