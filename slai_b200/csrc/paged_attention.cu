@@ -360,12 +360,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
 // ---- few rows: the end of a block's part of a pair ------------------------------------------------------------------------------
 // Each of the block's FW warps has a maximum, a sum and an output of every row for its own positions: `so` [warp][rows][HS] (WF floats apart), ml_s; outputs and sums are
 // `carried` times their size apart.  They become the result, or the block's slot of `part`.
-#ifndef FEW_W
-#define FEW_W 4
-#define FEW_S 3
-#define FEW_B 2
-#endif
-constexpr int FW = FEW_W, FT = 32 * FW, FR = 8;
+constexpr int FW = 4, FT = 32 * FW, FS = 3, FB = 2, FR = 8;  // warps, threads, stages of a warp, blocks an SM, rows
 template <int HS, typename T>
 __device__ __forceinline__ void few_end(const AttnArgs& A, const Start& s, const Tile& t, int head, int unit, bool whole, int lo, int hi, const float* so, int WF,
                                         const float2 (*ml_s)[FR], unsigned int& bad, float carried) {
@@ -416,14 +411,16 @@ __device__ __forceinline__ void few_end(const AttnArgs& A, const Start& s, const
 // positions (the matrix unit truncates when it adds) and go on in registers.
 // What such a call costs is reading the cache: each of the block's warps has a ring of its own of stages of 16 positions, brought in by asynchronous
 // copies that go around the registers, and takes every FW-th 16 positions of the block's share with a running maximum and sum of its own; they are joined in shared
-// memory at the end.
-constexpr int FP = 16, FS = FEW_S;
+// memory at the end.  A token of each of 64 sequences of 100 to 3900 positions, 64 heads on 8: 529 MB in 96 to 100 us, 82 to 85 % of the copy rate; a token at 32750: 134 MB in
+// 33 us, 27 of them this kernel's (24 us of loop, of which the first positions' way takes 6), the rest the join's.  us of the two by warps, stages, blocks an
+// SM: 4, 3, 2 102, 33; 4, 2, 3 97, 42; 6, 2, 2 103, 46; 8, 3, 1 119, 31.  (16 rows to an instruction, high and low parts one after the other: 161, 53.)
+constexpr int FP = 16;
 template <int HS>
 constexpr int FEW_SMEM = FW * FS * 2 * FP * HS * 2;
 
 // ALIGNED: pages hold a multiple of 16 positions, so 16 of them have one page.
 template <int HS, bool ALIGNED>
-__global__ void __launch_bounds__(FT, FEW_B) paged_attn_few_kernel(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(FT, FB) paged_attn_few_kernel(const __grid_constant__ AttnArgs A) {
     constexpr int ROW = HS * 2, CH = HS / 8, TILE = FP * ROW, STAGE = 2 * TILE, KS = HS / 16, NT8 = HS / 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(128) unsigned char few_sm[];
@@ -604,36 +601,14 @@ int launch_few(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
 
 // ---- f32 caches, few rows ----------------------------------------------------------------------------------------------------------
 // The same with f32 arithmetic: stages of 8 positions; four lanes take a position's score (a quarter of the dimensions each, the queries from shared memory), a lane
-// four dimensions of the output.  R: rows that there is room for (1, 4 or 8).  Reading the cache bounds it: 8 rows take about half of the instructions that
-// there is time for meanwhile.
+// four dimensions of the output.  R: rows that there is room for (1, 4 or 8; 1 where a cache head has one query head: 69 -> 55 us for the following).  Reading the
+// cache bounds it: a token of each of 8 sequences of 515 to 1546 positions, 32 heads, pages of 20: 271 MB in 55 us, 76 % of the copy rate.
 constexpr int EP = 8;
 template <int HS, int R>
 constexpr int FEW32_SMEM = FW * FS * 2 * EP * HS * 4 + R * HS * 4 + FW * EP * R * 4;
 
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float a, float b) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(f32x2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 template <int HS, int R, bool ALIGNED>
-__global__ void __launch_bounds__(FT, FEW_B) paged_attn_few32_kernel(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(FT, FB) paged_attn_few32_kernel(const __grid_constant__ AttnArgs A) {
     constexpr int ROW = HS * 4, CH = HS / 4, TILE = EP * ROW, STAGE = 2 * TILE, STEP = 32 / CH;  // STEP: rows a pass of the warp covers
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ __align__(128) unsigned char few_sm[];
@@ -825,7 +800,8 @@ int launch_few32_of(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
 // 64 rows against 32 positions at a time, both in shared memory (keys and values in two buffers, asynchronous copies); f32 arithmetic, two at a time.  Thread (ty, tx) of
 // 16 x 16 has rows 4 ty .. + 3: scores of positions tx and tx + 16, and of the sums of values the dimensions 4 tx .. + 3 (and 64 + 4 tx .. + 3); a row's
 // sixteen threads are half a warp.  Shared memory and multipliers take about the same time.  (8 x 16 threads with 8 rows each read less, but a tile of 37 rows
-// was three warps, each alone on its scheduler: 5.5 us for 32 positions.)
+// was three warps, each alone on its scheduler: 5.5 us for 32 positions.)  31 TFLOP/s with 511 tokens behind 2000; 37 tokens behind 300, 32 heads: 25 us, latencies
+// of one tile and the join.
 constexpr int BT = 256, BR = 64, BP = 32, BN = 4;  // threads, rows, positions; rows a thread
 template <int HS>
 struct Block32 {
@@ -1042,7 +1018,7 @@ Lane paged_attention_lane(int kv_dtype, int hs, int group, int sms) {
     l.least = 2;
     if (paged_attention_few(kv_dtype, hs)) {
         l.rows = kv_dtype == SLAI_KV_F16 || group > 4 ? FR : group == 1 ? 1 : 4;
-        l.blocks = FEW_B * sms;
+        l.blocks = FB * sms;
         // us a call, cut / not cut where it can be: one token, 32 heads, at position 300 8.4 / 7.0, 515 8.8 / 10.2; a token of each of 8 sequences, 32 heads, at
         // 100 10.4 / 5.3, 515 20.6 / 16.9, 1000 31.4 / 27.6; 64 heads on 8 at 300 9.9 / 8.6, 515 11.2 / 12.5.
         l.join = 5;

@@ -1,21 +1,28 @@
 // Paged attention for many rows and f16 caches: chunks of prompts, on the 5th-generation tensor cores.
 //
 // A tile is 256 rows (token, query head of the group), two halves A and B of 128 that share the keys and values: scores S = Q K^T of 128 x 128 positions and
-// sums P V of them are products of tcgen05.mma with their f32 results in tensor memory, where a thread has a row.  Queries and weights are pairs of halves
-// (22 bits), two products each: one rounding of either to f16 would put 1e-4 into the result, the pairs leave 3e-7.  The tensor core truncates when it adds:
-// both sums end with their 128 positions, and a half's output goes on in its threads' registers, times the factor by which the running maximum moved.
+// sums P V of them are products of tcgen05.mma with their f32 results in tensor memory, where a lane has a row.  Queries and weights are pairs of halves
+// (22 bits), two products each: one rounding of either to f16 would put 1e-4 into the result, the pairs leave 5e-7 (1e-6 behind 7000 positions; f32 arithmetic 2e-6).
+// A row of queries is carried times a power of two that puts its largest element below 2^15: elements down to 2^-17 of that keep their 22 bits, smaller ones are
+// off by up to 2^-40 of the largest.  The tensor core truncates when it adds: both sums end with their 128 positions, and a half's output goes on in its
+// threads' registers, times the factor by which the running maximum moved.
 //
 //   warp 0       issues the products: QK_A(j), PV_B(j-1), QK_B(j), PV_A(j): while one half's threads are at its softmax the tensor cores are at the other's
 //                products.  Three regions of 128 columns of tensor memory hold scores and weights in turn, one the outputs.
 //   warps 1-3    keys and values of 128 positions, in turn, into a tile of shared memory each: by TMA, a box per page, where pages divide 128 positions or are
 //                divided by them, else (and where a sequence ends inside the tile: positions behind the last are zeros, whatever the page holds there) by
-//                asynchronous 16-byte copies that write the swizzle themselves.  (All by the latter, a tile took as long as the two products that hide it: 522 us for
-//                1023 tokens of 64 heads on 8 at position 7001.)
+//                asynchronous 16-byte copies that write the swizzle themselves.  (All by the latter: 522 us instead of 494.)
 //   warps 4-11   half A, warps 12-19 half B: softmax, two threads a row, 64 positions and then 64 dimensions each: S out of tensor memory once for its maximum and once
-//                more for the weights, which take its columns' place as the next product's operand; then the product's result.  (With one thread a row its
-//                chain of latencies was 2.1 us a unit, twice what the other half's products hide.)
+//                more for the weights, which take its columns' place as the next product's operand; then the product's result.
 // A region is written again by the third QK after its own; by then the PV that read it is complete: before each PV its issuer waits until the output of the PV
 // before has been read (one region for all of them), so that only the last PV issued can be under way.
+//
+// What bounds it: 1023 tokens of 64 heads on 8 behind 7001 positions, 457 to 465 us, 545 TFLOP/s, 1090 executed; the kernel itself 409 us, 1230 executed, where the card's
+// power allows 1400 (the clock falls to 1.55 GHz).  A unit of 128 positions takes 5600 cycles for products of 4096: a half's softmax (maximum 500, weights
+// 2000: 16 exponentials a cycle and SM, the wait for tensor memory), its product, the read of that and the next scores are one chain, longer than the other half's
+// products.  Few tokens: 511 of 32 heads 24.7 us, of which the queries' way to shared memory takes 5, the results' 3, the join of tiles on several blocks 5.
+// Tried and taken back: a row a thread with twice the registers (chunk 453 us, but 139 for 96 us with 2047 tokens of 32 heads); half of the exponentials by a
+// polynomial (547 for 497); queries by eight lanes a row, in a function of their own or not (the softmax's registers came out worse: 480 to 580).
 //
 // Every wait is bounded (common.cuh, bounded_wait).
 #include <type_traits>
@@ -78,29 +85,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t a, uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void tmem_st4(uint32_t a, const uint32_t (&r)[4]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
-}
-// Two f32 at a time
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float a, float b) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 pack2(uint32_t a, uint32_t b) { return pack2(__uint_as_float(a), __uint_as_float(b)); }
-__device__ __forceinline__ float2 unpack2(f32x2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
