@@ -83,6 +83,8 @@ static_assert(sizeof(Tile) == 32 && sizeof(Start) == 64 && sizeof(Join) == 32 &&
 
 struct Lane {  // one of the two kinds of kernel
     int rows = 0, unit = 0;    // tile height, positions of a unit
+    int low = 0;               // a lower tile height (0: none), for steps that are sooner done so.  What decides, for (rows, low): us of a unit of the block with the most,
+    double unit_us[2] = {}, whole_us[2] = {}, cut_us[2] = {};  // and of all else, where pairs are whole and where they are cut
     int blocks = 0;            // most blocks
     int least = 1;             // units a block has at least, if the line allows it
     double fixed = 0, each = 0;  // us of a launch, and of a unit in a launch that fills the GPU: which lane takes the sequences that either could take
@@ -93,7 +95,7 @@ struct Layout {  // of the device copy, in ints
     int starts[2], joins[2], count, rows, dynamic, total;  // count: numbers of the step's rows and of each lane's joins
 };
 inline int tiles_cap(const Config& c, const Lane& l) {
-    return l.blocks ? (int)std::min<long long>(((long long)c.max_tokens * (c.n_q_heads / c.n_kv_heads)) / l.rows + c.max_seqs, 1ll << 30) : 0;
+    return l.blocks ? (int)std::min<long long>(((long long)c.max_tokens * (c.n_q_heads / c.n_kv_heads)) / (l.low ? l.low : l.rows) + c.max_seqs, 1ll << 30) : 0;
 }
 inline Layout layout(const Config& c, const Lane (&lanes)[2]) {
     Layout L;
@@ -168,6 +170,10 @@ class Planner {
             double us[2];
             for (int way = 0; way < 2; way++) us[way] = cost(n_seq, pos0, n_new, group, way ? most_ : few_);
             if (us[1] < us[0]) now_ = most_;
+        }
+        for (int k = 0; k < 2; k++) {
+            height_[k] = lanes_[k].rows;
+            if (lanes_[k].low && takes(k, 1, n_seq, pos0, n_new, group) < takes(k, 0, n_seq, pos0, n_new, group)) height_[k] = lanes_[k].low;
         }
         long long rows = 0, entries = 0, line[2] = {0, 0};
         for (int b = 0; b < n_seq; b++) {
@@ -312,15 +318,35 @@ class Planner {
             if (line[k] > 0) us += lanes_[k].fixed + lanes_[k].each * line[k] * cfg_.n_kv_heads;
         return us;
     }
+    // Roughly the us of lane k's sequences in tiles of its rows, or of its lower height.
+    double takes(int k, int lower, int n_seq, const int32_t* pos0, const int32_t* n_new, int group) const {
+        const Lane& l = lanes_[k];
+        const int height = lower ? l.low : l.rows;
+        double line = 0, pairs = 0, longest = 0;
+        for (int b = 0; b < n_seq; b++) {
+            if (n_new[b] <= 0 || pos0[b] < 0 || lane_of(n_new[b]) != k) continue;
+            const int64_t all = (int64_t)n_new[b] * group;
+            for (int64_t first = 0; first < all; first += height) {
+                const double units = (double)((pos0[b] + (std::min(all, first + height) - 1) / group) / l.unit + 1);
+                pairs += 1;
+                line += units + PAIR_COST;
+                longest = std::max(longest, units);
+            }
+        }
+        if (pairs == 0 || l.blocks == 0) return 0;
+        const double share = std::max((double)l.least, line * cfg_.n_kv_heads / l.blocks);
+        if (l.join > 0 && pairs * cfg_.n_kv_heads <= l.blocks && longest <= share + share / 8 + l.join) return l.whole_us[lower] + l.unit_us[lower] * longest;
+        return l.cut_us[lower] + l.unit_us[lower] * share;
+    }
     template <class F>
     void for_tiles(int, int pos0, int n_new, int group, F f) const {
-        const Lane& l = lanes_[lane_of(n_new)];
-        const int all = n_new * group;
-        for (int first = 0; first < all; first += l.rows) {
+        const int k = lane_of(n_new), all = n_new * group, height = height_[k];
+        const Lane& l = lanes_[k];
+        for (int first = 0; first < all; first += height) {
             Tile t = {};
             t.pos0 = pos0;
             t.first = first;
-            t.rows = std::min(l.rows, all - first);
+            t.rows = std::min(height, all - first);
             const int last = pos0 + (first + t.rows - 1) / group;  // the last position any of its rows sees
             t.units = last / l.unit + 1;
             f(t);
@@ -329,7 +355,7 @@ class Planner {
     Config cfg_ = {};
     Lane lanes_[2];
     Layout lay_ = {};
-    int few_ = 0, most_ = 0, now_ = 0, mark_ = 0;
+    int few_ = 0, most_ = 0, now_ = 0, mark_ = 0, height_[2] = {0, 0};
     std::vector<int> seen_, tmp_;
 };
 

@@ -14,13 +14,14 @@
 //                asynchronous 16-byte copies that write the swizzle themselves.  (All by the latter: 522 us instead of 494.)
 //   warps 4-11   half A, warps 12-19 half B: softmax, two threads a row, 64 positions and then 64 dimensions each: S out of tensor memory once for its maximum and once
 //                more for the weights, which take its columns' place as the next product's operand; then the product's result.
+// Steps that are sooner done in tiles of 128 rows have half A alone (Lane::low): QK_A(j + 1) goes before PV_A(j), and a unit takes 2.6 us instead of 3.4.
 // A region is written again by the third QK after its own; by then the PV that read it is complete: before each PV its issuer waits until the output of the PV
 // before has been read (one region for all of them), so that only the last PV issued can be under way.
 //
 // What bounds it: 1023 tokens of 64 heads on 8 behind 7001 positions, 457 to 465 us, 545 TFLOP/s, 1090 executed; the kernel itself 409 us, 1230 executed, where the card's
 // power allows 1400 (the clock falls to 1.55 GHz).  A unit of 128 positions takes 5600 cycles for products of 4096: a half's softmax (maximum 500, weights
 // 2000: 16 exponentials a cycle and SM, the wait for tensor memory), its product, the read of that and the next scores are one chain, longer than the other half's
-// products.  Few tokens: 511 of 32 heads 24.7 us, of which the queries' way to shared memory takes 5, the results' 3, the join of tiles on several blocks 5.
+// products.  Few tokens: 511 of 32 heads 21.2 us in tiles of 128 rows, of which the queries' way to shared memory takes 5, the results' 3 (in tiles of 256: 24.7).
 // Tried and taken back: a row a thread with twice the registers (chunk 453 us, but 139 for 96 us with 2047 tokens of 32 heads); half of the exponentials by a
 // polynomial (547 for 497); queries by eight lanes a row, in a function of their own or not (the softmax's registers came out worse: 480 to 580).
 //
@@ -100,7 +101,7 @@ template <int HS>
 struct Smem {
     static constexpr int BLOCK = 128 * 128, BLOCKS = HS / 64, Q = BLOCKS * BLOCK, TILE = BLOCKS * BLOCK;
     struct Rest {
-        unsigned long long bars[2 * PSLOTS + 10];
+        unsigned long long bars[2 * PSLOTS + 12];
         float max_s[4 * PR];  // what the two threads of a row tell one another
         unsigned int bad_s[2][2][4];
         uint32_t tmem_slot;
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
         return;
     }
     const uint32_t sb = smem_u32(smem), ring = sb + L::RING;
-    const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * PSLOTS, q_full = kv_empty + 8 * PSLOTS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
+    const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * PSLOTS, q_full = kv_empty + 8 * PSLOTS, s_full = q_full + 16, p_full = s_full + 32, o_full = p_full + 16,
                    o_free = o_full + 16, all_done = o_free + 8;
     const Cache& c = A.c;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hs = c.hs;
@@ -172,7 +173,8 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(q_full + 8 * i, 8);
-            mbar_init(s_full + 8 * i, 1);
+            mbar_init(s_full + 16 * i, 1);
+            mbar_init(s_full + 16 * i + 8, 1);
             mbar_init(p_full + 8 * i, 8);
             mbar_init(o_full + 8 * i, 1);
         }
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
         } else {
             // ---- products ----
             const uint32_t id_qk = idesc(128, false), id_pv = idesc(HS, true);
-            uint32_t n_q[2] = {0, 0}, n_s[2] = {0, 0}, n_pv = 0, qk = 0;  // phases: queries, scores of each half; outputs; scores of both
+            uint32_t n_q[2] = {0, 0}, n_qk[2] = {0, 0}, n_s[2] = {0, 0}, n_pv = 0, qk = 0;  // phases: queries, scores, weights of each half; outputs; scores of both
             uint32_t tile = 0;  // of the ring's sequence, at the part's first
             for_parts(s, c, [&](const Tile&, int, const Part& p) {
                 const int n[2] = {p.na, p.nb};
@@ -281,10 +283,11 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
 #pragma unroll
                             for (int k = 0; k < HS / 16; k++)
                                 umma_ss(d, desc_k(q + w * L::Q + (k / 4) * L::BLOCK + 32 * (k % 4)), desc_k(b + (k / 4) * L::BLOCK + 32 * (k % 4)), id_qk, w == 0 || k > 0);
-                        umma_commit(s_full + 8 * h);
+                        umma_commit(s_full + 16 * h + 8 * (n_qk[h] & 1));
                         if (h == 1 || j >= p.nb) umma_commit(kv_empty + 8 * (kt % PSLOTS));
                     }
                     __syncwarp();
+                    n_qk[h]++;
                     qk++;
                 };
                 auto do_pv = [&](int h, int j) {
@@ -308,7 +311,14 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
                     n_s[h]++;
                     n_pv++;
                 };
-                for (int j = 0; j <= p.n; j++) {
+                if (n[1] == 0) {  // half A alone: the next scores come before the product that waits for this one's weights
+                    do_qk(0, 0);
+                    for (int j = 0; j < n[0]; j++) {
+                        if (j + 1 < n[0]) do_qk(0, j + 1);
+                        do_pv(0, j);
+                    }
+                }
+                for (int j = 0; j <= p.n && n[1] > 0; j++) {
                     if (j < n[0]) do_qk(0, j);
                     if (j > 0 && j - 1 < n[1]) do_pv(1, j - 1);
                     if (j < n[1]) do_qk(1, j);
@@ -386,7 +396,7 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
             for (int j = 0; j < n; j++) {
                 const uint32_t reg = tmem + 128 * ((qk + j + (h == 0 ? min(j, p.nb) : min(j + 1, p.na))) % 3) + lanes + 64 * g;
                 const int p0 = (p.unit + j) * PU + 64 * g;
-                wait(s_full + 8 * h, n_s);
+                wait(s_full + 16 * h + 8 * (n_s & 1), n_s >> 1);
                 __syncwarp();
                 tc_after();
                 float resc;
@@ -568,6 +578,11 @@ int launch(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
 Lane paged_prompt_lane(int sms) {
     Lane l;
     l.rows = 2 * PR;
+    // us a call, tiles of 256 / of 128 rows: 32 heads, 256 tokens 18 / 15, 511 25 / 21, 1023 40 / 54; 64 heads on 8 behind 2000, 64 tokens
+    // 35 / 29, 511 82 / 111; 8 heads, 1023 tokens 33 / 26, 2047 43 / 47; 16 heads on 2 behind 1000, 256 tokens 29 / 25, 1023 46 / 52.
+    l.low = PR;
+    l.unit_us[0] = 3.4, l.whole_us[0] = 11, l.cut_us[0] = 25;  // (lines through these and longer ones)
+    l.unit_us[1] = 2.6, l.whole_us[1] = 12, l.cut_us[1] = 19;
     l.unit = PU;
     l.blocks = sms;
     l.fixed = 13;

@@ -27,6 +27,12 @@ Host* host_paged_create(const int* cfg, const int* lanes, int few, int most, cha
         l[i].blocks = lanes[5 * i + 2];
         l[i].least = lanes[5 * i + 3];
         l[i].join = lanes[5 * i + 4];
+        l[i].low = i ? l[i].rows / 2 : 0;
+        l[i].unit_us[0] = 3.4;
+        l[i].unit_us[1] = 2.6;
+        l[i].whole_us[0] = l[i].whole_us[1] = 12;
+        l[i].cut_us[0] = 25;
+        l[i].cut_us[1] = 19;
     }
     Host* h = new Host();
     h->c = c;
