@@ -78,7 +78,7 @@ int make_handle(slai_ctx* ctx, slai_paged* p) {
     const Lane few = paged_attention_lane(c.kv_dtype, c.head_size, group, sms);
     const int few_rows = f16 ? FEW_ROWS : std::max(few.rows, 4);
     Lane many;
-    if (fast && (long long)c.max_tokens * group > few_rows) many = f16 ? paged_prompt_lane(sms) : paged_attention_block_lane(sms);
+    if (fast && (long long)c.max_tokens * group > few_rows) many = f16 ? paged_prompt_lane(sms) : paged_prompt32_lane(sms);
     p->planner.init(c, few, many, few_rows, PERHAPS_ROWS);
     const size_t bytes = (size_t)p->planner.lay().total * 4;
     SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_plan, bytes));

@@ -61,13 +61,14 @@ __device__ __forceinline__ long long place_of(const Cache& c, int table, int p, 
 
 bool paged_attention_few(int kv_dtype, int hs);
 paged::Lane paged_attention_lane(int kv_dtype, int hs, int group, int sms);
-paged::Lane paged_attention_block_lane(int sms);  // f32 caches, many rows
 // One lane's kernel with `blocks` blocks, and the joins of at most `joins` pairs of at most `longest` results.
 int paged_attention_launch(slai_ctx* ctx, paged::AttnArgs& A, int kv_dtype, int lane, int blocks, int joins, int longest, bool pdl);
 
-// paged_prompt.cu
+// paged_prompt.cu, paged_prompt32.cu
 paged::Lane paged_prompt_lane(int sms);
 int paged_prompt_launch(slai_ctx* ctx, const paged::AttnArgs& A, int blocks, bool pdl);
+paged::Lane paged_prompt32_lane(int sms);
+int paged_prompt32_launch(slai_ctx* ctx, const paged::AttnArgs& A, int blocks, bool pdl);
 
 // paged_append.cu
 struct QkArgs {

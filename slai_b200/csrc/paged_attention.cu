@@ -796,218 +796,6 @@ int launch_few32_of(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
     return A.tile_rows <= 4 ? launch_few32<HS, 4, false>(ctx, A, blocks, pdl) : launch_few32<HS, 8, false>(ctx, A, blocks, pdl);
 }
 
-// ---- f32 caches, many rows -----------------------------------------------------------------------------------------------------------
-// 64 rows against 32 positions at a time, both in shared memory (keys and values in two buffers, asynchronous copies); f32 arithmetic, two at a time.  Thread (ty, tx) of
-// 16 x 16 has rows 4 ty .. + 3: scores of positions tx and tx + 16, and of the sums of values the dimensions 4 tx .. + 3 (and 64 + 4 tx .. + 3); a row's
-// sixteen threads are half a warp.  Shared memory and multipliers take about the same time.  (8 x 16 threads with 8 rows each read less, but a tile of 37 rows
-// was three warps, each alone on its scheduler: 5.5 us for 32 positions.)  31 TFLOP/s with 511 tokens behind 2000; 37 tokens behind 300, 32 heads: 25 us, latencies
-// of one tile and the join.
-constexpr int BT = 256, BR = 64, BP = 32, BN = 4;  // threads, rows, positions; rows a thread
-template <int HS>
-struct Block32 {
-    static constexpr int KS = HS + 4, Q = BR * KS, K = BP * KS, V = BP * HS, PS = BR + 4;
-    static constexpr int SMEM = 4 * (Q + 2 * (K + V) + BP * PS);
-};
-template <int HS>
-__global__ void __launch_bounds__(BT, 2) paged_attn_block32_kernel(const __grid_constant__ AttnArgs A) {
-    using L = Block32<HS>;
-    constexpr int CH = HS / 4, STEP = 32 / CH, KS = L::KS, DV = HS / 64;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    extern __shared__ __align__(128) unsigned char few_sm[];
-    float* q_s = reinterpret_cast<float*>(few_sm);   // [64][HS + 4]
-    float* kv_s = q_s + L::Q;                        // two of: keys [32][HS + 4], values [32][HS]
-    float* p_s = kv_s + 2 * (L::K + L::V);           // [32][64 + 4]: weights
-    const Cache& c = A.c;
-    const Start s = load_start(c.plan, A.starts_at, blockIdx.x);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tx = tid & 15, ty = tid >> 4, hs = c.hs, chunks = hs / 4, ch = lane % CH, rl = lane / CH;
-    const uint32_t kv_a = (uint32_t)__cvta_generic_to_shared(kv_s), q_a = (uint32_t)__cvta_generic_to_shared(q_s);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    Tile t = s.t;
-    int head = s.head, unit = s.unit, tile = s.tile;
-    for (int left = s.count; left > 0;) {
-        const int n = min(left, t.units - unit);
-        const bool whole = n == t.units;
-        const int lo = unit * A.unit, hi = min((unit + n) * A.unit, t.pos0 + (t.first + t.rows - 1) / c.group + 1);  // positions [lo, hi)
-        const int tiles = (hi - lo + BP - 1) / BP;
-        auto request = [&](int i) {  // warp w brings rows 4 w .. + 3
-            const int p0 = lo + i * BP;
-            const long long at = p0 + lane < hi ? 4 * place_of(c, t.table, p0 + lane, head) : -1;
-            const uint32_t kd = kv_a + 4 * (i & 1) * (L::K + L::V), vd = kd + 4 * L::K;
-#pragma unroll
-            for (int k = 0; k < 4; k += STEP) {
-                const int r = 4 * warp + k + rl;
-                const long long a = __shfl_sync(0xffffffffu, at, r);
-                const uint32_t bytes = a >= 0 && ch < chunks ? 16u : 0u;  // (none: zeros, nothing is read)
-                const long long src = bytes ? a + 16 * ch : 0;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(kd + 4 * (r * KS + 4 * ch)), "l"(__cvta_generic_to_global(c.keys + src)), "r"(bytes) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(vd + 4 * (r * HS + 4 * ch)), "l"(__cvta_generic_to_global(c.values + src)), "r"(bytes) : "memory");
-            }
-        };
-        // queries: all on their way at once
-        if (A.qvec) {
-#pragma unroll
-            for (int k = 0; k < BR / 8; k += STEP) {
-                const int r = 8 * k + 8 * rl + warp, pr = t.first + min(r, t.rows - 1), tok = pr / c.group;
-                const uint32_t bytes = r < t.rows && ch < chunks ? 16u : 0u;
-                const float* q = A.q + (bytes ? (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs + 4 * ch : 0);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_a + 4 * (r * KS + 4 * ch)), "l"(__cvta_generic_to_global(q)), "r"(bytes) : "memory");
-            }
-        } else {
-            for (int r = warp; r < BR; r += BT / 32) {
-                const int pr = t.first + min(r, t.rows - 1), tok = pr / c.group;
-                const float* q = A.q + (t.row0 + tok) * A.q_ld + (long long)(head * c.group + pr % c.group) * hs;
-#pragma unroll
-                for (int d = lane; d < HS; d += 32) q_s[r * KS + d] = r < t.rows && d < hs ? __ldcg(q + d) : 0.f;
-            }
-        }
-        request(0);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        const float by = A.scale * LOG2E;  // scores as powers of two's exponents
-        const bool on = 8 * warp < t.rows;  // this warp has rows
-        int vis[BN];  // last position a row sees
-#pragma unroll
-        for (int r = 0; r < BN; r++) vis[r] = BN * ty + r < t.rows ? t.pos0 + (t.first + BN * ty + r) / c.group : 0x7fffffff;
-        f32x2 acc[BN][2 * DV];
-        float m[BN], l[BN];
-#pragma unroll
-        for (int r = 0; r < BN; r++) {
-#pragma unroll
-            for (int d = 0; d < 2 * DV; d++) acc[r][d] = 0;
-            m[r] = -INFINITY;
-            l[r] = 0.f;
-        }
-        for (int i = 0; i < tiles; i++) {
-            if (i + 1 < tiles) request(i + 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            __syncthreads();
-            const float* ks = kv_s + (i & 1) * (L::K + L::V);
-            const float* vs = ks + L::K;
-            const int p0 = lo + i * BP;
-            if (on) {
-                f32x2 sc[BN][2];
-#pragma unroll
-                for (int r = 0; r < BN; r++) sc[r][0] = sc[r][1] = 0;
-#pragma unroll 4
-                for (int d = 0; d < HS; d += 4) {
-                    const ulonglong2 k0 = *reinterpret_cast<const ulonglong2*>(ks + tx * KS + d), k1 = *reinterpret_cast<const ulonglong2*>(ks + (tx + 16) * KS + d);
-#pragma unroll
-                    for (int r = 0; r < BN; r++) {
-                        const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q_s + (BN * ty + r) * KS + d);
-                        sc[r][0] = fma2(q2.x, k0.x, fma2(q2.y, k0.y, sc[r][0]));
-                        sc[r][1] = fma2(q2.x, k1.x, fma2(q2.y, k1.y, sc[r][1]));
-                    }
-                }
-                float w[BN][2];
-#pragma unroll
-                for (int r = 0; r < BN; r++) {
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const float2 x = unpack2(sc[r][u]);
-                        // (rows behind the tile's last see the positions that are not there too: nothing of theirs is kept)
-                        w[r][u] = p0 + tx + 16 * u > min(vis[r], hi - 1) ? -INFINITY : (x.x + x.y) * by;
-                    }
-                    float mt = fmaxf(w[r][0], w[r][1]);
-#pragma unroll
-                    for (int o = 8; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-                    const float m_new = fmaxf(m[r], mt), base = m_new == -INFINITY ? 0.f : m_new, resc = ex2(m[r] - base);
-                    m[r] = m_new;
-                    w[r][0] = ex2(w[r][0] - base);
-                    w[r][1] = ex2(w[r][1] - base);
-                    l[r] = l[r] * resc + (w[r][0] + w[r][1]);  // (this thread's positions only)
-                    const f32x2 f = pack2(resc, resc);
-#pragma unroll
-                    for (int d = 0; d < 2 * DV; d++) acc[r][d] = mul2(acc[r][d], f);
-                }
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int r = 0; r < BN; r += 4)
-                        *reinterpret_cast<float4*>(p_s + (tx + 16 * u) * L::PS + BN * ty + r) = make_float4(w[r][u], w[r + 1][u], w[r + 2][u], w[r + 3][u]);
-                __syncwarp();
-#pragma unroll 2
-                for (int j = 0; j < BP; j++) {
-                    ulonglong2 v2[DV];
-#pragma unroll
-                    for (int d = 0; d < DV; d++) v2[d] = *reinterpret_cast<const ulonglong2*>(vs + j * HS + 64 * d + 4 * tx);
-#pragma unroll
-                    for (int r0 = 0; r0 < BN; r0 += 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(p_s + j * L::PS + BN * ty + r0);
-                        const float xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const f32x2 f = pack2(xs[r], xs[r]);
-#pragma unroll
-                            for (int d = 0; d < DV; d++) {
-                                acc[r0 + r][2 * d] = fma2(f, v2[d].x, acc[r0 + r][2 * d]);
-                                acc[r0 + r][2 * d + 1] = fma2(f, v2[d].y, acc[r0 + r][2 * d + 1]);
-                            }
-                        }
-                    }
-                }
-            }
-            __syncthreads();  // the buffer is requested again next round
-        }
-        const size_t slot = ((size_t)s.me * 2 + (unit == 0)) * A.tile_rows;
-        if (on) {
-            unsigned int bad = 0;  // of this thread's rows
-#pragma unroll
-            for (int r = 0; r < BN; r++) {
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
-                const int row = BN * ty + r;
-                const bool there = row < t.rows;
-                const int pr = t.first + min(row, t.rows - 1), tok = pr / c.group;
-                float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs : A.part + (slot + min(row, t.rows - 1)) * hs;
-                const float f = whole ? 1.f / l[r] : 1.f;
-                float sum = l[r];
-#pragma unroll
-                for (int d = 0; d < DV; d++) {
-                    const float2 a = unpack2(acc[r][2 * d]), b = unpack2(acc[r][2 * d + 1]);
-                    sum += (a.x + a.y) + (b.x + b.y);
-                    const int e = 64 * d + 4 * tx;
-                    if (there && e < hs) {
-                        if (!whole || A.qvec) {
-                            *reinterpret_cast<float4*>(o + e) = make_float4(a.x * f, a.y * f, b.x * f, b.y * f);
-                        } else {
-                            o[e] = a.x * f; o[e + 1] = a.y * f; o[e + 2] = b.x * f; o[e + 3] = b.y * f;
-                        }
-                    }
-                }
-                if (there && !whole && tx == 0) *reinterpret_cast<float2*>(A.part_ml + (slot + row) * 2) = make_float2(m[r], l[r]);
-                if (there && !(fabsf(sum) < INFINITY)) bad |= 1u << r;
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
-            const unsigned int both = __shfl_sync(0xffffffffu, bad, 0) | __shfl_sync(0xffffffffu, bad, 16) << BN;  // of the warp's rows
-            for (int r = 0; r < 2 * BN && both; r++)
-                if (both >> r & 1) {
-                    const int row = 2 * BN * warp + r, pr = t.first + row, tok = pr / c.group;
-                    float* o = whole ? A.out + (t.row0 + tok) * A.out_ld + (long long)(head * c.group + pr % c.group) * hs : A.part + (slot + row) * hs;
-                    __syncwarp();
-                    row_again<float>(A, t, head, row, lo, hi, o, whole ? nullptr : A.part_ml + (slot + row) * 2);
-                }
-        }
-        left -= n + PAIR_COST;
-        unit = 0;
-        if (left > 0 && ++head == c.n_kv) {
-            head = 0;
-            t = load_tile(c.plan, s.tiles, ++tile);
-        }
-    }
-}
-
-template <int HS>
-int launch_block32(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
-    auto kern = paged_attn_block32_kernel<HS>;
-    static PerDeviceOnce attr;
-    if (attr.need(ctx->device)) {
-        SLAI_CHECK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Block32<HS>::SMEM));
-        attr.set(ctx->device);
-    }
-    return launch_dependent(ctx, kern, dim3((unsigned)blocks), BT, Block32<HS>::SMEM, pdl, A);
-}
-
 }  // namespace
 
 // Whether a handle's few-row launches can take the kernels above (with rows that can be read in 16-byte pieces).
@@ -1030,20 +818,10 @@ Lane paged_attention_lane(int kv_dtype, int hs, int group, int sms) {
     }
     return l;
 }
-Lane paged_attention_block_lane(int sms) {
-    Lane l;
-    l.rows = BR;
-    l.unit = BP;
-    l.least = 1;
-    l.blocks = 2 * sms;
-    l.fixed = 20;
-    l.each = 0.02;
-    return l;
-}
 static int launch_lane(slai_ctx* ctx, const AttnArgs& A, int kv_dtype, int lane, int blocks, bool pdl) {
     if (lane == 1 && A.vec) {
         if (kv_dtype == SLAI_KV_F16) return paged_prompt_launch(ctx, A, blocks, pdl);
-        return A.c.hs <= 64 ? launch_block32<64>(ctx, A, blocks, pdl) : launch_block32<128>(ctx, A, blocks, pdl);
+        return paged_prompt32_launch(ctx, A, blocks, pdl);
     }
     if (lane == 0 && A.vec && paged_attention_few(kv_dtype, A.c.hs)) {
         if (kv_dtype == SLAI_KV_F32) return A.c.hs <= 64 ? launch_few32_of<64>(ctx, A, blocks, pdl) : launch_few32_of<128>(ctx, A, blocks, pdl);
