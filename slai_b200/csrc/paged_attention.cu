@@ -811,7 +811,7 @@ Lane paged_attention_lane(int kv_dtype, int hs, int group, int sms) {
         // 100 10.4 / 5.3, 515 20.6 / 16.9, 1000 31.4 / 27.6; 64 heads on 8 at 300 9.9 / 8.6, 515 11.2 / 12.5.
         l.join = kv_dtype == SLAI_KV_F32 && l.rows == FR ? 1 : 5;  // (a unit of eight rows in f32 takes as long as the join: a token of 64 heads on 8 at 300 18.8 / 13.6 us if cut only at 5 / from 1)
         l.fixed = 5;
-        l.each = kv_dtype == SLAI_KV_F16 ? 0.0054 : 0.0126;
+        l.each = kv_dtype == SLAI_KV_F16 ? 0.0054 : l.rows == 1 ? 0.004 : l.rows == FR ? 0.018 : 0.0126;
     } else {
         l.rows = GR;
         l.blocks = 4 * sms;

@@ -8,11 +8,11 @@
 //   warp 0       issues the products: QK(j + 1), then PV(j).  Queries are in tensor memory (2 x HS columns), scores, whose place the weights take, too (two stages of 64
 //                columns), and one output.
 //   warps 4-7    softmax, a thread a row: queries into tensor memory, scores out of it, weights into it, outputs out of it, results.
-//   warps 8-15   keys and values: out of the pages a step ahead into registers, in two parts each into shared memory, rows of 128 bytes in the tensor core's swizzle.
+//   warps 8-23   keys and values, two sets of eight in turn: out of the pages two steps ahead into registers, in two parts each into shared memory, rows of 128 bytes in the tensor core's swizzle.
 //                Values lie there with a row a dimension: a thread reads four positions of one dimension, a warp's threads next to each other.
 //
 // Barriers: a stage of scores, weights, keys and values has a unit's number's parity; a unit's QK and PV being complete is what frees them.
-// 1023 tokens of 32 heads behind 2000 positions 259 us, 162 TFLOP/s, 487 executed; 37 tokens behind 300 21 us.  (f32 arithmetic of 64 rows and 32 positions in shared memory: 31
+// 1023 tokens of 32 heads behind 2000 positions 212 us, 198 TFLOP/s, 594 executed; 37 tokens behind 300 19 us.  (f32 arithmetic of 64 rows and 32 positions in shared memory: 31
 // TFLOP/s, 25 us.)
 // Every wait is bounded (common.cuh, bounded_wait).
 #include <type_traits>
@@ -23,8 +23,8 @@ using namespace paged;
 
 namespace {
 
-constexpr int XT = 512, XR = 128, XP = 32, XU = 32;  // threads, rows of a tile, positions at a time, positions of a unit of the plan
-constexpr int LOADERS = 8;                           // warps
+constexpr int XT = 768, XR = 128, XP = 32, XU = 64;  // threads, rows of a tile, positions at a time, positions of a unit of the plan
+constexpr int LOADERS = 8;                           // warps of either set
 
 // kind::tf32: f32 results (bits 4-5 = 1), tf32 operands (bits 7-9 and 10-12 = 2), N / 8 in bits 17-22, M / 16 in bits 24-28
 __device__ __forceinline__ uint32_t idesc(int n) { return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(XR >> 4) << 24); }
@@ -32,15 +32,11 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
                  : "memory");
 }
-// v = hi + lo, 22 bits
-__device__ __forceinline__ uint32_t tf32(float v) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
-    return r;
-}
+// v = hi + lo: the value rounded to tf32's 11 bits, and the rest, of which the tensor core takes 11 bits.  An infinite value leaves NaN in lo, a NaN one of hi's.
+// (By cvt.rna.tf32, two a value: 244 us instead of 212 for 1023 tokens of 32 heads behind 2000.)
 __device__ __forceinline__ void split(float v, uint32_t& hi, uint32_t& lo) {
-    hi = tf32(v);
-    lo = tf32(v - __uint_as_float(hi));
+    hi = (__float_as_uint(v) + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(v - __uint_as_float(hi));
 }
 
 // Shared memory: keys and values of two units, [unit][keys, values][high, low][HS * 128 bytes]; a row of the tile in f32 (queries on their way in, results out).
@@ -122,9 +118,9 @@ __global__ void __launch_bounds__(XT, 1) paged_attn_prompt32_kernel(const __grid
     constexpr int CH = HS / 4, STEP = 32 / CH;  // 16-byte pieces of a row, rows a pass of a warp covers
     const int ch = lane % CH, rl = lane / CH, chunks = hs / 4;
 
-    // Registers: 4 x 32 x 72 + 4 x 32 x 208 + 8 x 32 x 104 = 62464 of the launch's 512 x 128.
+    // Registers: 4 x 32 x 40 + 4 x 32 x 208 + 16 x 32 x 56 = 60416 of the launch's 768 x 80.
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
             // ---- products ----
             const uint32_t id_qk = idesc(XP), id_pv = idesc(HS);
@@ -174,10 +170,12 @@ __global__ void __launch_bounds__(XT, 1) paged_attn_prompt32_kernel(const __grid
             __syncwarp();
         }
     } else if (warp >= 8) {
-        // ---- keys and values: this warp's positions are 4 w .. + 3 of 32 ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        const int w = warp - 8;
-        uint32_t u = 0;
+        // ---- keys and values of every second unit: this warp's positions are 4 w .. + 3 of 32 ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        const int w = (warp - 8) & 7;
+        const uint32_t g = (warp - 8) >> 3;
+        unsigned char* slot = smem + 2 * g * L::SLOT;
+        uint32_t u = 0;  // the part's first unit
         for_parts(s, c, [&](const Tile& t, int head, const Part& p) {
             auto place = [&](int j) {  // lane i: of position i % 4, -1 behind the last
                 const int at = p.lo + XP * j + 4 * w + (lane & 3);
@@ -209,14 +207,16 @@ __global__ void __launch_bounds__(XT, 1) paged_attn_prompt32_kernel(const __grid
                 *reinterpret_cast<uint4*>(to) = hi;
                 *reinterpret_cast<uint4*>(to + L::PART) = lo;
             };
-            long long at = place(0);
-            load_k(at);
-            load_v(at);
-            at = p.n > 1 ? place(1) : -1;
-            for (int j = 0; j < p.n; j++, u++) {
-                const uint32_t g = u & 1;
-                unsigned char* slot = smem + 2 * g * L::SLOT;
-                if (u >= 2) wait(qk_done + 8 * g, (u >> 1) - 1);
+            int j = (u ^ g) & 1;
+            if (j < p.n) {
+                const long long at = place(j);
+                load_k(at);
+                load_v(at);
+            }
+            for (; j < p.n; j += 2) {
+                const uint32_t round = (u + j) >> 1;
+                const long long at = j + 2 < p.n ? place(j + 2) : -1;
+                if (round > 0) wait(qk_done + 8 * g, round - 1);
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 4 / STEP; i++) {
@@ -226,17 +226,19 @@ __global__ void __launch_bounds__(XT, 1) paged_attn_prompt32_kernel(const __grid
                 fence_async();
                 __syncwarp();
                 if (lane == 0 && limit) mbar_arrive(k_full + 8 * g);
-                if (j + 1 < p.n) load_k(at);
-                if (u >= 2) wait(pv_done + 8 * g, (u >> 1) - 1);
+                if (round > 0) wait(pv_done + 8 * g, round - 1);
                 __syncwarp();
 #pragma unroll
                 for (int d = 0; d < HS / 32; d++) put(slot + L::SLOT + (32 * d + lane) * 128 + ((w ^ (lane & 7)) << 4), vr[d][0], vr[d][1], vr[d][2], vr[d][3]);
                 fence_async();
                 __syncwarp();
                 if (lane == 0 && limit) mbar_arrive(v_full + 8 * g);
-                if (j + 1 < p.n) load_v(at);
-                at = j + 2 < p.n ? place(j + 2) : -1;
+                if (j + 2 < p.n) {  // (not before: the fence waits for loads)
+                    load_k(at);
+                    load_v(at);
+                }
             }
+            u += p.n;
         });
     } else {
         // ---- softmax: a thread a row ----
@@ -421,10 +423,12 @@ Lane paged_prompt32_lane(int sms) {
     l.rows = XR;
     l.unit = XU;
     l.blocks = sms;
-    l.least = 1;
-    l.fixed = 14;
-    l.each = 0.0075;
-    l.join = 5;
+    // us a call, units of 64, two at least / of 32, one / of 32, two: 16 heads on 2 behind 2000, 37 tokens 24.3 / 34.2 / 34.0; 32 heads behind 300, 128 tokens
+    // 22.9 / 28.3 / 28.3, 37 tokens 20.9 / 21.0 / 21.0 (three of 64: 26.0).
+    l.least = 2;
+    l.fixed = 15;
+    l.each = 0.007;
+    l.join = 2;  // 32 heads behind 300, 16 tokens: five units whole 23.9 us, cut 19.6
     return l;
 }
 
