@@ -14,6 +14,10 @@
 // Barriers: a stage of scores, weights, keys and values has a unit's number's parity; a unit's QK and PV being complete is what frees them.
 // 1023 tokens of 32 heads behind 2000 positions 212 us, 198 TFLOP/s, 594 executed; 37 tokens behind 300 19 us.  (f32 arithmetic of 64 rows and 32 positions in shared memory: 31
 // TFLOP/s, 25 us.)
+// What bounds it: 32 positions take 2150 cycles, about as long as the products (1500 at the full rate, 32 columns of scores do not reach it) and, in one chain beside them, scores, weights
+// and outputs through the four warps; without the loads 187 us, with a third of the products 181, with neither nor the splits 155.  Tried and taken back: eight more
+// warps for the outputs (251 us: their barriers are one more hop in the chain); one set of loading warps (257 us, and with twice the steps ahead no better: the fence before
+// the tensor core's reads waits for loads).
 // Every wait is bounded (common.cuh, bounded_wait).
 #include <type_traits>
 
@@ -428,7 +432,7 @@ Lane paged_prompt32_lane(int sms) {
     l.least = 2;
     l.fixed = 15;
     l.each = 0.007;
-    l.join = 2;  // 32 heads behind 300, 16 tokens: five units whole 23.9 us, cut 19.6
+    l.join = 2;  // 32 heads behind 300, 16 tokens: five units whole 20.6 us, cut 17.2
     return l;
 }
 

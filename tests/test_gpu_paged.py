@@ -293,6 +293,29 @@ def test_sizes_of_queries(ctx, backend, size, dtype):
     attend(ctx, P, [189, 260], [1, 140], q=q)
 
 
+@pytest.mark.parametrize("keys, values", [(1e-25, 1e30), (1e25, 1e-30), (1e-33, 1e-33), (1e30, 3e35)])
+@pytest.mark.parametrize("hs, page", [(128, 16), (72, 40)])
+def test_sizes_of_f32_keys_and_values(ctx, backend, keys, values, hs, page):
+    """Far beyond halves; the queries make up for the keys, so that scores are the usual ones."""
+    P = Pages(backend, 4, 2, hs, page, [150, 400, 61], F32, seed=12)
+    P.host[0] *= np.float32(keys)
+    P.host[1] *= np.float32(values)
+    P.upload()
+    q = (P.rng.standard_normal((37 + 140 + 3, 4, hs)) * 2 / keys).astype(np.float32)
+    attend(ctx, P, [113, 260, 58], [37, 140, 3], q=q)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hq, hk", [(16, 16), (24, 8)])
+def test_many_short_chunks(ctx, backend, hq, hk, dtype):
+    """Several pairs to a block, most of them of one unit or two."""
+    rng = np.random.default_rng(13)
+    n_new = [int(x) for x in rng.integers(17, 61, 40)]
+    pos0 = [int(x) for x in rng.integers(0, 90, 40) * (rng.random(40) < 0.5)]
+    n_new[7], n_new[20], n_new[21] = 140, 1, 0
+    attend(ctx, Pages(backend, hq, hk, 128, 16, [p + n for p, n in zip(pos0, n_new)], dtype, "pos", seed=13), pos0, n_new)
+
+
 def test_keys_far_from_zero_and_scale(ctx, backend):
     P = Pages(backend, 4, 2, 128, 16, [300, 150], F16, seed=7)
     for b, n in ((0, 300), (1, 150)):
