@@ -166,14 +166,17 @@ class Planner {
             }
         } back = {now_, before, false};
         now_ = few_;
-        if (most_ > few_ && n_seq > 0) {
+        long long tokens = 0;
+        for (int b = 0; b < n_seq; b++) tokens += std::max(0, n_new[b]);
+        const bool fits = tokens <= cfg_.max_tokens;  // (else it is refused below)
+        if (most_ > few_ && fits) {
             double us[2];
             for (int way = 0; way < 2; way++) us[way] = cost(n_seq, pos0, n_new, group, way ? most_ : few_);
             if (us[1] < us[0]) now_ = most_;
         }
         for (int k = 0; k < 2; k++) {
             height_[k] = lanes_[k].rows;
-            if (lanes_[k].low && takes(k, 1, n_seq, pos0, n_new, group) < takes(k, 0, n_seq, pos0, n_new, group)) height_[k] = lanes_[k].low;
+            if (lanes_[k].low && fits && takes(k, 1, n_seq, pos0, n_new, group) < takes(k, 0, n_seq, pos0, n_new, group)) height_[k] = lanes_[k].low;
         }
         long long rows = 0, entries = 0, line[2] = {0, 0};
         for (int b = 0; b < n_seq; b++) {

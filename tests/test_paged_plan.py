@@ -2,6 +2,7 @@
 import ctypes as C
 import os
 import subprocess
+import time
 
 import numpy as np
 import pytest
@@ -90,6 +91,14 @@ def test_steps_that_are_refused(lib):
     narrow = Plan(lib, table=3)
     assert "max_table" in narrow([20, 16], [1, 1], table([[3, 9], [4, 5]]))
     assert narrow([20, 0], [1, 1], table([[3, 9], [4]])) == ""
+
+
+def test_far_too_many_tokens_are_refused_at_once(lib):
+    """Their tiles, billions, are not counted first."""
+    p = Plan(lib, heads=64, kv=1, most=128)
+    begin = time.perf_counter()
+    assert "too narrow" in p([0] * 8, [2**31 - 2000] * 8, table([[0]] * 8))
+    assert time.perf_counter() - begin < 1
 
 
 def test_pages_that_are_only_read_may_be_shared(lib):
