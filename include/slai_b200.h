@@ -275,7 +275,7 @@ int slai_kv_append(slai_ctx* ctx, void* d_key_cache, void* d_value_cache, int kv
  * 0 .. h_pos0 + h_n_new - 1 in order.  The step's rows (of q, k, v and of the results) are the new tokens, sequence after sequence.  Lengths and tables are
  * checked on the host (SLAI_ERR_SHAPE; the step before stays in force): capacity, page numbers, and that a page which gets new tokens is used once (pages that
  * are only read may be shared).  The call copies the tables and returns; it serves every layer until the next step.  It cannot be recorded: a recorded
- * append or attention (slai_pass_*) reads the step that is current when it runs, up to the handle's capacity.
+ * append or attention (slai_pass_*) reads the step that is current when it runs, so its buffers hold max_tokens rows.
  * One handle is used on one context's stream.  Destroy handles before their context. */
 typedef struct slai_paged_config {
     int32_t n_q_heads, n_kv_heads, head_size; /* n_kv_heads divides n_q_heads; head_size 1 .. 256 */
@@ -312,7 +312,8 @@ int slai_qk_norm_rope(slai_ctx* ctx, const slai_qk_params* params, int n_tokens,
 int slai_paged_append(slai_paged* p, const slai_paged_layer* layer, const slai_qk_params* params, const float* d_q, const float* d_k, const float* d_v,
                       float* d_q_out);
 /* Causal attention (ops/batched_multiquery_attention.rs:32-156) of the step's tokens: token at position t attends to positions 0 .. t of its sequence, which
- * are in the pages by then.  Rows of q and out: n_q_heads * head_size floats, q_ld / out_ld apart (0 = packed).  scale 0: 1 / sqrt(head_size).  Sums,
+ * are in the pages by then.  Rows of q and out: n_q_heads * head_size floats, q_ld / out_ld apart (0 = packed); no element of
+ * out is one of q's.  scale 0: 1 / sqrt(head_size).  Sums,
  * weights and results are f32; f16 keys and values take part as they are cached.  Results do not depend on timing; their last bits may depend on what else is in the step. */
 int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, const float* d_q, int64_t q_ld, float scale, float* d_out, int64_t out_ld);
 

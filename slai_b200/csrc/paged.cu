@@ -258,6 +258,7 @@ SLAI_API int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, 
     SLAI_REQUIRE(ctx, A.q_ld >= row && A.out_ld >= row, SLAI_ERR_SHAPE, "paged attention: rows of %lld and %lld floats are shorter than %lld", (long long)A.q_ld,
                  (long long)A.out_ld, (long long)row);
     SLAI_REQUIRE(ctx, isfinite(scale), SLAI_ERR_INVALID_ARG, "paged attention: scale %g", (double)scale);
+    SLAI_REQUIRE(ctx, d_q != d_out, SLAI_ERR_INVALID_ARG, "paged attention: queries are read while results are written, out cannot be q");
     A.scale = scale == 0.f ? (float)(1.0 / sqrt((double)c.head_size)) : scale;
     A.q = d_q;
     A.out = d_out;

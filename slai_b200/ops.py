@@ -300,6 +300,8 @@ class PagedLayer:
     def __init__(self, keys, values, page_stride: int, head_stride: int, pos_stride: int):
         self.keys, self.values = keys, values  # held: the pages outlive the layer
         self.strides = (page_stride, head_stride, pos_stride)
+        self.elements = min(len(keys), len(values))
+        self.nbytes = min(getattr(keys, "nbytes", None) or 4 * len(keys), getattr(values, "nbytes", None) or 4 * len(values))
         self.c = _lib.PagedLayer(keys.ptr, values.ptr, page_stride, head_stride, pos_stride)
         self.at = C.addressof(self.c)
 
@@ -313,6 +315,7 @@ class PagedKv:
         self.backend = backend
         self.n_q_heads, self.n_kv_heads, self.head_size, self.page_size, self.n_pages = n_q_heads, n_kv_heads, head_size, page_size, n_pages
         self.kv_dtype, self.max_tokens, self.width = kv_dtype, max_tokens, n_q_heads * head_size
+        self.kv_bytes = 2 if kv_dtype == KV_F16 else 4
         self.rows = None  # of the current step
         cfg = _lib.PagedConfig(n_q_heads, n_kv_heads, head_size, page_size, n_pages, kv_dtype, max_seqs, max_tokens, max_table or max(1, n_pages))
         h = C.c_void_p()
@@ -333,8 +336,12 @@ class PagedKv:
     def check_layer(self, layer: PagedLayer):
         page, head, pos = layer.strides
         need = (self.n_pages - 1) * page + (self.n_kv_heads - 1) * head + (self.page_size - 1) * pos + self.head_size
-        if len(layer.keys) < need or len(layer.values) < need:
-            raise SlaiError(_lib.ERR_SHAPE, f"paged: pages of {len(layer.keys)} and {len(layer.values)} elements, {need} needed")
+        if layer.elements < need or layer.nbytes < self.kv_bytes * need:
+            raise SlaiError(_lib.ERR_SHAPE, f"paged: pages of {layer.elements} elements in {layer.nbytes} bytes, {need} elements of {self.kv_bytes} needed")
+
+    def rows_in_use(self):
+        """Rows that a call's buffers hold: the step's, or, for a call that is recorded and replayed for other steps, the most that a step can have."""
+        return self.max_tokens if getattr(self.backend, "_recording", False) else self.rows
 
     def __del__(self):
         try:
@@ -488,7 +495,7 @@ class LlmContext:
     def paged_append(self, paged: PagedKv, layer: PagedLayer, how: QkNormRope, q, k, v, q_out):
         """The same for the rows of the current step; keys and values go into their pages, q to q_out."""
         paged.check_layer(layer)
-        n = paged.rows
+        n = paged.rows_in_use()
         if n:
             m, w, k_w = n - 1, how.q_width, how.k_width
             if w:
@@ -508,7 +515,7 @@ class LlmContext:
     def paged_attention(self, paged: PagedKv, layer: PagedLayer, q, out, scale: float = 0.0, q_ld: int = 0, out_ld: int = 0):
         """Causal attention of the step's tokens to what their sequences hold (scale 0: 1 / sqrt(head_size))."""
         paged.check_layer(layer)
-        n, width = paged.rows, paged.width
+        n, width = paged.rows_in_use(), paged.width
         if n:
             if len(q) < (n - 1) * (q_ld or width) + width:
                 _refuse_rows("paged_attention: q", q, n, width, q_ld)

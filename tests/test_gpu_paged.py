@@ -533,9 +533,14 @@ def test_refusals(ctx, backend):
     refused(S, "shorter", ctx.qk_norm_rope, QkNormRope(64, 4, 2, 1, q_ld=64), backend.zeros(1, np.int32), buf, buf, buf, buf)
     refused(S, "not the cache's", ctx.paged_append, P.kv, P.layer, QkNormRope(128, 4, 2), buf, buf, buf, buf)
     refused(S, "not the cache's", ctx.paged_append, P.kv, P.layer, QkNormRope(64, 4, 4), buf, buf, buf, buf)
+    refused(I, "out cannot be q", ctx.paged_attention, P.kv, P.layer, buf, buf)
+    refused(S, "elements of 4", ctx.paged_attention, Pages(backend, 4, 2, 64, 16, [40, 20], F32).kv, P.layer, buf, buf)  # f16 pages for an f32 cache
+    two, out = backend.zeros(4 * 64 * 2), backend.zeros(4 * 64 * 60)
     with backend.record() as rec:
         refused(I, "recorded", P.kv.step, [39, 19], [1, 1], P.tables)
         refused(I, "recorded", ctx.qk_norm_rope, QkNormRope(64, 4, 2, 1, 12345.0), backend.pos if hasattr(backend, "pos") else buf.view(0, 1), buf, buf, buf, buf)
-        ctx.paged_attention(P.kv, P.layer, buf, buf.view(4 * 64 * 4, 4 * 64 * 4))
+        refused(S, "floats for 60 rows", ctx.paged_attention, P.kv, P.layer, buf, two)  # (other steps come)
+        refused(S, "floats for 60 rows", ctx.paged_append, P.kv, P.layer, QkNormRope(64, 4, 2, None), buf, two, two, buf)
+        ctx.paged_attention(P.kv, P.layer, buf, out)
     rec.close()
     attend(ctx, P, [39, 19], [1, 1])  # and goes on
