@@ -18,11 +18,11 @@
 // A region is written again by the third QK after its own; by then the PV that read it is complete: before each PV its issuer waits until the output of the PV
 // before has been read (one region for all of them), so that only the last PV issued can be under way.
 //
-// What bounds it: 1023 tokens of 64 heads on 8 behind 7001 positions, 457 to 465 us, 545 TFLOP/s, 1090 executed; the kernel itself 409 us, 1230 executed, where the card's
-// power allows 1400 (the clock falls to 1.55 GHz).  A unit of 128 positions takes 5600 cycles for products of 4096: a half's softmax (maximum 500, weights
+// What bounds it: 1023 tokens of 64 heads on 8 behind 7001 positions, 445 us, 566 TFLOP/s, 1130 executed; the kernel itself 396 us, 1270 executed, where the card's
+// power allows 1400 (the clock falls to 1.55 GHz).  A unit of 128 positions takes 5400 cycles for products of 4096: a half's softmax (maximum 500, weights
 // 2000: 16 exponentials a cycle and SM, the wait for tensor memory), its product, the read of that and the next scores are one chain, longer than the other half's
-// products.  Few tokens: 511 of 32 heads 21.2 us in tiles of 128 rows, of which the queries' way to shared memory takes 5, the results' 3 (in tiles of 256: 24.7).
-// Tried and taken back: a row a thread with twice the registers (chunk 453 us, but 139 for 96 us with 2047 tokens of 32 heads); half of the exponentials by a
+// products.  Few tokens: 511 of 32 heads 20.6 us in tiles of 128 rows, of which the queries' way to shared memory takes 5, the results' 3 (in tiles of 256: 24.7).
+// Descriptors in uniform registers: 464 -> 445 us.  Tried and taken back: a row a thread with twice the registers (chunk 453 us, but 139 for 96 us with 2047 tokens of 32 heads); half of the exponentials by a
 // polynomial (547 for 497); queries by eight lanes a row, in a function of their own or not (the softmax's registers came out worse: 480 to 580).
 //
 // Every wait is bounded (common.cuh, bounded_wait).
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = tmem_slot, out_cols = tmem + 3 * 128;
+    const uint32_t tmem = uniform(tmem_slot), out_cols = tmem + 3 * 128;
     const Start s = load_start(c.plan, A.starts_at, blockIdx.x);  // (there before any kernel of its step starts)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -241,15 +241,16 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
                     }
                     const uint32_t kt = tile + 2 * j;
                     kv_wait(kt);
+                    const uint32_t slot = uniform(kt % PSLOTS), d = uniform(region(place_of_s(h, j)));
                     tc_after();
                     __syncwarp();
                     if (elect_one() && limit) {
-                        const uint32_t d = region(place_of_s(h, j)), q = sb + h * 2 * L::Q, b = ring + (kt % PSLOTS) * L::TILE;
+                        const uint64_t queries = desc_k(sb + h * 2 * L::Q), keys = desc_k(ring + slot * L::TILE);
 #pragma unroll
                         for (int w = 1; w >= 0; w--)  // the low parts first
 #pragma unroll
                             for (int k = 0; k < HS / 16; k++)
-                                umma_ss(d, desc_k(q + w * L::Q + (k / 4) * L::BLOCK + 32 * (k % 4)), desc_k(b + (k / 4) * L::BLOCK + 32 * (k % 4)), id_qk, w == 0 || k > 0);
+                                umma_ss(d, queries + (w * L::Q + (k / 4) * L::BLOCK + 32 * (k % 4)) / 16, keys + ((k / 4) * L::BLOCK + 32 * (k % 4)) / 16, id_qk, w == 0 || k > 0);
                         umma_commit(s_full + 16 * h + 8 * (n_qk[h] & 1));
                         if (h == 1 || j >= p.nb) umma_commit(kv_empty + 8 * (kt % PSLOTS));
                     }
@@ -262,15 +263,16 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
                     wait(p_full + 8 * h, first_s[h] + j);
                     kv_wait(vt);
                     if (n_pv > 0) wait(o_free, n_pv - 1);
+                    const uint32_t slot = uniform(vt % PSLOTS), a = uniform(region(place_of_s(h, j)));
                     tc_after();
                     __syncwarp();
                     if (elect_one() && limit) {
-                        const uint32_t a = region(place_of_s(h, j)), b = ring + (vt % PSLOTS) * L::TILE;
+                        const uint64_t values = desc_mn(ring + slot * L::TILE, L::BLOCK);
 #pragma unroll
                         for (int w = 1; w >= 0; w--)
 #pragma unroll
                             for (int k = 0; k < PU / 16; k++)
-                                umma_ts(out_cols, a + 16 * k + 8 * w, desc_mn(b + 2048 * k, L::BLOCK), id_pv, w == 0 || k > 0);
+                                umma_ts(out_cols, a + 16 * k + 8 * w, values + 2048 * k / 16, id_pv, w == 0 || k > 0);
                         umma_commit(o_full + 8 * h);
                         if (h == 1 || j >= p.nb) umma_commit(kv_empty + 8 * (vt % PSLOTS));
                     }
