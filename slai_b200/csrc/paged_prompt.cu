@@ -18,7 +18,7 @@
 // A region is written again by the third QK after its own; by then the PV that read it is complete: before each PV its issuer waits until the output of the PV
 // before has been read (one region for all of them), so that only the last PV issued can be under way.
 //
-// What bounds it: 1023 tokens of 64 heads on 8 behind 7001 positions, 445 us, 566 TFLOP/s, 1130 executed; the kernel itself 396 us, 1270 executed, where the card's
+// What bounds it: 1023 tokens of 64 heads on 8 behind 7001 positions, 445 us, 566 TFLOP/s, 1130 executed; the kernel itself 388 us, 1300 executed, where the card's
 // power allows 1400 (the clock falls to 1.55 GHz).  A unit of 128 positions takes 5400 cycles for products of 4096: a half's softmax (maximum 500, weights
 // 2000: 16 exponentials a cycle and SM, the wait for tensor memory), its product, the read of that and the next scores are one chain, longer than the other half's
 // products.  Few tokens: 511 of 32 heads 20.6 us in tiles of 128 rows, of which the queries' way to shared memory takes 5, the results' 3 (in tiles of 256: 24.7).
