@@ -440,10 +440,11 @@ def test_conversations_in_pages(ctx, backend, dtype, hs, hq, hk, page, variant):
         pos = [p + n for p, n in zip(pos, n_new)]
 
 
-def test_a_recorded_pass_follows_the_steps(ctx, backend):
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_a_recorded_pass_follows_the_steps(ctx, backend, dtype):
     """Append and attention recorded once, replayed for steps of other lengths: tokens only, a chunk beside tokens, fewer sequences."""
     hq, hk, hs = 8, 2, 128
-    P = Pages(backend, hq, hk, hs, 16, [260, 200, 150], F16, max_tokens=160, seed=12)
+    P = Pages(backend, hq, hk, hs, 16, [260, 200, 150], dtype, max_tokens=160, seed=12)
     how = QkNormRope(hs, hq, hk, 1)
     q, qo, out = (backend.zeros(160 * hq * hs) for _ in range(3))
     k, v = (backend.zeros(160 * hk * hs) for _ in range(2))
@@ -465,7 +466,7 @@ def test_a_recorded_pass_follows_the_steps(ctx, backend):
             if n:
                 here = np.arange(p, p + n)
                 check(rot[at:at + n], *R.norm_rope(xs[0][at:at + n], None, 0, 1, 10000.0, here))
-                assert (P.at(1, b, here) == xs[2][at:at + n].astype(np.float16)).all()
+                assert (P.at(1, b, here) == xs[2][at:at + n].astype(P.np_type)).all()
                 want, bound = R.attention(rot[at:at + n], P.at(0, b, np.arange(p + n)), P.at(1, b, np.arange(p + n)), p, hs**-0.5)
                 check(got[at:at + n], want, bound, f"sequence {b}")
             at += n
