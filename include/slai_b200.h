@@ -314,7 +314,7 @@ int slai_paged_append(slai_paged* p, const slai_paged_layer* layer, const slai_q
 /* Causal attention (ops/batched_multiquery_attention.rs:32-156) of the step's tokens: token at position t attends to positions 0 .. t of its sequence, which
  * are in the pages by then.  Rows of q and out: n_q_heads * head_size floats, q_ld / out_ld apart (0 = packed); no element of
  * out is one of q's.  scale 0: 1 / sqrt(head_size).  Sums,
- * weights and results are f32; f16 keys and values take part as they are cached.  Results do not depend on timing; their last bits may depend on what else is in the step. */
+ * weights and results are f32; f16 keys and values take part as they are cached.  Results do not depend on timing; their last bits may depend on what else is in the step and on whether the call is recorded. */
 int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, const float* d_q, int64_t q_ld, float scale, float* d_out, int64_t out_ld);
 
 /* ---- Llama-2 family: Llama2Config (models/llama2/cpu.rs:46-67), Llama2::launch (transformer.rs:316-381) */

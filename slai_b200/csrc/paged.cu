@@ -271,6 +271,7 @@ SLAI_API int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, 
     A.err_flag = ctx->d_counters + CNT_ERR_FLAG;
     A.wait_limit = ctx->wait_limit;
     const bool recording = capturing(ctx);
+    A.recorded = recording;
     for (int k = 0; k < 2; k++) {
         const Lane& l = p->planner.lane(k);
         if (l.blocks == 0) continue;

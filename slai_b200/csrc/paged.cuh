@@ -24,6 +24,7 @@ struct AttnArgs {
     float scale;
     int n_pages;
     int tile_rows, unit;     // of the lane
+    int recorded;            // the launch has room for any step: blocks and joins that this one does not have
     int vec;                 // rows of the cache can be read in 16-byte pieces
     int qvec;                // ... and rows of q and out
     float* part;             // [block][2][tile_rows][hs]: sums of (tile, head) pairs that lie on several blocks

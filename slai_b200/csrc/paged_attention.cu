@@ -189,11 +189,10 @@ __device__ __forceinline__ float join_weight(float m, float M) { return m == -IN
 struct JoinOf {  // one pair
     int row0, first, rows, head, begin, nb;
 };
-__device__ __forceinline__ bool load_join(const AttnArgs& A, JoinOf& j) {
-    const int4* g = reinterpret_cast<const int4*>(A.c.plan + A.joins_at) + 2 * blockIdx.x;
+__device__ __forceinline__ JoinOf load_join(const AttnArgs& A, int i) {
+    const int4* g = reinterpret_cast<const int4*>(A.c.plan + A.joins_at) + 2 * i;
     const int4 a = __ldcg(g), b = __ldcg(g + 1);
-    j = {a.x, a.y, a.z, a.w, b.x, b.y - b.x + 1};
-    return (int)blockIdx.x < __ldcg(A.c.plan + A.count_at);
+    return {a.x, a.y, a.z, a.w, b.x, b.y - b.x + 1};
 }
 __device__ __forceinline__ size_t part_slot(const AttnArgs& A, const JoinOf& j, int i, int r) { return ((size_t)(j.begin + i) * 2 + (i == 0)) * A.tile_rows + r; }
 __device__ __forceinline__ float* join_out(const AttnArgs& A, const JoinOf& j, int r) {
@@ -214,14 +213,10 @@ __device__ __forceinline__ void join_add(float4& a, float f, float4 o) {
 
 // A few results to a pair: a warp takes four rows; eight lanes of it have a row's weights.
 constexpr int JT = 64, JR = 4, JROWS = JT / 32 * JR;
-__global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ AttnArgs A) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hs = A.c.hs;
-    JoinOf j;
-    const bool on = load_join(A, j);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int r0 = (int)blockIdx.y * JROWS + warp * JR, n = min(JR, j.rows - r0);
-    if (!on || n <= 0) return;
+// Rows r0 .. r0 + JR - 1 of a pair, by one warp.
+__device__ __forceinline__ void join_rows(const AttnArgs& A, const JoinOf& j, int r0, int lane) {
+    const int n = min(JR, j.rows - r0), hs = A.c.hs;
+    if (n <= 0) return;
     const float2* ml = reinterpret_cast<const float2*>(A.part_ml);
     const int mine = min(lane >> 3, n - 1), b8 = lane & 7;
     const bool quads = hs % 4 == 0;
@@ -283,19 +278,26 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ 
         }
     }
 }
+// MORE: there may be more pairs than blocks for them.
+template <bool MORE>
+__global__ void __launch_bounds__(JT) paged_join_kernel(const __grid_constant__ AttnArgs A) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int joins = __ldcg(A.c.plan + A.count_at);
+    JoinOf j = load_join(A, blockIdx.x);  // (there is room for it, whether it is one or not)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int r0 = (int)blockIdx.y * JROWS + warp * JR;
+    if ((int)blockIdx.x < joins) join_rows(A, j, r0, lane);
+    if (MORE)
+        for (int i = blockIdx.x + gridDim.x; i < joins; i += gridDim.x) join_rows(A, load_join(A, i), r0, lane);
+}
 
 // Many results to a pair (one long sequence over many blocks): a block takes a row, its warps every LW-th result.
 constexpr int LT = 128, LW = LT / 32, JOIN_MANY = 8;
-__global__ void __launch_bounds__(LT) paged_join_many_kernel(const __grid_constant__ AttnArgs A) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hs = A.c.hs, r = (int)blockIdx.y;
-    JoinOf j;
-    const bool on = load_join(A, j);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!on || r >= j.rows) return;
+// Row r of a pair, by the block.
+__device__ __forceinline__ void join_row(const AttnArgs& A, const JoinOf& j, int r, float (&num_s)[LW][256], float (&den_s)[LW]) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hs = A.c.hs;
     const float2* ml = reinterpret_cast<const float2*>(A.part_ml);
-    __shared__ float num_s[LW][256];
-    __shared__ float den_s[LW];
     float M = -INFINITY;
     for (int b = lane; b < j.nb; b += 32) M = fmaxf(M, __ldcg(ml + part_slot(A, j, b, r)).x);
 #pragma unroll
@@ -336,13 +338,32 @@ __global__ void __launch_bounds__(LT) paged_join_many_kernel(const __grid_consta
         join_out(A, j, r)[d] = n / den;
     }
 }
+// MORE: there may be more pairs than blocks for them.
+template <bool MORE>
+__global__ void __launch_bounds__(LT) paged_join_many_kernel(const __grid_constant__ AttnArgs A) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int r = (int)blockIdx.y;
+    const int joins = __ldcg(A.c.plan + A.count_at);
+    JoinOf j = load_join(A, blockIdx.x);  // (there is room for it, whether it is one or not)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ float num_s[LW][256];
+    __shared__ float den_s[LW];
+    if ((int)blockIdx.x < joins && r < j.rows) join_row(A, j, r, num_s, den_s);
+    if (MORE)
+        for (int i = blockIdx.x + gridDim.x; i < joins; i += gridDim.x) {
+            j = load_join(A, i);
+            __syncthreads();  // the sums before have been read
+            if (r < j.rows) join_row(A, j, r, num_s, den_s);
+        }
+}
 
 // `longest`: most results of a pair.  us of the call, a warp for four rows / a block for each: 272 pairs of 2 or 3 results of 8 rows 98.8 / 102; 8 pairs of 37 results
 // 38.8 / 32.5; 141 pairs of 2 or 3 of 256 rows 475 / 494.
+template <bool MORE>
 int launch_join(slai_ctx* ctx, const AttnArgs& A, int joins, int longest, bool pdl) {
     if (joins <= 0) return SLAI_OK;
-    if (longest > JOIN_MANY && A.tile_rows <= 16) return launch_dependent(ctx, paged_join_many_kernel, dim3((unsigned)joins, (unsigned)A.tile_rows), LT, 0, pdl, A);
-    return launch_dependent(ctx, paged_join_kernel, dim3((unsigned)joins, (unsigned)((A.tile_rows + JROWS - 1) / JROWS)), JT, 0, pdl, A);
+    if (longest > JOIN_MANY && A.tile_rows <= 16) return launch_dependent(ctx, paged_join_many_kernel<MORE>, dim3((unsigned)joins, (unsigned)A.tile_rows), LT, 0, pdl, A);
+    return launch_dependent(ctx, paged_join_kernel<MORE>, dim3((unsigned)joins, (unsigned)((A.tile_rows + JROWS - 1) / JROWS)), JT, 0, pdl, A);
 }
 
 // ---- PTX wrappers --------------------------------------------------------------------------------------------------------
@@ -833,5 +854,7 @@ static int launch_lane(slai_ctx* ctx, const AttnArgs& A, int kv_dtype, int lane,
 int paged_attention_launch(slai_ctx* ctx, AttnArgs& A, int kv_dtype, int lane, int blocks, int joins, int longest, bool pdl) {
     if (blocks <= 0) return SLAI_OK;
     const int rc = launch_lane(ctx, A, kv_dtype, lane, blocks, pdl);
-    return rc ? rc : launch_join(ctx, A, joins, longest, pdl);
+    if (rc) return rc;
+    // (recorded: a launch for the most pairs that there can be took 2 to 3 us when there were none)
+    return A.recorded ? launch_join<true>(ctx, A, (joins + 3) / 4, longest, pdl) : launch_join<false>(ctx, A, joins, longest, pdl);
 }

@@ -128,6 +128,11 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
         if (threadIdx.x == 0) atomicExch(A.err_flag, (unsigned int)ERR_PAGED);
         return;
     }
+    if (A.recorded && __ldcg(A.c.plan + A.starts_at + (int)(sizeof(Start) / 4) * blockIdx.x + 3) <= 0) {  // (count) there is room for more blocks than the step has
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     const uint32_t sb = smem_u32(smem), ring = sb + L::RING;
     const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * PSLOTS, q_full = kv_empty + 8 * PSLOTS, s_full = q_full + 16, p_full = s_full + 32, o_full = p_full + 16,
                    o_free = o_full + 16, all_done = o_free + 8;

@@ -93,6 +93,11 @@ __global__ void __launch_bounds__(XT, 1) paged_attn_prompt32_kernel(const __grid
         if (threadIdx.x == 0) atomicExch(A.err_flag, (unsigned int)ERR_PAGED);
         return;
     }
+    if (A.recorded && __ldcg(A.c.plan + A.starts_at + (int)(sizeof(Start) / 4) * blockIdx.x + 3) <= 0) {  // (count) there is room for more blocks than the step has
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     const uint32_t sb = smem_u32(smem);
     const uint32_t k_full = smem_u32(rest.bars), v_full = k_full + 16, qk_done = v_full + 16, p_full = qk_done + 16, pv_done = p_full + 16, q_full = pv_done + 16, all_done = q_full + 8;
     const Cache& c = A.c;

@@ -489,6 +489,34 @@ def test_a_recorded_pass_follows_the_steps(ctx, backend, dtype):
     rec.close()
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hq, hk, n_new", [(16, 8, [1] * 40), (16, 16, [131] * 9), (16, 8, [1] * 20 + [100] * 9)])
+def test_a_recorded_pass_with_many_pairs_on_several_blocks(ctx, backend, hq, hk, n_new, dtype):
+    """More joins than a recorded launch has blocks for at once.  (A recorded call may join in another order than the step's own: held to the formula's bound, not to
+    that call's bits; its replays have the same bits.)"""
+    rng = np.random.default_rng(21)
+    pos0 = [int(x) for x in rng.integers(300, 1200, len(n_new))]
+    P = Pages(backend, hq, hk, 128, 16, [p + n for p, n in zip(pos0, n_new)], dtype, seed=21)
+    rows = sum(n_new)
+    q = rng.standard_normal((rows, hq, 128)).astype(np.float32) * 2
+    P.kv.step(pos0, n_new, P.tables)
+    most = P.kv.max_tokens * hq * 128
+    qd, out = backend.zeros(most), backend.vector(np.full(most, 4.5, np.float32))
+    backend.write_buffer(qd.ptr, q.reshape(-1))
+    with backend.record() as rec:
+        ctx.paged_attention(P.kv, P.layer, qd, out)
+    rec.launch()
+    got, at = out.to_numpy(), 0
+    rec.launch()
+    assert np.array_equal(got, out.to_numpy()) and (got[q.size:] == 4.5).all()
+    rec.close()
+    for b, (p, n) in enumerate(zip(pos0, n_new)):
+        held = np.arange(p + n)
+        want, bound = R.attention(q[at:at + n], P.at(0, b, held), P.at(1, b, held), p, 128**-0.5)
+        check(got[:q.size].reshape(q.shape)[at:at + n], want, bound, f"sequence {b}")
+        at += n
+
+
 def test_two_handles_and_two_contexts(ctx, backend):
     """Handles of one context alternate; another context on the same GPU works beside them."""
     from slai_b200.ops import Backend, LlmContext
