@@ -1,0 +1,31 @@
+// Orders of work inside the paged chunk kernels, apart from what does the work: plain C++, which the kernels and the host's tests both compile.
+#pragma once
+#include <stdint.h>
+
+#ifndef PAGED_HD
+#ifdef __CUDACC__
+#define PAGED_HD __host__ __device__ __forceinline__
+#else
+#define PAGED_HD inline
+#endif
+#endif
+
+namespace paged {
+
+// Products of a part of `n` units whose first has number `u`, with two stages of tensor memory that hold a unit's scores and then, in their place, its weights
+// (paged_prompt32.cu).  scores(i): QK of unit i, into stage i % 2.  outputs(i): PV of unit i, once the weights stand in stage i % 2.  Products of
+// different shapes and accumulators have no order of their own: before scores(i) overwrites the weights of unit i - 2, done(i - 2) waits for the PV that reads them.
+template <class Done, class Scores, class Outputs>
+PAGED_HD void chunk_products(uint32_t u, int n, Done done, Scores scores, Outputs outputs) {
+    auto next = [&](uint32_t i) {
+        if (i >= 2) done(i - 2);
+        scores(i);
+    };
+    next(u);
+    for (int j = 0; j < n; j++) {
+        if (j + 1 < n) next(u + j + 1);
+        outputs(u + j);
+    }
+}
+
+}  // namespace paged

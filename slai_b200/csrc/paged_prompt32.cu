@@ -12,8 +12,9 @@
 //   warps 12-27  keys and values, two sets of eight in turn: out of the pages two steps ahead into registers, in two parts each into shared memory, rows of 128 bytes in the tensor core's swizzle.
 //                Values lie there with a row a dimension: a thread reads four positions of one dimension, a warp's threads next to each other.
 //
-// Barriers: a stage of scores, weights, keys and values has a unit's number's parity; a unit's QK and PV being complete is what frees them.
-// 1023 tokens of 32 heads behind 2000 positions 208 us, 202 TFLOP/s, 606 executed, where the card's power sets the clock (1.6 GHz); 37 tokens behind 300 17 us.  (f32 arithmetic
+// Barriers: a stage of scores, weights, keys and values has a unit's number's parity; a unit's QK and PV being complete is what frees them.  (The issuer waits for the PV of
+// unit u - 1 before the QK of unit u + 1 takes its stage: paged_order.h.  It costs 1 %, 211 for 208 us: most of it is time in which the next weights were waited for.)
+// 1023 tokens of 32 heads behind 2000 positions 211 us, 199 TFLOP/s, 597 executed, where the card's power sets the clock (1.6 GHz); 37 tokens behind 300 16 us.  (f32 arithmetic
 // of 64 rows and 32 positions in shared memory: 31 TFLOP/s, 25 us.)
 // What bounds it: 32 positions take 2500 cycles (511 tokens), of which the 44 products take 1960 (1540 at the full rate) and what their issuer waits for between them 540.
 // Descriptors in uniform registers: 225 -> 208 us.  A thread a row: 209, but 19 for 17 us with few tokens.
@@ -21,6 +22,7 @@
 // Every wait is bounded (common.cuh, bounded_wait).
 #include <type_traits>
 
+#include "paged_order.h"
 #include "paged_tc.cuh"
 
 using namespace paged;
@@ -174,11 +176,7 @@ __global__ void __launch_bounds__(XT, 1) paged_attn_prompt32_kernel(const __grid
                     }
                     __syncwarp();
                 };
-                do_qk(u);
-                for (int j = 0; j < p.n; j++) {
-                    if (j + 1 < p.n) do_qk(u + j + 1);
-                    do_pv(u + j);
-                }
+                chunk_products(u, p.n, [&](uint32_t i) { wait(pv_done + 8 * (i & 1), i >> 1); }, do_qk, do_pv);
                 u += p.n;
             });
             if (elect_one()) umma_commit(all_done);  // no product is under way when the block ends
