@@ -28,4 +28,18 @@ PAGED_HD void chunk_products(uint32_t u, int n, Done done, Scores scores, Output
     }
 }
 
+// One slot of a ring, as its filler sees it (paged_prompt.cu).  Fill i completes phase i of the slot's "full" barrier; its reader completes phase i of "empty".
+// A wait that gives up returns false: nothing is filled then, nor counted, so that settle() waits for the last fill that was asked for, whatever was left out behind it.
+// (A phase is told by its parity alone: a wait for one that nobody begins would be over at once, or never.)
+struct SlotFills {
+    uint32_t sent = 0;
+    template <class Empty>  // empty(i): waits for phase i
+    PAGED_HD bool may_fill(Empty empty) const { return sent == 0 || empty(sent - 1); }
+    PAGED_HD void filled() { sent++; }
+    template <class Full>  // full(i): waits for phase i
+    PAGED_HD void settle(Full full) const {
+        if (sent > 0) full(sent - 1);
+    }
+};
+
 }  // namespace paged

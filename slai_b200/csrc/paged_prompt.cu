@@ -30,6 +30,7 @@
 
 #include <cuda.h>
 
+#include "paged_order.h"
 #include "paged_tc.cuh"
 
 using namespace paged;
@@ -177,18 +178,20 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
             constexpr int CH = HS / 8, STEP = 32 / CH;  // 16-byte pieces of a row, rows a pass of the warp covers
             const int ch = lane % CH, rl = lane / CH, chunks = hs / 8;
             const uint32_t dst0 = ring + slot * L::TILE + (ch >> 3) * L::BLOCK;
-            int next = slot, base = 0, round = 0;  // number of this warp's next tile, of the part's first
+            int next = slot, base = 0;  // number of this warp's next tile, of the part's first
+            SlotFills fills;
+            auto give_up = [&]() { return !fills.may_fill([&](uint32_t i) { return wait(kv_empty + 8 * slot, i), !__any_sync(0xffffffffu, limit == 0); }); };
             for_parts(s, c, [&](const Tile& t, int head, const Part& p) {
                 const int hi = t.pos0 + (t.first + t.rows - 1) / c.group + 1;
-                for (; next < base + 2 * p.n; next += PSLOTS, round++) {
+                for (; next < base + 2 * p.n; next += PSLOTS) {
                     const int j = (next - base) >> 1, p0 = (p.unit + j) * PU;
                     const char* from = (next - base) & 1 ? c.values : c.keys;
                     if (box > 0 && p0 + PU <= hi) {
                         // a page is a box of `box` rows and 64 dimensions; lane i has the number of the tile's i-th
                         const int i_page = p0 / c.page_size, boxes = PU / box;
                         const int id = lane < boxes ? __ldcg(c.plan + t.table + i_page + (lane * box) / c.page_size) : 0;
-                        if (round > 0) wait(kv_empty + 8 * slot, round - 1);
-                        if (__any_sync(0xffffffffu, limit == 0)) continue;
+                        if (give_up()) continue;
+                        fills.filled();
                         if (elect_one()) mbar_expect_tx(kv_full + 8 * slot, L::TILE);
                         __syncwarp();
                         for (int i = 0; i < boxes; i++) {
@@ -206,8 +209,8 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
                     long long at[4];  // places of positions 32 i + lane, -1 behind the last
 #pragma unroll
                     for (int i = 0; i < 4; i++) at[i] = p0 + 32 * i + lane < hi ? 2 * place_of(c, t.table, p0 + 32 * i + lane, head) : -1;
-                    if (round > 0) wait(kv_empty + 8 * slot, round - 1);
-                    if (__any_sync(0xffffffffu, limit == 0)) continue;
+                    if (give_up()) continue;
+                    fills.filled();
 #pragma unroll
                     for (int i = 0; i < 4; i++)
 #pragma unroll 4
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(PT, 1) paged_attn_prompt_kernel(const __grid_c
             });
             asm volatile("cp.async.wait_all;" ::: "memory");
             limit = LAST_POLLS;
-            if (round > 0) wait(kv_full + 8 * slot, round - 1);  // the last copy lands before the block ends
+            fills.settle([&](uint32_t i) { wait(kv_full + 8 * slot, i); });  // the last copy lands before the block ends
         } else {
             // ---- products ----
             const uint32_t id_qk = idesc(128, false), id_pv = idesc(HS, true);

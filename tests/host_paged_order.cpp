@@ -49,3 +49,41 @@ const char* host_chunk_products(const int* units, int parts) {
     return why.c_str();
 }
 }
+
+namespace {
+struct Barrier {  // phases begun and completed; a wait knows a phase by its parity alone
+    uint32_t done = 0;
+    bool over(uint32_t phase) const { return (done & 1) != (phase & 1); }
+};
+}  // namespace
+extern "C" {
+// `rounds` fills of a slot whose reader stops after `reads` of them (a wait for the next then gives up, as do all behind it), the last fill being still on its way: how often
+// settle() says that all have landed while one has not, or waits for a phase that nobody will complete.
+int host_settles_wrongly(int rounds, int reads) {
+    SlotFills f;
+    Barrier full, empty;
+    int asked = 0;
+    bool gone = false;
+    for (int r = 0; r < rounds; r++) {
+        const bool go = f.may_fill([&](uint32_t i) {
+            if (gone) return false;
+            if (empty.done < (uint32_t)reads && (uint32_t)asked > empty.done) empty.done++;  // the reader has had its last fill
+            gone = !empty.over(i);
+            return !gone;
+        });
+        if (!go) continue;
+        if (asked > 0) full.done = asked;  // the reader can only have read what had landed
+        f.filled();
+        asked++;
+    }
+    int wrong = 0;
+    bool waited = false;
+    f.settle([&](uint32_t i) {
+        waited = true;
+        if (full.over(i)) wrong++;       // over although the last is on its way
+        full.done = asked;
+        if (!full.over(i)) wrong++;      // not over although it has landed
+    });
+    return wrong + (asked > 0 && !waited);
+}
+}

@@ -22,3 +22,9 @@ def lib(tmp_path_factory):
 def test_scores_wait_for_the_product_that_reads_what_they_overwrite(lib, units):
     """Two products of different shapes have no order but the one that a wait gives them."""
     assert lib.host_chunk_products((C.c_int * len(units))(*units), len(units)).decode() == ""
+
+
+@pytest.mark.parametrize("rounds", range(0, 9))
+@pytest.mark.parametrize("reads", range(0, 9))
+def test_the_last_fill_of_a_slot_is_waited_for_when_a_wait_gave_up(lib, rounds, reads):
+    assert lib.host_settles_wrongly(rounds, reads) == 0
