@@ -276,7 +276,8 @@ int slai_kv_append(slai_ctx* ctx, void* d_key_cache, void* d_value_cache, int kv
  * checked on the host (SLAI_ERR_SHAPE; the step before stays in force): capacity, page numbers, and that a page which gets new tokens is used once (pages that
  * are only read may be shared).  The call copies the tables and returns; it serves every layer until the next step.  It cannot be recorded: a recorded
  * append or attention (slai_pass_*) reads the step that is current when it runs, so its buffers hold max_tokens rows.
- * One handle is used on one context's stream.  Destroy handles before their context. */
+ * One handle is used on one context's stream.  Destroy handles before their context, and not while a pass is recorded (SLAI_ERR_INVALID_ARG).  A pass that was recorded
+ * with a handle keeps what it needs of it: after slai_paged_destroy its replays go on with the handle's last step (the pages and rows are the caller's to keep). */
 typedef struct slai_paged_config {
     int32_t n_q_heads, n_kv_heads, head_size; /* n_kv_heads divides n_q_heads; head_size 1 .. 256 */
     int32_t page_size, n_pages, kv_dtype;     /* slai_kv_dtype */

@@ -6,6 +6,7 @@
 #include <stdint.h>
 #include <stdio.h>
 #include <atomic>
+#include <memory>
 #include <string>
 #include <vector>
 #include <unordered_map>
@@ -48,6 +49,9 @@ struct slai_ctx {
     void* d_scratch = nullptr;      // attention split partials etc.
     size_t scratch_bytes = 0;
     std::vector<void*> retired_scratch;  // outgrown scratch buffers: recorded passes may still point at them, freed with the context
+    bool in_pass = false;                          // between slai_pass_begin and slai_pass_end
+    std::vector<std::shared_ptr<void>> pass_keeps;  // what the calls recorded so far need of a handle's memory: the pass has it from its end on
+    std::vector<std::shared_ptr<void>> kept;        // ... of calls that somebody else's capture of the stream recorded: freed with the context
     std::vector<RopeTable> rope_tables;
     std::vector<TurnTable> turn_tables;
     unsigned long long* trace_buf = nullptr;  // trace build only: per-block stamps of the last 64 GEMV launches
@@ -120,6 +124,8 @@ __device__ __forceinline__ bool bounded_wait(uint32_t a, uint32_t parity, unsign
 #endif
 
 int slai_set_error(slai_ctx* ctx, int code, const char* fmt, ...);
+// A recorded call on the context's stream uses `memory`, which lives as long as the pass (ops.cu).
+int slai_keep_for_pass(slai_ctx* ctx, const std::shared_ptr<void>& memory);
 int slai_check_wait_flag(slai_ctx* ctx);  // ops.cu: SLAI_ERR_TIMEOUT if a bounded device-side wait ran out (stream must be idle)
 
 // Every exported function runs with its context's device current and puts the caller's device back on return, so

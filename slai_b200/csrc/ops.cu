@@ -4,6 +4,8 @@
 #include <math.h>
 #include <stdlib.h>
 
+#include <exception>
+
 #include "common.cuh"
 #include "gemv_frag.cuh"
 #include "layout.cuh"
@@ -85,6 +87,8 @@ SLAI_API int slai_ctx_destroy(slai_ctx* ctx) {
     for (auto& t : ctx->turn_tables) cudaFree(t.d_turns);
     if (ctx->d_scratch) cudaFree(ctx->d_scratch);
     for (void* p : ctx->retired_scratch) cudaFree(p);
+    ctx->pass_keeps.clear();
+    ctx->kept.clear();
     if (ctx->d_counters) cudaFree(ctx->d_counters);
     cudaEventDestroy(ctx->ev0);
     slai_tp_shutdown(ctx);
@@ -199,11 +203,24 @@ SLAI_API int slai_free_host(slai_ctx* ctx, void* h_ptr) {
 // ---- recorded passes ---------------------------------------------------------------------------------
 struct slai_pass {
     cudaGraphExec_t exec = nullptr;
+    std::vector<std::shared_ptr<void>> keeps;
 };
+int slai_keep_for_pass(slai_ctx* ctx, const std::shared_ptr<void>& memory) {
+    auto& list = ctx->in_pass ? ctx->pass_keeps : ctx->kept;
+    for (auto& m : list)
+        if (m == memory) return SLAI_OK;
+    try {
+        list.push_back(memory);
+    } catch (const std::exception&) {
+        return slai_set_error(ctx, SLAI_ERR_OOM, "pass: no host memory");
+    }
+    return SLAI_OK;
+}
 SLAI_API int slai_pass_begin(slai_ctx* ctx) {
     if (!ctx) return SLAI_ERR_INVALID_ARG;
     SLAI_ENTER(ctx);
     SLAI_CHECK_CUDA(ctx, cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal));
+    ctx->in_pass = true;
     return SLAI_OK;
 }
 SLAI_API int slai_pass_end(slai_ctx* ctx, slai_pass** out) {
@@ -212,12 +229,16 @@ SLAI_API int slai_pass_end(slai_ctx* ctx, slai_pass** out) {
     *out = nullptr;
     cudaGraph_t graph = nullptr;
     cudaError_t e = cudaStreamEndCapture(ctx->stream, &graph);
+    std::vector<std::shared_ptr<void>> keeps;
+    keeps.swap(ctx->pass_keeps);
+    ctx->in_pass = false;
     if (e != cudaSuccess || !graph) {
         cudaGetLastError();
         return slai_set_error(ctx, SLAI_ERR_CUDA, "pass: recording failed (%s); a recorded call allocated or blocked",
                               cudaGetErrorString(e));
     }
     slai_pass* p = new slai_pass();
+    p->keeps.swap(keeps);
     e = cudaGraphInstantiate(&p->exec, graph, 0);
     cudaGraphDestroy(graph);
     if (e != cudaSuccess) {

@@ -45,25 +45,34 @@ int turn_table(slai_ctx* ctx, int hs, float base, const double** out) {
 }
 }  // namespace
 
+namespace {
+// What the kernels of a handle read and write beside the caller's buffers.  Passes that were recorded with the handle have a share in it.
+struct DeviceSide {
+    int* plan = nullptr;
+    float *part[2] = {}, *ml[2] = {};
+    ~DeviceSide() {
+        cudaFree(plan);
+        for (int k = 0; k < 2; k++) {
+            cudaFree(part[k]);
+            cudaFree(ml[k]);
+        }
+    }
+};
+}  // namespace
+
 struct slai_paged {
     slai_ctx* ctx = nullptr;
     Config cfg = {};
     Planner planner;
     Step step;
-    int* d_plan = nullptr;
+    std::shared_ptr<DeviceSide> dev = std::make_shared<DeviceSide>();
     int* h_plan[SLOTS] = {};
     cudaEvent_t copied[SLOTS] = {};
     int slot = 0;
-    float *d_part[2] = {}, *d_ml[2] = {};
     ~slai_paged() {
-        cudaFree(d_plan);
         for (int i = 0; i < SLOTS; i++) {
             if (h_plan[i]) cudaFreeHost(h_plan[i]);
             if (copied[i]) cudaEventDestroy(copied[i]);
-        }
-        for (int k = 0; k < 2; k++) {
-            cudaFree(d_part[k]);
-            cudaFree(d_ml[k]);
         }
     }
 };
@@ -81,7 +90,7 @@ int make_handle(slai_ctx* ctx, slai_paged* p) {
     if (fast && (long long)c.max_tokens * group > few_rows) many = f16 ? paged_prompt_lane(sms) : paged_prompt32_lane(sms);
     p->planner.init(c, few, many, few_rows, PERHAPS_ROWS);
     const size_t bytes = (size_t)p->planner.lay().total * 4;
-    SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_plan, bytes));
+    SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->dev->plan, bytes));
     for (int i = 0; i < SLOTS; i++) {
         SLAI_CHECK_CUDA(ctx, cudaMallocHost(&p->h_plan[i], bytes));
         SLAI_CHECK_CUDA(ctx, cudaEventCreateWithFlags(&p->copied[i], cudaEventDisableTiming));
@@ -89,8 +98,8 @@ int make_handle(slai_ctx* ctx, slai_paged* p) {
     for (int k = 0; k < 2; k++) {
         const Lane& l = p->planner.lane(k);
         if (l.blocks == 0) continue;
-        SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_part[k], sizeof(float) * 2 * l.blocks * l.rows * c.head_size));
-        SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->d_ml[k], sizeof(float) * 2 * l.blocks * l.rows * 2));
+        SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->dev->part[k], sizeof(float) * 2 * l.blocks * l.rows * c.head_size));
+        SLAI_CHECK_CUDA(ctx, cudaMalloc(&p->dev->ml[k], sizeof(float) * 2 * l.blocks * l.rows * 2));
     }
     return SLAI_OK;
 }
@@ -105,7 +114,7 @@ int fill_cache(slai_paged* p, const slai_paged_layer* layer, Cache* out) {
                  (long long)layer->head_stride, (long long)layer->pos_stride, c.head_size);
     const uintptr_t esz = c.kv_dtype == SLAI_KV_F16 ? 2 : 4;
     SLAI_REQUIRE(ctx, ((uintptr_t)layer->d_keys | (uintptr_t)layer->d_values) % esz == 0, SLAI_ERR_INVALID_ARG, "paged: the pages are not aligned to their type");
-    out->plan = p->d_plan;
+    out->plan = p->dev->plan;
     out->count_at = p->planner.lay().count;
     out->rows_at = p->planner.lay().rows;
     out->keys = (char*)layer->d_keys;
@@ -173,6 +182,7 @@ SLAI_API int slai_paged_create(slai_ctx* ctx, const slai_paged_config* cfg, slai
 SLAI_API int slai_paged_destroy(slai_paged* p) {
     if (!p) return SLAI_OK;
     SLAI_ENTER(p->ctx);
+    SLAI_REQUIRE(p->ctx, !capturing(p->ctx), SLAI_ERR_INVALID_ARG, "paged: a handle cannot be destroyed while a pass is recorded");
     cudaStreamSynchronize(p->ctx->stream);
     delete p;
     return SLAI_OK;
@@ -196,10 +206,10 @@ SLAI_API int slai_paged_step(slai_paged* p, int n_seq, const int32_t* h_pos0, co
     const Layout& L = p->planner.lay();
     const size_t head = (size_t)L.rows + 2 * (size_t)st.n_rows, gap = L.dynamic - head;
     if (gap <= 16384) {  // one copy of what lies between them too: 64 KB are less than a second request
-        SLAI_CHECK_CUDA(ctx, cudaMemcpyAsync(p->d_plan, h, 4 * ((size_t)L.dynamic + st.used), cudaMemcpyHostToDevice, ctx->stream));
+        SLAI_CHECK_CUDA(ctx, cudaMemcpyAsync(p->dev->plan, h, 4 * ((size_t)L.dynamic + st.used), cudaMemcpyHostToDevice, ctx->stream));
     } else {
-        SLAI_CHECK_CUDA(ctx, cudaMemcpyAsync(p->d_plan, h, 4 * head, cudaMemcpyHostToDevice, ctx->stream));
-        if (st.used) SLAI_CHECK_CUDA(ctx, cudaMemcpyAsync(p->d_plan + L.dynamic, h + L.dynamic, 4 * (size_t)st.used, cudaMemcpyHostToDevice, ctx->stream));
+        SLAI_CHECK_CUDA(ctx, cudaMemcpyAsync(p->dev->plan, h, 4 * head, cudaMemcpyHostToDevice, ctx->stream));
+        if (st.used) SLAI_CHECK_CUDA(ctx, cudaMemcpyAsync(p->dev->plan + L.dynamic, h + L.dynamic, 4 * (size_t)st.used, cudaMemcpyHostToDevice, ctx->stream));
     }
     SLAI_CHECK_CUDA(ctx, cudaEventRecord(p->copied[p->slot], ctx->stream));
     p->slot = (p->slot + 1) % SLOTS;
@@ -238,6 +248,7 @@ SLAI_API int slai_paged_append(slai_paged* p, const slai_paged_layer* layer, con
     A.q = d_q; A.k = d_k; A.v = d_v; A.q_out = d_q_out;
     A.kv_f16 = p->cfg.kv_dtype == SLAI_KV_F16;
     if (capturing(ctx)) {
+        if ((rc = slai_keep_for_pass(ctx, p->dev))) return rc;
         A.rows = p->cfg.max_tokens;
         A.counted = 1;
     }
@@ -271,6 +282,7 @@ SLAI_API int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, 
     A.err_flag = ctx->d_counters + CNT_ERR_FLAG;
     A.wait_limit = ctx->wait_limit;
     const bool recording = capturing(ctx);
+    if (recording && (rc = slai_keep_for_pass(ctx, p->dev))) return rc;
     A.recorded = recording;
     for (int k = 0; k < 2; k++) {
         const Lane& l = p->planner.lane(k);
@@ -280,8 +292,8 @@ SLAI_API int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, 
         A.count_at = p->planner.lay().count + 1 + k;
         A.tile_rows = l.rows;
         A.unit = l.unit;
-        A.part = p->d_part[k];
-        A.part_ml = p->d_ml[k];
+        A.part = p->dev->part[k];
+        A.part_ml = p->dev->ml[k];
         if ((rc = paged_attention_launch(ctx, A, c.kv_dtype, k, recording ? l.blocks : p->step.blocks[k], recording ? l.blocks : p->step.joins[k],
                                          recording ? l.blocks : p->step.longest[k], ctx->use_pdl))) return rc;
     }

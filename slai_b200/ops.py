@@ -116,6 +116,7 @@ class RecordedPass:
 
     def __enter__(self):
         self.backend._deferred = []
+        self.backend._deferred_handles = []
         self.backend._recording = True
         self.backend.check(self.backend.lib.slai_pass_begin(self.backend.h))
         return self
@@ -126,6 +127,9 @@ class RecordedPass:
         for ptr in self.backend._deferred:  # buffers dropped by the garbage collector while recording
             self.backend.free(ptr)
         self.backend._deferred = []
+        for destroy, h in self.backend._deferred_handles:  # ... and handles
+            destroy(h)
+        self.backend._deferred_handles = []
         if et is None:
             self.backend.check(rc)
         return False
@@ -345,9 +349,12 @@ class PagedKv:
 
     def __del__(self):
         try:
-            if self.backend.h and self.h and not getattr(self.backend, "_recording", False):
-                self.backend.lib.slai_paged_destroy(self.h)
-                self.h = None
+            if self.backend.h and self.h:
+                destroy, h, self.h = self.backend.lib.slai_paged_destroy, self.h, None
+                if getattr(self.backend, "_recording", False):
+                    self.backend._deferred_handles.append((destroy, h))  # (as Backend.free)
+                else:
+                    destroy(h)
         except Exception:
             pass
 

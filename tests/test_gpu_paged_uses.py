@@ -1,0 +1,65 @@
+"""Ways in which a program may use the paged operators beside one call after the other."""
+import gc
+
+import numpy as np
+import pytest
+
+from slai_b200 import _lib
+from slai_b200._lib import KV_F16, KV_F32
+from slai_b200.ops import QkNormRope
+from test_gpu_paged import Pages, attend, refused
+
+pytestmark = pytest.mark.gpu
+F16, F32 = KV_F16, KV_F32
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_a_recorded_pass_outlives_its_handle(ctx, backend, dtype):
+    """Its replays go on with the last step, whoever has asked for memory since; the handle's memory goes with the pass."""
+    hq, hk, hs, most = 16, 8, 128, 150
+    P = Pages(backend, hq, hk, hs, 16, [1500, 700, 300], dtype, max_tokens=most, seed=31)
+    how = QkNormRope(hs, hq, hk, 1)
+    x = [P.rng.standard_normal(most * h * hs).astype(np.float32) for h in (hq, hk, hk)]
+    q, k, v = (backend.vector(a) for a in x)
+    qo, out = backend.zeros(q.n), backend.zeros(q.n)
+    P.kv.step([1499, 600, 299], [1, 100, 1], P.tables)
+    calls = lambda: (ctx.paged_append(P.kv, P.layer, how, q, k, v, qo), ctx.paged_attention(P.kv, P.layer, qo, out))  # noqa: E731
+    calls()
+    with backend.record() as rec:
+        calls()
+    rec.launch()
+    want = out.to_numpy()
+    assert np.abs(want[:102 * hq * hs]).min() > 0
+
+    def free_bytes():
+        backend.synchronize()
+        return backend.mem_info()[0]
+
+    before = free_bytes()
+    P.kv = None
+    gc.collect()
+    junk = [backend.vector(np.full(1 << 18, -1, np.int32), np.int32) for _ in range(64)]  # would lie where the plan and the partial results were
+    backend.write_buffer(out.ptr, np.full(out.n, 4.5, np.float32))
+    rec.launch(3)
+    got = out.to_numpy()
+    assert np.array_equal(got[:102 * hq * hs], want[:102 * hq * hs]) and (got[102 * hq * hs:] == 4.5).all()
+    for j in junk:
+        assert (j.to_numpy() == -1).all()
+    del junk, j
+    assert free_bytes() <= before
+    rec.close()
+    assert free_bytes() > before
+
+
+def test_a_handle_is_not_destroyed_while_a_pass_is_recorded(ctx, backend):
+    P = Pages(backend, 4, 2, 64, 16, [40, 20], F16)
+    P.kv.step([39, 19], [1, 1], P.tables)
+    q, out = backend.zeros(60 * 4 * 64), backend.zeros(60 * 4 * 64)
+    ctx.paged_attention(P.kv, P.layer, q, out)
+    with backend.record() as rec:
+        ctx.paged_attention(P.kv, P.layer, q, out)
+        refused(_lib.ERR_INVALID_ARG, "recorded", lambda: backend.check(backend.lib.slai_paged_destroy(P.kv.h)))
+    rec.launch(2)
+    backend.synchronize()
+    rec.close()
+    attend(ctx, P, [39, 19], [1, 1])
