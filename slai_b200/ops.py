@@ -377,6 +377,10 @@ class QkNormRope:
         self.at = C.addressof(self.c)
 
 
+def _refuse_context():
+    raise SlaiError(_lib.ERR_INVALID_ARG, "paged: the handle is another context's (its calls would run on that context's stream)")
+
+
 def _refuse_rows(what: str, x, rows: int, width: int, ld: int):
     raise SlaiError(_lib.ERR_SHAPE, f"{what}: {0 if x is None else len(x)} floats for {rows} rows of {width}, {ld or width} apart")
 
@@ -501,6 +505,8 @@ class LlmContext:
 
     def paged_append(self, paged: PagedKv, layer: PagedLayer, how: QkNormRope, q, k, v, q_out):
         """The same for the rows of the current step; keys and values go into their pages, q to q_out."""
+        if paged.backend is not self.backend:
+            _refuse_context()
         paged.check_layer(layer)
         n = paged.rows_in_use()
         if n:
@@ -521,6 +527,8 @@ class LlmContext:
 
     def paged_attention(self, paged: PagedKv, layer: PagedLayer, q, out, scale: float = 0.0, q_ld: int = 0, out_ld: int = 0):
         """Causal attention of the step's tokens to what their sequences hold (scale 0: 1 / sqrt(head_size))."""
+        if paged.backend is not self.backend:
+            _refuse_context()
         paged.check_layer(layer)
         n, width = paged.rows_in_use(), paged.width
         if n:

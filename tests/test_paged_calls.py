@@ -2,7 +2,9 @@
 import numpy as np
 import pytest
 
-from slai_b200.ops import Backend, GpuVector, PagedKv, RecordedPass
+from slai_b200 import _lib
+from slai_b200._lib import KV_F16, SlaiError
+from slai_b200.ops import Backend, GpuVector, LlmContext, PagedKv, PagedLayer, QkNormRope, RecordedPass
 
 
 class Library:
@@ -53,3 +55,31 @@ def test_a_handle_that_is_dropped_while_a_pass_is_recorded_is_destroyed_behind_i
     h = kv.h.value
     del kv
     assert [a[0].value for a in be.lib.named("slai_paged_destroy")][1:] == [h]
+
+
+def refused(code, word, f, *args, **kw):
+    with pytest.raises(SlaiError, match=word) as e:
+        f(*args, **kw)
+    assert e.value.code == code
+
+
+def cache(be, hq=4, hk=2, hs=64, page=16, n_pages=10, dtype=KV_F16, **kw):
+    """A handle and a layer of the right size."""
+    pages = [GpuVector(be, n_pages * hk * page * hs, np.float16 if dtype == KV_F16 else np.float32) for _ in range(2)]
+    return PagedKv(be, hq, hk, hs, page, n_pages, dtype, **kw), PagedLayer(*pages, hk * page * hs, page * hs, hs)
+
+
+def test_a_handle_is_used_in_its_own_context(be):
+    """Its calls run on its context's stream, which another context's buffers are not ordered with."""
+    other = NoGpu()
+    kv, layer = cache(other)
+    kv.step([3], [1], np.zeros((1, 1), np.int32))
+    x = [GpuVector(be, 4 * 64) for _ in range(5)]
+    refused(_lib.ERR_INVALID_ARG, "another context", LlmContext(be).paged_attention, kv, layer, x[0], x[1])
+    refused(_lib.ERR_INVALID_ARG, "another context", LlmContext(be).paged_append, kv, layer, QkNormRope(64, 4, 2), *x[:4])
+    for b in (be, other):
+        assert not b.lib.named("slai_paged_attention") and not b.lib.named("slai_paged_append")
+    ctx = LlmContext(other)
+    ctx.paged_attention(kv, layer, x[0], x[1])
+    ctx.paged_append(kv, layer, QkNormRope(64, 4, 2), *x[:4])
+    assert len(other.lib.named("slai_paged_attention")) == len(other.lib.named("slai_paged_append")) == 1
