@@ -14,10 +14,14 @@ import numpy as np
 from . import _lib
 from ._lib import (AttnParams, SlaiError, FMT_F32, FMT_Q8_0, FMT_Q4_K, FMT_Q5_K, FMT_Q6_K, KV_F16, KV_F32)
 
+_F32, _I32 = np.dtype(np.float32), np.dtype(np.int32)
+
 
 class Backend:
     """The `B: Backend` of slang-hal as the decode path uses it: buffers, `write_buffer`, `read_buffer`,
     `synchronize` (call sites: crates/slai-chat/src/chat_llama2.rs:180-230).  One CUDA stream per backend."""
+
+    _recording = False  # between a RecordedPass's enter and exit
 
     def __init__(self, device: int = 0):
         self.lib = _lib.load()
@@ -320,6 +324,7 @@ class PagedKv:
         self.n_q_heads, self.n_kv_heads, self.head_size, self.page_size, self.n_pages = n_q_heads, n_kv_heads, head_size, page_size, n_pages
         self.kv_dtype, self.max_tokens, self.width = kv_dtype, max_tokens, n_q_heads * head_size
         self.kv_bytes = 2 if kv_dtype == KV_F16 else 4
+        self.last = (n_pages - 1, n_kv_heads - 1, page_size - 1, head_size)  # the last element's place, by a layer's strides
         self.rows = None  # of the current step
         cfg = _lib.PagedConfig(n_q_heads, n_kv_heads, head_size, page_size, n_pages, kv_dtype, max_seqs, max_tokens, max_table or max(1, n_pages))
         h = C.c_void_p()
@@ -338,14 +343,15 @@ class PagedKv:
         self.rows = int(n_new.sum())
 
     def check_layer(self, layer: PagedLayer):
+        pages, heads, positions, size = self.last
         page, head, pos = layer.strides
-        need = (self.n_pages - 1) * page + (self.n_kv_heads - 1) * head + (self.page_size - 1) * pos + self.head_size
+        need = pages * page + heads * head + positions * pos + size
         if layer.elements < need or layer.nbytes < self.kv_bytes * need:
             raise SlaiError(_lib.ERR_SHAPE, f"paged: pages of {layer.elements} elements in {layer.nbytes} bytes, {need} elements of {self.kv_bytes} needed")
 
     def rows_in_use(self):
         """Rows that a call's buffers hold: the step's, or, for a call that is recorded and replayed for other steps, the most that a step can have."""
-        return self.max_tokens if getattr(self.backend, "_recording", False) else self.rows
+        return self.max_tokens if self.backend._recording else self.rows
 
     def __del__(self):
         try:
@@ -366,8 +372,8 @@ class QkNormRope:
     def __init__(self, head_size: int, n_q_heads: int, n_kv_heads: int, variant: RoPEVariant | None = RoPEVariant.Original, base_freq: float = 10000.0,
                  eps: float = 1e-5, q_norm=None, k_norm=None, q_ld: int = 0, k_ld: int = 0, v_ld: int = 0, q_out_ld: int = 0, k_out_ld: int = 0):
         for w in (q_norm, k_norm):
-            if w is not None and len(w) != head_size:
-                raise SlaiError(_lib.ERR_SHAPE, f"qk: {len(w)} norm weights for heads of {head_size}")
+            if w is not None and (len(w) != head_size or getattr(w, "dtype", _F32) != _F32):
+                raise SlaiError(_lib.ERR_SHAPE, f"qk: {len(w)} norm weights of {getattr(w, 'dtype', _F32)} for heads of {head_size} floats")
         self.norms = (q_norm, k_norm)  # held
         self.q_width, self.k_width = n_q_heads * head_size, n_kv_heads * head_size
         self.q_ld, self.k_ld, self.v_ld = q_ld or self.q_width, k_ld or self.k_width, v_ld or self.k_width
@@ -375,6 +381,7 @@ class QkNormRope:
         self.c = _lib.QkParams(head_size, n_q_heads, n_kv_heads, -1 if variant is None else int(variant), base_freq, eps, _ptr(q_norm).value,
                                _ptr(k_norm).value, q_ld, k_ld, v_ld, q_out_ld, k_out_ld)
         self.at = C.addressof(self.c)
+        self.rows = (self.q_width, self.k_width, self.q_ld, self.k_ld, self.v_ld, self.q_out_ld, self.k_out_ld)
 
 
 def _refuse_context():
@@ -382,6 +389,10 @@ def _refuse_context():
 
 
 def _refuse_rows(what: str, x, rows: int, width: int, ld: int):
+    if x is not None and len(x) >= (rows - 1) * (ld or width) + width:
+        if x.dtype == _F32:  # (a type of its own that says it is f32)
+            return
+        raise SlaiError(_lib.ERR_SHAPE, f"{what}: rows are floats, not {x.dtype}")
     raise SlaiError(_lib.ERR_SHAPE, f"{what}: {0 if x is None else len(x)} floats for {rows} rows of {width}, {ld or width} apart")
 
 
@@ -486,18 +497,20 @@ class LlmContext:
     def qk_norm_rope(self, how: QkNormRope, positions, q, k, q_out, k_out):
         """Norm and rotation of the rows of q and k, token t at position positions[t] (int32 on the device; negative: left as it is)."""
         n = len(positions)
+        if getattr(positions, "dtype", _I32) is not _I32 and np.dtype(positions.dtype).itemsize != 4:
+            raise SlaiError(_lib.ERR_SHAPE, f"qk_norm_rope: positions are int32 numbers, not {positions.dtype}")
         if n > 0:
-            m, w, k_w = n - 1, how.q_width, how.k_width
+            m, f, (w, k_w, q_ld, k_ld, _, q_out_ld, k_out_ld) = n - 1, _F32, how.rows
             if w:
-                if q is None or len(q) < m * how.q_ld + w:
-                    _refuse_rows("qk_norm_rope: q", q, n, w, how.q_ld)
-                if q_out is None or len(q_out) < m * how.q_out_ld + w:
-                    _refuse_rows("qk_norm_rope: q_out", q_out, n, w, how.q_out_ld)
+                if q is None or len(q) < m * q_ld + w or getattr(q, "dtype", f) is not f:
+                    _refuse_rows("qk_norm_rope: q", q, n, w, q_ld)
+                if q_out is None or len(q_out) < m * q_out_ld + w or getattr(q_out, "dtype", f) is not f:
+                    _refuse_rows("qk_norm_rope: q_out", q_out, n, w, q_out_ld)
             if k_w:
-                if k is None or len(k) < m * how.k_ld + k_w:
-                    _refuse_rows("qk_norm_rope: k", k, n, k_w, how.k_ld)
-                if k_out is None or len(k_out) < m * how.k_out_ld + k_w:
-                    _refuse_rows("qk_norm_rope: k_out", k_out, n, k_w, how.k_out_ld)
+                if k is None or len(k) < m * k_ld + k_w or getattr(k, "dtype", f) is not f:
+                    _refuse_rows("qk_norm_rope: k", k, n, k_w, k_ld)
+                if k_out is None or len(k_out) < m * k_out_ld + k_w or getattr(k_out, "dtype", f) is not f:
+                    _refuse_rows("qk_norm_rope: k_out", k_out, n, k_w, k_out_ld)
         rc = self.lib.slai_qk_norm_rope(self.h, how.at, n, positions.ptr, None if q is None else q.ptr, None if k is None else k.ptr,
                                         None if q_out is None else q_out.ptr, None if k_out is None else k_out.ptr)
         if rc:
@@ -510,16 +523,16 @@ class LlmContext:
         paged.check_layer(layer)
         n = paged.rows_in_use()
         if n:
-            m, w, k_w = n - 1, how.q_width, how.k_width
+            m, f, (w, k_w, q_ld, k_ld, v_ld, q_out_ld, _) = n - 1, _F32, how.rows
             if w:
-                if q is None or len(q) < m * how.q_ld + w:
-                    _refuse_rows("paged_append: q", q, n, w, how.q_ld)
-                if q_out is None or len(q_out) < m * how.q_out_ld + w:
-                    _refuse_rows("paged_append: q_out", q_out, n, w, how.q_out_ld)
-            if k is None or len(k) < m * how.k_ld + k_w:
-                _refuse_rows("paged_append: k", k, n, k_w, how.k_ld)
-            if v is None or len(v) < m * how.v_ld + k_w:
-                _refuse_rows("paged_append: v", v, n, k_w, how.v_ld)
+                if q is None or len(q) < m * q_ld + w or getattr(q, "dtype", f) is not f:
+                    _refuse_rows("paged_append: q", q, n, w, q_ld)
+                if q_out is None or len(q_out) < m * q_out_ld + w or getattr(q_out, "dtype", f) is not f:
+                    _refuse_rows("paged_append: q_out", q_out, n, w, q_out_ld)
+            if k is None or len(k) < m * k_ld + k_w or getattr(k, "dtype", f) is not f:
+                _refuse_rows("paged_append: k", k, n, k_w, k_ld)
+            if v is None or len(v) < m * v_ld + k_w or getattr(v, "dtype", f) is not f:
+                _refuse_rows("paged_append: v", v, n, k_w, v_ld)
         rc = self.lib.slai_paged_append(paged.h, layer.at, how.at, None if q is None else q.ptr, None if k is None else k.ptr, None if v is None else v.ptr,
                                         None if q_out is None else q_out.ptr)
         if rc:
@@ -532,9 +545,9 @@ class LlmContext:
         paged.check_layer(layer)
         n, width = paged.rows_in_use(), paged.width
         if n:
-            if len(q) < (n - 1) * (q_ld or width) + width:
+            if len(q) < (n - 1) * (q_ld or width) + width or getattr(q, "dtype", _F32) is not _F32:
                 _refuse_rows("paged_attention: q", q, n, width, q_ld)
-            if len(out) < (n - 1) * (out_ld or width) + width:
+            if len(out) < (n - 1) * (out_ld or width) + width or getattr(out, "dtype", _F32) is not _F32:
                 _refuse_rows("paged_attention: out", out, n, width, out_ld)
         rc = self.lib.slai_paged_attention(paged.h, layer.at, q.ptr, q_ld, scale, out.ptr, out_ld)
         if rc:

@@ -83,3 +83,46 @@ def test_a_handle_is_used_in_its_own_context(be):
     ctx.paged_attention(kv, layer, x[0], x[1])
     ctx.paged_append(kv, layer, QkNormRope(64, 4, 2), *x[:4])
     assert len(other.lib.named("slai_paged_attention")) == len(other.lib.named("slai_paged_append")) == 1
+
+
+@pytest.mark.parametrize("wrong", [np.float16, np.uint8, np.float64, np.int32])
+def test_rows_of_another_type_are_refused(be, wrong):
+    """Enough elements, but not of four bytes: the kernels would read and write behind them.  (Those of four or more bytes would be read as what they are not.)"""
+    ctx, S = LlmContext(be), _lib.ERR_SHAPE
+    kv, layer = cache(be)
+    kv.step([3, 2], [1, 1], np.array([[0], [1]], np.int32))
+    f = lambda heads: GpuVector(be, 2 * heads * 64)  # noqa: E731
+    bad = lambda heads: GpuVector(be, 2 * heads * 64, wrong)  # noqa: E731
+    how, pos = QkNormRope(64, 4, 2), GpuVector(be, 2, np.int32)
+    for i in range(4):
+        x = [f(4), f(2), f(4), f(2)]
+        x[i] = bad(4 if i % 2 == 0 else 2)
+        refused(S, "rows are floats, not " + np.dtype(wrong).name, ctx.qk_norm_rope, how, pos, *x)
+        x = [f(4), f(2), f(2), f(4)]
+        x[i] = bad(4 if i in (0, 3) else 2)
+        refused(S, "rows are floats, not " + np.dtype(wrong).name, ctx.paged_append, kv, layer, how, *x)
+    refused(S, "rows are floats", ctx.paged_attention, kv, layer, bad(4), f(4))
+    refused(S, "rows are floats", ctx.paged_attention, kv, layer, f(4), bad(4).view(0, 512))
+    refused(S, "norm weights", QkNormRope, 64, 4, 2, q_norm=GpuVector(be, 64, wrong))
+    if np.dtype(wrong).itemsize != 4:
+        refused(S, "positions are int32", ctx.qk_norm_rope, how, GpuVector(be, 2, wrong), f(4), f(2), f(4), f(2))
+    assert not [n for n, _ in be.lib.calls if n in ("slai_qk_norm_rope", "slai_paged_append", "slai_paged_attention")]
+
+
+def test_rows_of_a_type_of_ones_own(be):
+    """Anything with a device pointer and a length; where it names its elements' type, that is f32 in any of its spellings."""
+    class Mine:
+        def __init__(self, n, **kw):
+            self.ptr, self.n = 4096, n
+            self.__dict__.update(kw)
+
+        def __len__(self):
+            return self.n
+
+    ctx = LlmContext(be)
+    kv, layer = cache(be)
+    kv.step([3], [1], np.zeros((1, 1), np.int32))
+    for kw in ({}, dict(dtype=np.float32), dict(dtype="float32"), dict(dtype=np.dtype("<f4"))):
+        ctx.paged_attention(kv, layer, Mine(256, **kw), Mine(256, **kw))
+        ctx.qk_norm_rope(QkNormRope(64, 4, 2), Mine(1), Mine(256, **kw), Mine(128, **kw), Mine(256, **kw), Mine(128, **kw))
+    assert len(be.lib.named("slai_paged_attention")) == len(be.lib.named("slai_qk_norm_rope")) == 4
