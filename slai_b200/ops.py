@@ -302,6 +302,21 @@ class BatchedMultiqueryAttentionParams:
         return AttnParams(self.seq_len, self.kv_dim, self.kv_mul, self.n_heads, self.head_size, self.pos)
 
 
+def _int32(what: str, x) -> np.ndarray:
+    """x as int32 numbers, if that is what they are: numpy cuts off what does not fit."""
+    a = np.asarray(x)
+    if a.dtype == _I32:
+        return np.ascontiguousarray(a)
+    try:
+        with np.errstate(invalid="ignore"):
+            b = np.ascontiguousarray(a, dtype=_I32)
+        if (b == a).all():
+            return b
+    except (OverflowError, TypeError, ValueError):
+        pass
+    raise SlaiError(_lib.ERR_SHAPE, f"paged step: {what} are not int32 numbers")
+
+
 class PagedLayer:
     """A layer's pages (`slai_paged_layer`): key and value buffers and the strides, in elements, between pages, cache heads and positions."""
 
@@ -333,8 +348,7 @@ class PagedKv:
 
     def step(self, pos0, n_new, tables):
         """Sequence b: `pos0[b]` cached positions, `n_new[b]` new tokens behind them, pages `tables[b]` in order of their positions."""
-        pos0, n_new = np.ascontiguousarray(pos0, dtype=np.int32), np.ascontiguousarray(n_new, dtype=np.int32)
-        tables = np.ascontiguousarray(tables, dtype=np.int32)
+        pos0, n_new, tables = _int32("pos0", pos0), _int32("n_new", n_new), _int32("tables", tables)
         n = pos0.size
         if pos0.ndim != 1 or n_new.shape != pos0.shape or tables.ndim != 2 or tables.shape[0] != n:
             raise SlaiError(_lib.ERR_SHAPE, f"paged step: lengths of {pos0.shape}, {n_new.shape} and tables of {tables.shape}")

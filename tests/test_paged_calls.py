@@ -126,3 +126,27 @@ def test_rows_of_a_type_of_ones_own(be):
         ctx.paged_attention(kv, layer, Mine(256, **kw), Mine(256, **kw))
         ctx.qk_norm_rope(QkNormRope(64, 4, 2), Mine(1), Mine(256, **kw), Mine(128, **kw), Mine(256, **kw), Mine(128, **kw))
     assert len(be.lib.named("slai_paged_attention")) == len(be.lib.named("slai_qk_norm_rope")) == 4
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("wrong", [1 << 31, (1 << 32) + 1, -(1 << 31) - 1, 1 << 64, 1.5, float("nan"), float("inf"), None, "a"])
+def test_lengths_and_tables_that_are_no_int32_numbers(be, which, wrong):
+    """... are refused, not cut to 32 bits: 2^32 + 1 would name page 1."""
+    kv, _ = cache(be)
+    args = [[3, 2], [1, 1], [[0], [1]]]
+    for t in (np.int64, np.int32, np.uint16, np.float64):
+        kv.step(*(np.array(a, t) for a in args))
+    kv.step(*args)
+    kv.step([], [], np.zeros((0, 3)))  # nobody takes part
+    kv.step(np.array([1]), np.array([1]), np.zeros((1, 0), np.int64))  # (the library refuses a table that is too narrow)
+    done = len(be.lib.named("slai_paged_step"))
+    assert done == 7 and be.lib.named("slai_paged_step")[0][1] == 2
+    if which == 2:
+        args[2][1][0] = wrong
+    else:
+        args[which][1] = wrong
+    refused(_lib.ERR_SHAPE, "int32", kv.step, *args)
+    assert len(be.lib.named("slai_paged_step")) == done and kv.rows == 1
+    if isinstance(wrong, int) and wrong < 1 << 62:
+        args[which] = np.array(args[which], np.int64)
+        refused(_lib.ERR_SHAPE, "int32", kv.step, *args)
