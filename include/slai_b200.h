@@ -281,7 +281,7 @@ int slai_kv_append(slai_ctx* ctx, void* d_key_cache, void* d_value_cache, int kv
 typedef struct slai_paged_config {
     int32_t n_q_heads, n_kv_heads, head_size; /* n_kv_heads divides n_q_heads; head_size 1 .. 256 */
     int32_t page_size, n_pages, kv_dtype;     /* slai_kv_dtype */
-    int32_t max_seqs, max_tokens, max_table;  /* capacity of a step: sequences, new tokens, table entries in use */
+    int32_t max_seqs, max_tokens, max_table;  /* capacity of a step: sequences, new tokens, table entries in use (a shared page: one for each of its sequences) */
 } slai_paged_config;
 /* A layer's pages.  Element e of cache head h at place s of page p is d_keys[p * page_stride + h * head_stride + s * pos_stride + e]; strides in
  * elements, each at least head_size: position-major pages as in the reference's cache, head-major ones, or anything between. */

@@ -331,7 +331,10 @@ class PagedLayer:
 
 class PagedKv:
     """Keys and values of many sequences in pages (`slai_paged`): what a model's layers have in common, and the current step.  The reference's cache is
-    one dense tensor of one sequence (crates/slai/src/models/llama2/transformer.rs:87-106)."""
+    one dense tensor of one sequence (crates/slai/src/models/llama2/transformer.rs:87-106).
+
+    max_table: table entries of a step, a page that several sequences share counting for each of them.  None: every sequence may use every page, up to 2^20 entries
+    in all (4 MB on the device, 8 MB of pinned memory), or each page once where there are more pages than that."""
 
     def __init__(self, backend: Backend, n_q_heads: int, n_kv_heads: int, head_size: int, page_size: int, n_pages: int, kv_dtype: int = KV_F16,
                  max_seqs: int = 8, max_tokens: int = 512, max_table: int | None = None):
@@ -341,7 +344,7 @@ class PagedKv:
         self.kv_bytes = 2 if kv_dtype == KV_F16 else 4
         self.last = (n_pages - 1, n_kv_heads - 1, page_size - 1, head_size)  # the last element's place, by a layer's strides
         self.rows = None  # of the current step
-        cfg = _lib.PagedConfig(n_q_heads, n_kv_heads, head_size, page_size, n_pages, kv_dtype, max_seqs, max_tokens, max_table or max(1, n_pages))
+        cfg = _lib.PagedConfig(n_q_heads, n_kv_heads, head_size, page_size, n_pages, kv_dtype, max_seqs, max_tokens, max_table or max(n_pages, min(n_pages * max_seqs, 1 << 20)))
         h = C.c_void_p()
         backend.check(backend.lib.slai_paged_create(backend.h, C.byref(cfg), C.byref(h)))
         self.h = h

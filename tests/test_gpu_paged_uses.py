@@ -6,7 +6,7 @@ import pytest
 
 from slai_b200 import _lib
 from slai_b200._lib import KV_F16, KV_F32
-from slai_b200.ops import QkNormRope
+from slai_b200.ops import PagedKv, QkNormRope
 from test_gpu_paged import Pages, attend, refused
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +63,12 @@ def test_a_handle_is_not_destroyed_while_a_pass_is_recorded(ctx, backend):
     backend.synchronize()
     rec.close()
     attend(ctx, P, [39, 19], [1, 1])
+
+
+def test_a_shared_prefix_longer_than_the_pages_there_are(ctx, backend):
+    """Eight sequences that share 12 pages of 28 use 112 table entries; a handle of the default size takes them."""
+    hq, hk, hs, page, seqs = 8, 2, 128, 16, 8
+    P = Pages(backend, hq, hk, hs, page, [14 * page - 3] * seqs, F16, seed=35)
+    P.tables[:, :12], P.tables[:, 12:] = np.arange(12)[::-1], 12 + np.arange(2 * seqs).reshape(seqs, 2)
+    P.kv = PagedKv(backend, hq, hk, hs, page, 28, F16, max_seqs=seqs, max_tokens=64)
+    attend(ctx, P, [13 * page + 5] * seqs, [8] * seqs)

@@ -150,3 +150,12 @@ def test_lengths_and_tables_that_are_no_int32_numbers(be, which, wrong):
     if isinstance(wrong, int) and wrong < 1 << 62:
         args[which] = np.array(args[which], np.int64)
         refused(_lib.ERR_SHAPE, "int32", kv.step, *args)
+
+
+@pytest.mark.parametrize("n_pages, max_seqs, want", [(100, 8, 800), (1, 1, 1), (1 << 16, 64, 1 << 20), (1 << 21, 4, 1 << 21), (0, 8, 0), (-3, 8, -3), (1 << 28, 1 << 20, 1 << 28)])
+def test_tables_have_room_for_pages_that_sequences_share(be, n_pages, max_seqs, want):
+    """(What is no number of pages goes on to the library, which refuses it.)"""
+    PagedKv(be, 4, 2, 64, 1, n_pages, max_seqs=max_seqs)
+    assert be.lib.named("slai_paged_create")[-1][1]._obj.max_table == want
+    PagedKv(be, 4, 2, 64, 1, n_pages, max_seqs=max_seqs, max_table=7)
+    assert be.lib.named("slai_paged_create")[-1][1]._obj.max_table == 7
