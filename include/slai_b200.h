@@ -297,7 +297,8 @@ int slai_paged_step(slai_paged* p, int n_seq, const int32_t* h_pos0, const int32
 /* What happens to q and k between their product and the attention.  Per head: RmsNorm (ops/rms_norm.rs:35-77) by `head_size` weights where they are given,
  * then the rotation of its pairs by the token's position (ops/rope.rs:45-85; -1 none, 0 Original, 1 Neox).  Angles keep their digits at any position (the
  * product is formed in 64 bits; slai_rope's in f32, as in the reference).  Leading dimensions: floats between the rows of two tokens, 0 = packed; q, k and v may
- * be parts of one product's rows.  An output may be its own input. */
+ * be parts of one product's rows.  An output may be its own input, with the same leading dimension; else it shares no float with an input or the other output
+ * (SLAI_ERR_INVALID_ARG). */
 typedef struct slai_qk_params {
     int32_t head_size, n_q_heads, n_kv_heads; /* head_size 1 .. 256, even with a rotation */
     int32_t rope_variant;
@@ -314,7 +315,7 @@ int slai_paged_append(slai_paged* p, const slai_paged_layer* layer, const slai_q
                       float* d_q_out);
 /* Causal attention (ops/batched_multiquery_attention.rs:32-156) of the step's tokens: token at position t attends to positions 0 .. t of its sequence, which
  * are in the pages by then.  Rows of q and out: n_q_heads * head_size floats, q_ld / out_ld apart (0 = packed); no element of
- * out is one of q's.  scale 0: 1 / sqrt(head_size).  Sums,
+ * out is one of q's (SLAI_ERR_INVALID_ARG).  scale 0: 1 / sqrt(head_size).  Sums,
  * weights and results are f32; f16 keys and values take part as they are cached.  Results do not depend on timing; their last bits may depend on what else is in the step and on whether the call is recorded. */
 int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, const float* d_q, int64_t q_ld, float scale, float* d_out, int64_t out_ld);
 

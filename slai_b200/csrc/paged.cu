@@ -5,6 +5,7 @@
 #include <exception>
 
 #include "paged.cuh"
+#include "row_overlap.h"
 
 using namespace paged;
 
@@ -150,6 +151,19 @@ int fill_qk(slai_ctx* ctx, const slai_qk_params* p, QkArgs& A) {
     return p->rope_variant < 0 ? (int)SLAI_OK : turn_table(ctx, p->head_size, p->rope_base_freq, &A.turns);
 }
 
+// Heads are written while others are still read: a result's rows are its own input's, or share no float with any.
+struct Rows {
+    const char* name;
+    const float* at;
+    int64_t ld, w;
+};
+int check_apart(slai_ctx* ctx, const char* call, const Rows& out, const Rows& in, bool in_place, int64_t n) {
+    if (in_place && out.at == in.at && (out.ld == in.ld || n <= 1)) return SLAI_OK;
+    SLAI_REQUIRE(ctx, !rows_overlap((uintptr_t)out.at, out.ld, out.w, (uintptr_t)in.at, in.ld, in.w, n), SLAI_ERR_INVALID_ARG,
+                 "%s: %s (rows %lld apart) shares floats with %s (rows %lld apart)", call, out.name, (long long)out.ld, in.name, (long long)in.ld);
+    return SLAI_OK;
+}
+
 }  // namespace
 
 SLAI_API int slai_paged_create(slai_ctx* ctx, const slai_paged_config* cfg, slai_paged** out) {
@@ -225,6 +239,14 @@ SLAI_API int slai_qk_norm_rope(slai_ctx* ctx, const slai_qk_params* params, int 
     const int rc = fill_qk(ctx, params, A);
     if (rc || n_tokens == 0) return rc;
     SLAI_REQUIRE(ctx, d_pos && (A.n_q == 0 || (d_q && d_q_out)) && (A.n_kv == 0 || (d_k && d_k_out)), SLAI_ERR_INVALID_ARG, "qk: rows or positions are missing");
+    const int64_t qw = (int64_t)A.n_q * A.hs, kw = (int64_t)A.n_kv * A.hs;
+    const Rows q = {"q", d_q, A.q_ld, qw}, k = {"k", d_k, A.k_ld, kw}, qo = {"q_out", d_q_out, A.q_out_ld, qw}, ko = {"k_out", d_k_out, A.k_out_ld, kw};
+    int bad = check_apart(ctx, "qk", qo, q, true, n_tokens);
+    if (!bad) bad = check_apart(ctx, "qk", ko, k, true, n_tokens);
+    if (!bad) bad = check_apart(ctx, "qk", qo, k, false, n_tokens);
+    if (!bad) bad = check_apart(ctx, "qk", ko, q, false, n_tokens);
+    if (!bad) bad = check_apart(ctx, "qk", qo, ko, false, n_tokens);
+    if (bad) return bad;
     A.rows = n_tokens;
     A.pos = d_pos;
     A.q = d_q; A.k = d_k; A.q_out = d_q_out; A.k_out = d_k_out;
@@ -252,6 +274,11 @@ SLAI_API int slai_paged_append(slai_paged* p, const slai_paged_layer* layer, con
         A.rows = p->cfg.max_tokens;
         A.counted = 1;
     }
+    const int64_t qw = (int64_t)A.n_q * A.hs, kw = (int64_t)A.n_kv * A.hs;
+    const Rows qo = {"q_out", d_q_out, A.q_out_ld, qw};
+    if ((rc = check_apart(ctx, "paged append", qo, {"q", d_q, A.q_ld, qw}, true, A.rows))) return rc;
+    if ((rc = check_apart(ctx, "paged append", qo, {"k", d_k, A.k_ld, kw}, false, A.rows))) return rc;
+    if ((rc = check_apart(ctx, "paged append", qo, {"v", d_v, A.v_ld, kw}, false, A.rows))) return rc;
     return qk_launch(ctx, A, ctx->use_pdl);
 }
 
@@ -270,6 +297,8 @@ SLAI_API int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, 
                  (long long)A.out_ld, (long long)row);
     SLAI_REQUIRE(ctx, isfinite(scale), SLAI_ERR_INVALID_ARG, "paged attention: scale %g", (double)scale);
     SLAI_REQUIRE(ctx, d_q != d_out, SLAI_ERR_INVALID_ARG, "paged attention: queries are read while results are written, out cannot be q");
+    const bool recording = capturing(ctx);
+    if ((rc = check_apart(ctx, "paged attention", {"out", d_out, A.out_ld, row}, {"q", d_q, A.q_ld, row}, false, recording ? c.max_tokens : p->step.n_rows))) return rc;
     A.scale = scale == 0.f ? (float)(1.0 / sqrt((double)c.head_size)) : scale;
     A.q = d_q;
     A.out = d_out;
@@ -281,7 +310,6 @@ SLAI_API int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, 
     A.qvec = (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)(A.q_ld * 4) | (uintptr_t)(A.out_ld * 4) | (uintptr_t)(c.head_size * 4)) & 15) == 0;
     A.err_flag = ctx->d_counters + CNT_ERR_FLAG;
     A.wait_limit = ctx->wait_limit;
-    const bool recording = capturing(ctx);
     if (recording && (rc = slai_keep_for_pass(ctx, p->dev))) return rc;
     A.recorded = recording;
     for (int k = 0; k < 2; k++) {

@@ -4,10 +4,11 @@ import gc
 import numpy as np
 import pytest
 
+import paged_reference as R
 from slai_b200 import _lib
 from slai_b200._lib import KV_F16, KV_F32
 from slai_b200.ops import PagedKv, QkNormRope
-from test_gpu_paged import Pages, attend, refused
+from test_gpu_paged import Pages, attend, check, refused
 
 pytestmark = pytest.mark.gpu
 F16, F32 = KV_F16, KV_F32
@@ -72,3 +73,46 @@ def test_a_shared_prefix_longer_than_the_pages_there_are(ctx, backend):
     P.tables[:, :12], P.tables[:, 12:] = np.arange(12)[::-1], 12 + np.arange(2 * seqs).reshape(seqs, 2)
     P.kv = PagedKv(backend, hq, hk, hs, page, 28, F16, max_seqs=seqs, max_tokens=64)
     attend(ctx, P, [13 * page + 5] * seqs, [8] * seqs)
+
+
+def test_results_that_share_floats_with_what_is_still_read(ctx, backend):
+    """In place with the same leading dimension; refused otherwise, however the rows come to overlap."""
+    I, hq, hk, hs, T = _lib.ERR_INVALID_ARG, 4, 2, 64, 20
+    ld = (hq + 2 * hk) * hs
+    rng = np.random.default_rng(36)
+    x = rng.standard_normal((T + 4, ld)).astype(np.float32)
+    pos = backend.vector(np.arange(T), np.int32)
+    buf, apart = backend.vector(x), [backend.zeros(T * hq * hs) for _ in range(2)]
+    part = lambda at, n: buf.view(at, (T - 1) * ld + n * hs)  # noqa: E731
+    q, k, v = part(0, hq), part(hq * hs, hk), part((hq + hk) * hs, hk)
+    how = lambda **kw: QkNormRope(hs, hq, hk, 1, q_ld=ld, k_ld=ld, v_ld=ld, **kw)  # noqa: E731
+    whole = buf.view(0, buf.n)
+    refused(I, "q_out .* shares floats with q ", ctx.qk_norm_rope, how(k_out_ld=ld), pos, q, k, whole, k)             # in place, but packed
+    refused(I, "k_out .* shares floats with k ", ctx.qk_norm_rope, how(q_out_ld=ld), pos, q, k, q, buf.view(hq * hs, buf.n - hq * hs))
+    refused(I, "q_out .* shares floats with k ", ctx.qk_norm_rope, how(q_out_ld=ld), pos, q, k, part(hq * hs, hq), apart[1])
+    refused(I, "q_out .* shares floats with k_out", ctx.qk_norm_rope, how(), pos, q, k, apart[0], apart[0])
+    refused(I, "k_out .* shares floats with q ", ctx.qk_norm_rope, how(k_out_ld=ld), pos, q, k, apart[0], part(hs, hk))
+    refused(I, "q_out .* shares floats with q ", ctx.qk_norm_rope, how(q_out_ld=ld), pos, q, k, part(ld, hq), apart[1])  # a row further on
+    P = Pages(backend, hq, hk, hs, 16, [T], F32, max_tokens=T)
+    P.kv.step([0], [T], P.tables)
+    refused(I, "q_out .* shares floats with q ", ctx.paged_append, P.kv, P.layer, how(), q, k, v, whole)
+    refused(I, "q_out .* shares floats with k ", ctx.paged_append, P.kv, P.layer, how(q_out_ld=ld), q, k, v, part(hq * hs, hq))
+    refused(I, "q_out .* shares floats with v", ctx.paged_append, P.kv, P.layer, QkNormRope(hs, hq, hk, 1, v_ld=ld, q_out_ld=ld), apart[0], apart[1], v, part((hq + hk - 1) * hs, hq))
+    refused(I, "out .* shares floats with q", ctx.paged_attention, P.kv, P.layer, q, part(hs, hq), 0.0, ld, ld)
+    refused(I, "out .* shares floats with q", ctx.paged_attention, P.kv, P.layer, q, part(ld, hq), 0.0, ld, ld)
+    refused(I, "out .* shares floats with q", ctx.paged_attention, P.kv, P.layer, q, buf.view(hs, buf.n - hs), 0.0, ld, 0)
+    assert np.array_equal(buf.to_numpy().reshape(x.shape), x)
+    # what shares nothing is taken: results between the queries' rows
+    P.host[0][:], P.host[1][:] = rng.standard_normal(P.host[0].size), rng.standard_normal(P.host[0].size)
+    P.upload()
+    ctx.paged_attention(P.kv, P.layer, q, part(hq * hs, hq), 0.0, ld, ld)
+    got = buf.to_numpy().reshape(x.shape)
+    want, bound = R.attention(x[:T, :hq * hs].reshape(T, hq, hs), P.at(0, 0, np.arange(T)), P.at(1, 0, np.arange(T)), 0, hs**-0.5)
+    check(got[:T, hq * hs:].reshape(T, hq, hs), want, bound)
+    assert np.array_equal(got[:, :hq * hs], x[:, :hq * hs]) and np.array_equal(got[T:], x[T:])
+    # one token's row has no next: in place and packed are the same
+    one = backend.vector(x[0])
+    at = lambda h, n: one.view(h * hs, n * hs)  # noqa: E731
+    ctx.qk_norm_rope(how(), backend.vector([5], np.int32), at(0, hq), at(hq, hk), at(0, hq), at(hq, hk))
+    want, bound = R.norm_rope(x[:1, :(hq + hk) * hs].reshape(1, hq + hk, hs), None, 0, 1, 10000.0, [5])
+    check(one.to_numpy()[:(hq + hk) * hs].reshape(want.shape), want, bound)
