@@ -284,7 +284,8 @@ typedef struct slai_paged_config {
     int32_t max_seqs, max_tokens, max_table;  /* capacity of a step: sequences, new tokens, table entries in use (a shared page: one for each of its sequences) */
 } slai_paged_config;
 /* A layer's pages.  Element e of cache head h at place s of page p is d_keys[p * page_stride + h * head_stride + s * pos_stride + e]; strides in
- * elements, each at least head_size: position-major pages as in the reference's cache, head-major ones, or anything between. */
+ * elements, each at least head_size: position-major pages as in the reference's cache, head-major ones, or anything between.  Whatever is written through them
+ * (slai_paged_append) has a row for every page, head and place: sorted, each stride covers what lies within it (SLAI_ERR_SHAPE). */
 typedef struct slai_paged_layer {
     void* d_keys;
     void* d_values;

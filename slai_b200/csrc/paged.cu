@@ -261,6 +261,9 @@ SLAI_API int slai_paged_append(slai_paged* p, const slai_paged_layer* layer, con
     QkArgs A = {};
     int rc = fill_cache(p, layer, &A.cache);
     if (rc) return rc;
+    SLAI_REQUIRE(ctx, rows_apart(p->cfg, layer->page_stride, layer->head_stride, layer->pos_stride), SLAI_ERR_SHAPE,
+                 "paged append: by strides of %lld, %lld and %lld (page, head, position) rows of %d elements lie on one another", (long long)layer->page_stride,
+                 (long long)layer->head_stride, (long long)layer->pos_stride, p->cfg.head_size);
     SLAI_REQUIRE(ctx, params->head_size == p->cfg.head_size && params->n_kv_heads == p->cfg.n_kv_heads && (params->n_q_heads == p->cfg.n_q_heads || params->n_q_heads == 0),
                  SLAI_ERR_SHAPE, "paged append: heads of %d, %d on %d, are not the cache's (%d, %d on %d)", params->head_size, params->n_q_heads, params->n_kv_heads,
                  p->cfg.head_size, p->cfg.n_q_heads, p->cfg.n_kv_heads);

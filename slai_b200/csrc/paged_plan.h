@@ -133,6 +133,22 @@ inline std::string check_config(const Config& c) {
     return "";
 }
 
+// Whether a layer's strides give every (page, cache head, place) a row of its own: whichever of the three moves least moves by a row at least, the next by all that
+// lies within, the last by all that lies within those.
+inline bool rows_apart(const Config& c, int64_t page_stride, int64_t head_stride, int64_t pos_stride) {
+    struct Dim {
+        int64_t stride, n;
+    } d[3] = {{page_stride, c.n_pages}, {head_stride, c.n_kv_heads}, {pos_stride, c.page_size}};
+    std::sort(d, d + 3, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+    __int128 span = c.head_size;  // from a row's first element to the last of all that lie within
+    for (const Dim& x : d) {
+        if (x.n == 1) continue;
+        if (x.stride < span) return false;
+        span += (__int128)(x.n - 1) * x.stride;
+    }
+    return true;
+}
+
 class Planner {
   public:
     // Sequences of up to `few` rows (tokens * group) go to lane 0, of more than `most` to lane 1 (it may be absent, blocks 0); those between to where the step

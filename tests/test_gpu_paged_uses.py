@@ -7,7 +7,7 @@ import pytest
 import paged_reference as R
 from slai_b200 import _lib
 from slai_b200._lib import KV_F16, KV_F32
-from slai_b200.ops import PagedKv, QkNormRope
+from slai_b200.ops import PagedKv, PagedLayer, QkNormRope
 from test_gpu_paged import Pages, attend, check, refused
 
 pytestmark = pytest.mark.gpu
@@ -116,3 +116,20 @@ def test_results_that_share_floats_with_what_is_still_read(ctx, backend):
     ctx.qk_norm_rope(how(), backend.vector([5], np.int32), at(0, hq), at(hq, hk), at(0, hq), at(hq, hk))
     want, bound = R.norm_rope(x[:1, :(hq + hk) * hs].reshape(1, hq + hk, hs), None, 0, 1, 10000.0, [5])
     check(one.to_numpy()[:(hq + hk) * hs].reshape(want.shape), want, bound)
+
+
+def test_an_append_through_strides_that_overlap(ctx, backend):
+    P = Pages(backend, 4, 2, 64, 16, [40, 20], F16)
+    P.kv.step([39, 19], [1, 1], P.tables)
+    x = [backend.zeros(2 * 4 * 64) for _ in range(4)]
+    large = [backend.zeros(4 * P.dev[0].n, np.float16) for _ in range(2)]  # (room for whatever the strides reach)
+    for strides in ((64, 64, 64), (2 * 16 * 64, 16 * 64, 16 * 64), (16 * 64, 16 * 64, 64), (2 * 16 * 64 - 1, 16 * 64, 64)):
+        refused(_lib.ERR_SHAPE, "lie on one another", ctx.paged_append, P.kv, PagedLayer(*large, *strides), QkNormRope(64, 4, 2), *x)
+    ctx.paged_append(P.kv, P.layer, QkNormRope(64, 4, 2), *x)
+    before = [h.copy() for h in P.host]
+    P.download()
+    for w in range(2):
+        assert not P.at(w, 0, [39]).any() and not P.at(w, 1, [19]).any()
+        P.put(w, 0, [39], before[w][P._index(0, [39])])
+        P.put(w, 1, [19], before[w][P._index(1, [19])])
+        assert np.array_equal(P.host[w], before[w])
