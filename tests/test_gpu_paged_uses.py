@@ -6,8 +6,8 @@ import pytest
 
 import paged_reference as R
 from slai_b200 import _lib
-from slai_b200._lib import KV_F16, KV_F32
-from slai_b200.ops import PagedKv, PagedLayer, QkNormRope
+from slai_b200._lib import KV_F16, KV_F32, SlaiError
+from slai_b200.ops import Backend, LlmContext, PagedKv, PagedLayer, QkNormRope
 from test_gpu_paged import Pages, attend, check, refused
 
 pytestmark = pytest.mark.gpu
@@ -133,3 +133,37 @@ def test_an_append_through_strides_that_overlap(ctx, backend):
         P.put(w, 0, [39], before[w][P._index(0, [39])])
         P.put(w, 1, [19], before[w][P._index(1, [19])])
         assert np.array_equal(P.host[w], before[w])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hs, page, pos0, n_new", [(128, 16, [7000], [300]), (128, 20, [300, 0], [100, 200]), (64, 64, [2000, 5], [150, 1])])
+def test_chunks_with_the_shortest_wait_limit(dtype, hs, page, pos0, n_new):
+    """16 rounds are enough for the waits inside a chunk's kernel (the prompt's products need more); one that took longer would be reported at the next synchronisation, once,
+    and go on until what it waits for is there.  Either way the bits are the same."""
+    be = Backend(0)
+    ctx = LlmContext(be)
+    P = Pages(be, 16, 4, hs, page, [p + n for p, n in zip(pos0, n_new)], dtype, seed=41)
+    q = be.vector(P.rng.standard_normal(sum(n_new) * 16 * hs))
+    out = be.zeros(q.n)
+    P.kv.step(pos0, n_new, P.tables)
+
+    def call():
+        be.write_buffer(out.ptr, np.full(out.n, 4.5, np.float32))
+        ctx.paged_attention(P.kv, P.layer, q, out)
+        be.synchronize()
+
+    call()
+    want = out.to_numpy()
+    be.set_wait_limit(16)
+    for _ in range(12):
+        try:
+            call()
+        except SlaiError as e:
+            assert e.code == _lib.ERR_TIMEOUT and "paged attention" in str(e)
+            be.synchronize()  # (reported once)
+        assert np.array_equal(out.to_numpy(), want)
+    be.set_wait_limit(1 << 20)
+    call()
+    assert np.array_equal(out.to_numpy(), want)
+    del P, q, out
+    be.close()
