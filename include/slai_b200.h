@@ -316,8 +316,12 @@ int slai_paged_append(slai_paged* p, const slai_paged_layer* layer, const slai_q
                       float* d_q_out);
 /* Causal attention (ops/batched_multiquery_attention.rs:32-156) of the step's tokens: token at position t attends to positions 0 .. t of its sequence, which
  * are in the pages by then.  Rows of q and out: n_q_heads * head_size floats, q_ld / out_ld apart (0 = packed); no element of
- * out is one of q's (SLAI_ERR_INVALID_ARG).  scale 0: 1 / sqrt(head_size).  Sums,
- * weights and results are f32; f16 keys and values take part as they are cached.  Results do not depend on timing; their last bits may depend on what else is in the step and on whether the call is recorded. */
+ * out is one of q's (SLAI_ERR_INVALID_ARG).  scale 0: 1 / sqrt(head_size).  Maxima,
+ * sums and results are f32.  What is multiplied: over f16 caches the keys and values as they are cached, queries (times the scale) and weights to 22 bits (pairs of halves; of
+ * a row's queries those below 2^-17 of its largest to 2^-40 of that).  Over f32 caches everything in f32 where a sequence has few rows (new tokens * query heads of a cache
+ * head: up to 4, or 8 where there are more than 4 such heads, and up to 128 where the step is sooner done so), else queries, keys, weights and values to 21 bits (pairs of
+ * tf32 numbers, the product of the low ones left out).  Heads that are no multiple of 8 (f32 caches: 4) or above 128, and pages off 16-byte boundaries: f32 throughout.
+ * Results do not depend on timing; their last bits may depend on what else is in the step and on whether the call is recorded. */
 int slai_paged_attention(slai_paged* p, const slai_paged_layer* layer, const float* d_q, int64_t q_ld, float scale, float* d_out, int64_t out_ld);
 
 /* ---- Llama-2 family: Llama2Config (models/llama2/cpu.rs:46-67), Llama2::launch (transformer.rs:316-381) */

@@ -556,7 +556,8 @@ class LlmContext:
             self.backend.check(rc)
 
     def paged_attention(self, paged: PagedKv, layer: PagedLayer, q, out, scale: float = 0.0, q_ld: int = 0, out_ld: int = 0):
-        """Causal attention of the step's tokens to what their sequences hold (scale 0: 1 / sqrt(head_size))."""
+        """Causal attention of the step's tokens to what their sequences hold (scale 0: 1 / sqrt(head_size)).  f32 sums; products of operands of 21 to 24 bits, by the
+        cache's type and the step: `slai_paged_attention`."""
         if paged.backend is not self.backend:
             _refuse_context()
         paged.check_layer(layer)
