@@ -1,4 +1,5 @@
-// Paged key / value cache: the handle with a step's plan, and the entry points of its operators (kernels: paged_append.cu, paged_attention.cu).
+// Paged key / value cache: the handle with a step's plan, and the entry points of its operators (kernels: paged_append.cu, paged_attention.cu,
+// paged_prompt.cu, paged_prompt32.cu).
 #include <math.h>
 #include <string.h>
 
@@ -11,8 +12,9 @@ using namespace paged;
 
 namespace {
 // Rows of a cache head that a sequence may bring and surely goes to the kernel for few rows, and may bring and perhaps does.  us of a call, kernel for few / for many:
-// one sequence at 300, 32 heads: 64 rows 9.7 / 17.4; at 3000, 32 rows 34 / 35, 64 rows 55 / 36; 64 heads on 8 at 3000, 64 rows 20 / 29, 128 rows 30 / 30; 16
-// sequences of 64 heads on 8 at 2000: 16 rows 43 / 56, 32 rows 87 / 56.
+// one sequence at 300, 32 heads: 64 rows 9.8 / 17.2; at 3000, 32 rows 34 / 34, 64 rows 56 / 35; 64 heads on 8 at 3000, 64 rows 20 / 27, 128 rows 30 / 28; 16
+// sequences of 64 heads on 8 at 2000: 16 rows 44 / 54, 32 rows 88 / 55.  (The planner's costs are older than the chunk kernel's last steps: of these it takes the slower
+// one for 64 rows of 64 heads on 8 at 3000.)
 constexpr int FEW_ROWS = 16, PERHAPS_ROWS = 128;
 constexpr int SLOTS = 2;  // pinned copies of a plan: the next step is planned while the last one's copy is on its way
 

@@ -114,9 +114,9 @@ __global__ void __launch_bounds__(QT) qk_any_kernel(const QkArgs A) {
 }
 
 // Heads of a multiple of 8 elements on 16-byte boundaries: LPH lanes take a head, 8 elements a lane (two 16-byte pieces that hold four whole pairs in either
-// variant), a warp 32 / LPH * U heads of one token, whose angles it needs once.  Memory bounds it: 4095 tokens of 64 + 8 heads of 128, 302 MB, 52.7 us (89 % of the
-// copy rate); 1919 tokens of 64 + 8 + 8 appended, 149 MB, 29.2 us (79 %).  us of the two by U and blocks an SM: 1 x 6 70.2, 36.5; 2 x 4 60.2, 32.1; 2 x 6 63.9, 34.0;
-// 4 x 3 57.5, 31.7; 8 x 2 64.7, 40.0; 4 x 3 with loads that leave L2 first 52.7, 29.2.
+// variant), a warp 32 / LPH * U heads of one token, whose angles it needs once.  Memory bounds it: 4095 tokens of 64 + 8 heads of 128, 302 MB, 53 to 58 us (81 to 89 % of
+// the copy rate); 1919 tokens of 64 + 8 + 8 appended, 149 MB, 29 to 31.5 us (73 to 79 %).  us of the two by U and blocks an SM: 1 x 6 70.2, 36.5; 2 x 4 60.2, 32.1; 2 x 6 63.9, 34.0;
+// 4 x 3 57.5, 31.7; 8 x 2 64.7, 40.0; 4 x 3 with loads that leave L2 first 52.7, 29.2 (the best runs).
 template <int LPH, int U, bool NEOX>
 __global__ void __launch_bounds__(QT, 3) qk_vec_kernel(const QkArgs A) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

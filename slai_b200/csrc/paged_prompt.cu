@@ -18,10 +18,11 @@
 // A region is written again by the third QK after its own; by then the PV that read it is complete: before each PV its issuer waits until the output of the PV
 // before has been read (one region for all of them), so that only the last PV issued can be under way.
 //
-// What bounds it: 1023 tokens of 64 heads on 8 behind 7001 positions, 445 us, 566 TFLOP/s, 1130 executed; the kernel itself 388 us, 1300 executed, where the card's
+// What bounds it: 1023 tokens of 64 heads on 8 behind 7001 positions, 440 us, 572 TFLOP/s, 1140 executed; the kernel itself 388 us, 1300 executed, where the card's
 // power allows 1400 (the clock falls to 1.55 GHz).  A unit of 128 positions takes 5400 cycles for products of 4096: a half's softmax (maximum 500, weights
 // 2000: 16 exponentials a cycle and SM, the wait for tensor memory), its product, the read of that and the next scores are one chain, longer than the other half's
-// products.  Few tokens: 511 of 32 heads 20.6 us in tiles of 128 rows, of which the queries' way to shared memory takes 5, the results' 3 (in tiles of 256: 24.7).
+// products.  Few tokens: 511 of 32 heads 21 us in tiles of 128 rows, of which the queries' way to shared memory takes 5, the results' 3 (in tiles of 256: 24.1).  Registers are
+// short: 180 bytes of spills stored, 404 loaded (heads up to 64: 116 and 180).
 // Descriptors in uniform registers: 464 -> 445 us.  Tried and taken back: a row a thread with twice the registers (chunk 453 us, but 139 for 96 us with 2047 tokens of 32 heads); half of the exponentials by a
 // polynomial (547 for 497); queries by eight lanes a row, in a function of their own or not (the softmax's registers came out worse: 480 to 580).
 //
@@ -555,17 +556,18 @@ int launch(slai_ctx* ctx, const AttnArgs& A, int blocks, bool pdl) {
 Lane paged_prompt_lane(int sms) {
     Lane l;
     l.rows = 2 * PR;
-    // us a call, tiles of 256 / of 128 rows: 32 heads, 256 tokens 18 / 15, 511 25 / 21, 1023 40 / 54; 64 heads on 8 behind 2000, 64 tokens
-    // 35 / 29, 511 82 / 111; 8 heads, 1023 tokens 33 / 26, 2047 43 / 47; 16 heads on 2 behind 1000, 256 tokens 29 / 25, 1023 46 / 52.
+    // us a call, tiles of 256 / of 128 rows: 32 heads, 256 tokens 17.5 / 14.4, 511 24.1 / 21.0, 1023 38 / 53; 64 heads on 8 behind 2000, 64 tokens
+    // 27.5 / 28.4, 511 73 / 109; 8 heads, 1023 tokens 25.2 / 23.5, 2047 38 / 44; 16 heads on 2 behind 1000, 256 tokens 26.2 / 23.7, 1023 45 / 52.  (The better one of each
+    // pair is taken but for 64 tokens of 64 heads.)
     l.low = PR;
-    l.unit_us[0] = 3.4, l.whole_us[0] = 11, l.cut_us[0] = 25;  // (lines through these and longer ones)
+    l.unit_us[0] = 3.4, l.whole_us[0] = 11, l.cut_us[0] = 25;  // (lines through these and longer ones, as they were before the last steps: all some us longer)
     l.unit_us[1] = 2.6, l.whole_us[1] = 12, l.cut_us[1] = 19;
     l.unit = PU;
     l.blocks = sms;
     l.fixed = 13;
     l.each = 0.0223;
     l.least = 1;
-    l.join = 2;  // us a call, cut / not cut where it can be: 32 heads, 511 tokens 32.7 / 28.6, 1023 58 / 46; 64 heads on 8, 511 tokens behind 2000 101 / 81
+    l.join = 2;  // us a call, cut / not cut where it can be: 32 heads, 511 tokens 27.7 / 24.1, 1023 45 / 38; 64 heads on 8, 511 tokens behind 2000 81 / 73
     return l;
 }
 

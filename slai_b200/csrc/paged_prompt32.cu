@@ -13,10 +13,12 @@
 //                Values lie there with a row a dimension: a thread reads four positions of one dimension, a warp's threads next to each other.
 //
 // Barriers: a stage of scores, weights, keys and values has a unit's number's parity; a unit's QK and PV being complete is what frees them.  (The issuer waits for the PV of
-// unit u - 1 before the QK of unit u + 1 takes its stage: paged_order.h.  It costs 1 %, 211 for 208 us: most of it is time in which the next weights were waited for.)
-// 1023 tokens of 32 heads behind 2000 positions 211 us, 199 TFLOP/s, 597 executed, where the card's power sets the clock (1.6 GHz); 37 tokens behind 300 16 us.  (f32 arithmetic
+// unit u - 1 before the QK of unit u + 1 takes its stage: paged_order.h.  It costs 1 % where power sets the clock, 211 for 208 us a call in a loop, and 8 % of
+// one launch under the profiler, 229 for 212.)
+// 1023 tokens of 32 heads behind 2000 positions 211 us, 199 TFLOP/s, 597 executed, where the card's power sets the clock (1.6 GHz); 37 tokens behind 300 15.2 us.  (f32 arithmetic
 // of 64 rows and 32 positions in shared memory: 31 TFLOP/s, 25 us.)
-// What bounds it: 32 positions take 2500 cycles (511 tokens), of which the 44 products take 1960 (1540 at the full rate) and what their issuer waits for between them 540.
+// What bounds it: 32 positions took 2500 cycles (511 tokens) before that wait, of which the 44 products take 1960 (1540 at the full rate) and what their issuer waits for
+// between them 540.
 // Descriptors in uniform registers: 225 -> 208 us.  A thread a row: 209, but 19 for 17 us with few tokens.
 // Tried and taken back: eight more warps for the outputs (251 us: one more hop in the chain); one set of loading warps (257).
 // Every wait is bounded (common.cuh, bounded_wait).
@@ -448,12 +450,12 @@ Lane paged_prompt32_lane(int sms) {
     l.rows = XR;
     l.unit = XU;
     l.blocks = sms;
-    // us a call, units of 64, two at least / of 32, one / of 32, two: 16 heads on 2 behind 2000, 37 tokens 24.3 / 34.2 / 34.0; 32 heads behind 300, 128 tokens
-    // 22.9 / 28.3 / 28.3, 37 tokens 20.9 / 21.0 / 21.0 (three of 64: 26.0).
+    // us a call, units of 64, two at least / of 32, one / of 32, two: 16 heads on 2 behind 2000, 37 tokens 19.4 / 27.6 / 27.6; 32 heads behind 300, 128 tokens
+    // 17.7 / 20.2 / 20.2, 37 tokens 15.3 / 16.6 / 16.5 (three of 64: 17.2).
     l.least = 2;
     l.fixed = 15;
     l.each = 0.007;
-    l.join = 2;  // 32 heads behind 300, 16 tokens: five units whole 20.6 us, cut 17.2
+    l.join = 2;  // 32 heads behind 300, 16 tokens, five units: whole 20.6 us, cut 17.2 (when this was chosen; cut now 14.9)
     return l;
 }
 
